@@ -33,7 +33,7 @@ except ImportError as e:
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpsgemm.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 IN_DTYPE = {"int8": 0, "fp8": 1, "fp16": 2, "bf16": 3, "int4": 6}  # "int4": the MoE stages' int8 x packed-int4 weights
 OUT_DTYPE = {"bf16": 0, "fp16": 1}
@@ -69,6 +69,7 @@ EXPORTS = (
     "psg_moe_topk_gating",
     "psg_moe_softmax_sorting",
     "psg_moe_softmax_sorting_fused",
+    "psg_rmsnorm_quant",
 )
 
 
@@ -228,6 +229,29 @@ class MoeGatingArgs(ctypes.Structure):
     ]
 
 
+class RmsnormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("residual_out", ctypes.c_void_p),
+        ("residual_out_stride", ctypes.c_int64),
+        ("normed", ctypes.c_void_p),
+        ("normed_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("pad0", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -273,7 +297,8 @@ def lib() -> ctypes.CDLL:
     handle.psg_moe_softmax_sorting.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
     handle.psg_moe_softmax_sorting_fused.restype = ctypes.c_int
     handle.psg_moe_softmax_sorting_fused.argtypes = [ctypes.c_int32] * 3
-    for name in ("psg_gemm_a8w8", "psg_gemm_mxfp4", "psg_gemm_a8w8_static", "psg_moe_gemm", "psg_moe_mx_gemm", "psg_moe_sorting", "psg_moe_topk_gating"):
+    for name in ("psg_gemm_a8w8", "psg_gemm_mxfp4", "psg_gemm_a8w8_static", "psg_moe_gemm", "psg_moe_mx_gemm", "psg_moe_sorting", "psg_moe_topk_gating",
+                 "psg_rmsnorm_quant"):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
@@ -311,6 +336,7 @@ def address(name: str) -> int:
 
 TYPE_ANY, TYPE_INT32, TYPE_FP32, TYPE_BF16, TYPE_FP16 = range(5)
 OPTIONAL = 256  # added to a type: None may stand in the operand's place
+ROWS = 512  # added to a type: the operand is [rows, columns] (``rows << 32 | columns`` in the place of the bytes) with dense rows any distance apart, which the struct holds behind the address
 
 
 def operands(*ops) -> bytes:
@@ -346,6 +372,25 @@ def stream_handle(stream) -> int:
     if h is None:
         raise TypeError(f"cannot use {type(stream).__name__} as a stream")
     return int(h)
+
+
+def stream_on(stream, device) -> int:
+    """:func:`stream_handle`, ``None`` being the current stream of ``device`` (whichever device is current)."""
+    if stream is None:
+        import torch
+
+        return int(torch.cuda.current_stream(device).cuda_stream)
+    return stream_handle(stream)
+
+
+def launch_on(device, fn, *args) -> int:
+    """``fn(*args)`` with ``device`` current: a kernel is loaded for and launched on the current device."""
+    import torch
+
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 class WorkspacePool:

@@ -23,10 +23,10 @@ struct Operand {
     int32_t arg;     // which of the call's argument structs
     int32_t offset;  // of the address in it
     int32_t item;    // bytes of an element, 0 = any
-    int32_t type;    // TYPE_*, plus OPTIONAL where None may stand in the operand's place
-    int64_t need;    // least bytes
+    int32_t type;    // TYPE_*, plus OPTIONAL where None may stand in the operand's place, ROWS for one that need not be contiguous
+    int64_t need;    // least bytes; ROWS: rows << 32 | columns, which it has exactly
 };
-enum { TYPE_ANY = 0, TYPE_INT32 = 1, TYPE_FP32 = 2, TYPE_BF16 = 3, TYPE_FP16 = 4, OPTIONAL = 256 };
+enum { TYPE_ANY = 0, TYPE_INT32 = 1, TYPE_FP32 = 2, TYPE_BF16 = 3, TYPE_FP16 = 4, OPTIONAL = 256, ROWS = 512 };
 
 bool type_is(const at::Tensor& t, int type) {
     switch (type) {
@@ -38,11 +38,11 @@ bool type_is(const at::Tensor& t, int type) {
     return true;
 }
 
-// a plain, contiguous device tensor on `device` (-1: on any, which becomes `device`)
-const at::Tensor* operand(PyObject* o, int64_t& device) {
+// a plain device tensor on `device` (-1: on any, which becomes `device`), contiguous unless `strided`
+const at::Tensor* operand(PyObject* o, int64_t& device, bool strided = false) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || !t.is_contiguous()) return nullptr;
+    if (!t.is_cuda() || (!strided && !t.is_contiguous())) return nullptr;
     const int64_t d = t.get_device();
     if (device < 0) device = d;
     return d == device ? &t : nullptr;
@@ -114,8 +114,18 @@ PyObject* launch(PyObject*, PyObject* const* a, Py_ssize_t n) {
             memcpy(&op, PyBytes_AS_STRING(a[2]) + i * (Py_ssize_t)sizeof(op), sizeof(op));
             if (a[4 + i] == Py_None && (op.type & OPTIONAL)) continue;
             if (op.arg < 0 || op.arg >= structs || op.offset < 0 || op.offset + (Py_ssize_t)sizeof(void*) > size[op.arg]) return DECLINED;
-            const at::Tensor* t = operand(a[4 + i], device);
-            if (!t || (op.item && (int64_t)t->element_size() != op.item) || !type_is(*t, op.type & ~OPTIONAL) || t->numel() * (int64_t)t->element_size() < op.need) return DECLINED;
+            const bool rows = op.type & ROWS;
+            const at::Tensor* t = operand(a[4 + i], device, rows);
+            if (!t || (op.item && (int64_t)t->element_size() != op.item) || !type_is(*t, op.type & ~(OPTIONAL | ROWS))) return DECLINED;
+            if (rows) {
+                const int64_t n = op.need >> 32, cols = op.need & 0xFFFFFFFF;
+                if (t->layout() != at::kStrided || t->dim() != 2 || t->size(0) != n || t->size(1) != cols || (cols > 1 && t->stride(1) != 1) || (n > 1 && t->stride(0) < cols)) return DECLINED;
+                const int64_t apart = n > 1 ? t->stride(0) : 0;
+                if (op.offset + 16 > size[op.arg]) return DECLINED;
+                memcpy(arg[op.arg] + op.offset + 8, &apart, sizeof(apart));
+            } else if (t->numel() * (int64_t)t->element_size() < op.need) {
+                return DECLINED;
+            }
             void* p = t->data_ptr();
             memcpy(arg[op.arg] + op.offset, &p, sizeof(p));
         }

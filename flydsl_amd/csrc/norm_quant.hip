@@ -1,0 +1,296 @@
+// Residual addition, root-mean-square norm and per-row quantisation in one pass (gfx950): what stands in front of every quantised product of a
+// decoder layer.
+//
+//   h = round(x + r)                       the residual stream, in the type of x (h = x without a residual)
+//   y = (h w) / sqrt(mean(h^2) + eps)      fp32
+//   s = max|y| / dmax, q = y / s           the rule of k_quant_pertoken: s = 1 for a row of zeros, NaN -> 0, +-Inf -> +-dmax, int8 towards zero, fp8 to nearest even
+//
+// The norm is of the rounded h, so that it is the norm of what the layers behind read as residual; q is made of y, not of its 16-bit rounding.
+// One pass: the maximum does not need the norm, max|y| = max|h w| / rms with the same rounding (a product with a positive factor is monotone), so the sum of squares and
+// the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
+// like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
+// Bound: HBM; every operand is read once and every output written once.
+#include "psg_common.h"
+#include "quant_rows.h"
+#include "norm_quant.h"
+
+namespace {
+
+// 16-byte pieces at any address that is a multiple of the element (global accesses of this target need no more)
+typedef v4i v4i_any __attribute__((aligned(2)));  // (fp32 elements are on 4 bytes)
+typedef v2i v2i_any __attribute__((aligned(1)));
+
+// Elements [i, i + 8) as they are stored; from `n` on they read as zero
+template <int XT, bool WHOLE>
+__device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n) {
+    constexpr int B = XT == X_F32 ? 4 : 2;
+    Raw8<XT> r;
+    if (WHOLE || n >= 8) {
+        const v4i_any* p = reinterpret_cast<const v4i_any*>(static_cast<const uint8_t*>(base) + i * B);
+        r.w[0] = p[0];
+        if constexpr (XT == X_F32) r.w[1] = p[1];
+    } else {
+#pragma unroll
+        for (int k = 0; k < (XT == X_F32 ? 2 : 1); k++) r.w[k] = (v4i){0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) {
+                if constexpr (XT == X_F32) r.w[e >> 2][e & 3] = static_cast<const int*>(base)[i + e];
+                else r.w[0][e >> 1] |= (int)((uint32_t)static_cast<const uint16_t*>(base)[i + e] << (16 * (e & 1)));
+            }
+    }
+    return r;
+}
+
+template <int XT, bool WHOLE>
+__device__ __forceinline__ void store_row(void* base, int64_t i, int n, const Raw8<XT>& r) {
+    constexpr int B = XT == X_F32 ? 4 : 2;
+    if (WHOLE || n >= 8) {
+        v4i_any* p = reinterpret_cast<v4i_any*>(static_cast<uint8_t*>(base) + i * B);
+        p[0] = r.w[0];
+        if constexpr (XT == X_F32) p[1] = r.w[1];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) {
+                if constexpr (XT == X_F32) static_cast<int*>(base)[i + e] = r.w[e >> 2][e & 3];
+                else static_cast<uint16_t*>(base)[i + e] = (uint16_t)((uint32_t)r.w[0][e >> 1] >> (16 * (e & 1)));
+            }
+    }
+}
+
+// eight values rounded to the type of x
+template <int XT>
+__device__ __forceinline__ Raw8<XT> round8(const float* v) {
+    Raw8<XT> r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (XT == X_F32) {
+            r.w[i >> 1][2 * (i & 1)] = __float_as_int(v[2 * i]);
+            r.w[i >> 1][2 * (i & 1) + 1] = __float_as_int(v[2 * i + 1]);
+        } else {
+            r.w[0][i] = pack2_out16<XT == X_BF16 ? OUT_BF16 : OUT_FP16>(v[2 * i], v[2 * i + 1]);
+        }
+    }
+    return r;
+}
+
+// v d / m rounded once, for m inside the bounds of quotient() and |v| <= m: its correction steps on the whole product.  SHORT: the product is exact (8 + 8 bits of a bf16
+// value and weight and 7 of d).
+template <bool SHORT>
+__device__ __forceinline__ float times_over(float v, float d, float m, float rm) {
+    const float hi = v * d;
+    if constexpr (SHORT) return quotient(hi, m, rm);
+    const float lo = __builtin_fmaf(v, d, -hi);
+    float q = hi * rm;
+    q = __builtin_fmaf(__builtin_fmaf(-q, m, hi) + lo, rm, q);
+    q = __builtin_fmaf(__builtin_fmaf(-q, m, hi) + lo, rm, q);
+    return __builtin_copysignf(q, v);
+}
+
+// A row belongs to NT threads: one wavefront (four rows a workgroup, no barrier) or a workgroup.  The first KEEP 8-element vectors of every thread stay in registers; a
+// longer row writes its h, or has it in x, and reads the rest of it once more, every thread what it has written itself.
+// WHOLE: rows are whole vectors.  WT: type of the weight.
+template <int XT, int WT, int NT, int KEEP, bool WHOLE>
+__global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParams p) {
+    __shared__ float red_s[NT / 64];
+    __shared__ uint32_t red_m[NT / 64];
+    const int wave = wave_id();
+    const int64_t row = NT == 64 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+    if (NT == 64 && row >= p.rows) return;  // a whole wavefront; no barrier follows
+    const int tid = NT == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+    const int nvec = (p.dim + 7) >> 3;
+    const int64_t xb = row * p.x_stride, rb = row * p.r_stride, hb = row * p.h_stride, nb = row * p.n_stride, qb = row * (int64_t)p.dim;
+    auto left = [&](int vi) { return p.dim - vi * 8; };
+    auto weights = [&](int vi) __attribute__((always_inline)) { return load_row<WT, WHOLE>(p.weight, (int64_t)vi * 8, left(vi)); };
+
+    float sum = 0.f, hw[KEEP][8];
+    uint32_t mb = 0;
+    // adds a vector's squares and its maximum, as h w with its sign dropped, on the bit patterns: NaN above Inf above every finite value
+    auto take = [&](const float* h, const float* w, float* out) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            sum = __builtin_fmaf(h[e], h[e], sum);
+            out[e] = h[e] * w[e];
+            const uint32_t u = __builtin_bit_cast(uint32_t, out[e]) & 0x7FFFFFFFu;
+            mb = u > mb ? u : mb;
+        }
+    };
+    auto add = [&](const Raw8<XT>& x, const Raw8<XT>& r, int vi, bool live, float* h) __attribute__((always_inline)) {
+        x.values(h);
+        if (p.residual) {
+            float v[8];
+            r.values(v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = h[e] + v[e];
+            const Raw8<XT> k = round8<XT>(v);
+            k.values(h);
+            if (live) store_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi), k);
+        }
+    };
+
+    {
+        // threads past the row read its first vector again: no load stands behind a branch of its own
+        Raw8<XT> x[KEEP], r[KEEP];
+        Raw8<WT> w[KEEP];
+        auto at = [&](int it) { return tid + it * NT < nvec ? tid + it * NT : 0; };
+#pragma unroll
+        for (int it = 0; it < KEEP; it++) r[it] = x[it] = load_row<XT, WHOLE>(p.x, xb + (int64_t)at(it) * 8, left(at(it)));
+        if (p.residual) {
+#pragma unroll
+            for (int it = 0; it < KEEP; it++) r[it] = load_row<XT, WHOLE>(p.residual, rb + (int64_t)at(it) * 8, left(at(it)));
+        }
+#pragma unroll
+        for (int it = 0; it < KEEP; it++) w[it] = weights(at(it));
+#pragma unroll
+        for (int it = 0; it < KEEP; it++) {
+            const bool live = tid + it * NT < nvec;
+            float h[8], wv[8];
+            add(x[it], r[it], tid + it * NT, live, h);
+            w[it].values(wv);
+            if (!live) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) h[e] = wv[e] = 0.f;
+            }
+            take(h, wv, hw[it]);
+        }
+    }
+    for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
+        const Raw8<XT> x = load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi));
+        const Raw8<XT> r = p.residual ? load_row<XT, WHOLE>(p.residual, rb + (int64_t)vi * 8, left(vi)) : x;
+        float w[8], h[8], y[8];
+        weights(vi).values(w);
+        add(x, r, vi, true, h);
+        take(h, w, y);
+    }
+
+    auto over_row = [&](float& s, uint32_t& m) __attribute__((always_inline)) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            s += __shfl_xor(s, off, 64);
+            const uint32_t o = (uint32_t)__shfl_xor((int)m, off, 64);
+            m = o > m ? o : m;
+        }
+        if constexpr (NT > 64) {
+            if ((tid & 63) == 0) red_s[wave] = s, red_m[wave] = m;
+            __syncthreads();
+            s = red_s[0], m = red_m[0];
+#pragma unroll
+            for (int i = 1; i < NT / 64; i++) {
+                s += red_s[i];
+                m = red_m[i] > m ? red_m[i] : m;
+            }
+        }
+    };
+    over_row(sum, mb);
+    const float rinv = 1.0f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+
+    // h w of a vector that is not in registers
+    auto again = [&](int vi, float* v) __attribute__((always_inline)) {
+        float w[8];
+        (p.residual ? load_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi)) : load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi))).values(v);
+        weights(vi).values(w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= w[e];
+    };
+
+    const float dmax = p.out == NORM_FP8 ? 448.0f : 127.0f;
+    float s = 1.0f;
+    const float mhw = __builtin_bit_cast(float, mb);
+    const float rm = 1.0f / mhw;
+    bool exact = true;  // no value needs cleaning, and the maximum lies where quotient() is exact; uniform over the row
+    if (p.out != NORM_NONE) {
+        float amax = mhw * rinv;
+        const bool special = !(amax < __builtin_inff());  // an Inf or NaN among the row's values, or a norm that is none
+        if (special) {
+            float m = 0.f, unused = 0.f;
+#pragma unroll
+            for (int it = 0; it < KEEP; it++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(clean(hw[it][e] * rinv, dmax)));
+            for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
+                float v[8];
+                again(vi, v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(clean(v[e] * rinv, dmax)));
+            }
+            uint32_t bits = __builtin_bit_cast(uint32_t, m);
+            if constexpr (NT > 64) __syncthreads();  // everybody has read what over_row left
+            over_row(unused, bits);
+            amax = __builtin_bit_cast(float, bits);
+        }
+        s = amax / dmax;
+        if (s == 0.0f) s = 1.0f;
+        if (tid == 0) p.scale[row] = s;
+        exact = !special && s >= 0x1p-80f && s <= 0x1p100f && mhw >= 0x1p-80f && mhw <= 0x1p100f;
+    }
+    auto finish = [&](int vi, const float* v) __attribute__((always_inline)) {
+        const int n = left(vi);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = v[e] * rinv;
+        if (p.normed) store_row<XT, WHOLE>(p.normed, nb + (int64_t)vi * 8, n, round8<XT>(y));
+        if (p.out == NORM_NONE) return;
+        if (exact) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = times_over<XT == X_BF16 && WT == X_BF16>(v[e], dmax, mhw, rm);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = clean(y[e], dmax) / s;
+        }
+        const v2i o = p.out == NORM_FP8 ? quant_pack8<1>(y) : quant_pack8<0>(y);
+        uint8_t* dst = p.q + qb + (int64_t)vi * 8;
+        if (WHOLE || n >= 8) {
+            *reinterpret_cast<v2i_any*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < n) dst[e] = (uint8_t)((uint32_t)o[e >> 2] >> (8 * (e & 3)));
+        }
+    };
+#pragma unroll
+    for (int it = 0; it < KEEP; it++) {
+        const int vi = tid + it * NT;
+        if (vi < nvec) finish(vi, hw[it]);
+    }
+    for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
+        float v[8];
+        again(vi, v);
+        finish(vi, v);
+    }
+}
+
+template <int XT, int WT, bool WHOLE>
+hipError_t launch(const NormParams& p, hipStream_t stream) {
+    const int nvec = (p.dim + 7) / 8;
+#define PSG_NORM(NT_, KEEP_)                                                                                                                     \
+    {                                                                                                                                            \
+        hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, NT_, KEEP_, WHOLE>), dim3(NT_ == 64 ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows), dim3(NT_ == 64 ? 256 : NT_), 0, stream, p); \
+        return hipGetLastError();                                                                                                                \
+    }
+    if (nvec <= 256 && p.rows >= 8 * psg_cu_count()) {
+        if (nvec <= 64) PSG_NORM(64, 1)
+        PSG_NORM(64, 4)
+    }
+    if (nvec <= 256) PSG_NORM(256, 1)
+    if (nvec <= 512) PSG_NORM(256, 2)
+    if (nvec <= 1024) PSG_NORM(256, 4)
+    PSG_NORM(1024, 4)
+#undef PSG_NORM
+}
+
+}  // namespace
+
+// x_dtype: 0 fp32, 1 bf16, 2 fp16.  Requires rows, dim >= 1 and addresses that are multiples of their elements.
+hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream) {
+    // (rows that begin off 16 bytes cost what their lines cost; what WHOLE spares is the code for the end of a row)
+    const bool whole = p.dim % 8 == 0;
+#define PSG_NORM_T(XT_, WT_) return whole ? launch<XT_, WT_, true>(p, stream) : launch<XT_, WT_, false>(p, stream);
+    switch (x_dtype) {
+        case X_F32: PSG_NORM_T(X_F32, X_F32)
+        case X_BF16: if (p.w_f32) PSG_NORM_T(X_BF16, X_F32) else PSG_NORM_T(X_BF16, X_BF16)
+        case X_F16: if (p.w_f32) PSG_NORM_T(X_F16, X_F32) else PSG_NORM_T(X_F16, X_F16)
+    }
+#undef PSG_NORM_T
+    return hipErrorInvalidValue;
+}

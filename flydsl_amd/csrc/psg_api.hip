@@ -11,6 +11,7 @@
 #include "psg_common.h"
 #include "moe_gating.h"
 #include "moe_rows.h"
+#include "norm_quant.h"
 #include "tile_order.h"
 
 hipError_t psg_launch_a8w8_tiled(const A8W8Params& p, int kind, int store, int tile_m, int tile_n, hipStream_t stream);
@@ -38,6 +39,7 @@ hipError_t psg_launch_tile_order(int tiles_m, int tiles_n, int group_m, int32_t*
 hipError_t psg_launch_quant_pertoken(const void* x, int x_dtype, void* y, float* scale, int M, int K, int out_fp8, hipStream_t stream);
 hipError_t psg_launch_quant_mxfp4(const void* x, int x_dtype, void* packed, void* scales, int M, int R, int K, int shuffled,
                                   hipStream_t stream);
+hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream);
 
 // Scratch of the entry point that allocates nothing (psg_gemm_a8w8_static): the split-K partial sums of the tiled
 // path live here instead of in a caller-supplied workspace.  Every GPU the library runs on holds its own copy of the
@@ -1311,6 +1313,44 @@ int psg_quant_mxfp4(const void* x, int32_t x_dtype, void* packed, void* scales, 
     const int R = (M + 31) / 32 * 32;  // scales cover whole 32-row chunks; the padding rows get scale byte 0
     const hipError_t e = psg_launch_quant_mxfp4(x, x_dtype, packed, scales, M, R, K, shuffled, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_quant_mxfp4 launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_rmsnorm_quant(const psg_rmsnorm_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (a->x_dtype < 0 || a->x_dtype > 2) return fail(PSG_E_DTYPE, "x_dtype %d unknown (0 fp32, 1 bf16, 2 fp16)", a->x_dtype);
+    if (a->weight_dtype != 0 && a->weight_dtype != a->x_dtype) return fail(PSG_E_DTYPE, "weight_dtype %d must be fp32 or that of x (%d)", a->weight_dtype, a->x_dtype);
+    if (a->out_dtype != PSG_IN_INT8 && a->out_dtype != PSG_IN_FP8_E4M3FN && a->out_dtype != -1) return fail(PSG_E_DTYPE, "out_dtype must be int8, fp8 or -1 (none)");
+    if (a->rows < 0 || a->rows > 0x7FFFFFFF) return fail(PSG_E_SHAPE, "rows=%lld outside [0, 2^31)", (long long)a->rows);
+    if (a->dim < 1 || a->dim > (1 << 24)) return fail(PSG_E_SHAPE, "dim=%d outside [1, 2^24]", a->dim);
+    if (!(a->eps >= 0.0f) || std::isinf(a->eps)) return fail(PSG_E_SHAPE, "eps must be finite and not negative");
+    const bool quant = a->out_dtype != -1;
+    if (a->rows == 0) {
+        g_err[0] = 0;
+        return 0;
+    }
+    if (!a->x || !a->weight) return fail(PSG_E_NULL, "x and weight must be non-NULL");
+    if (quant ? !a->q || !a->scale : !a->normed) return fail(PSG_E_NULL, quant ? "q and scale must be non-NULL" : "normed must be non-NULL without a quantised output");
+    if (a->residual && !a->residual_out) return fail(PSG_E_NULL, "residual_out must be non-NULL with a residual");
+    const int64_t strides[4] = {a->x_stride, a->residual_stride, a->residual_out_stride, a->normed_stride};
+    int64_t s[4];
+    for (int i = 0; i < 4; i++) {
+        s[i] = strides[i] ? strides[i] : a->dim;
+        if (s[i] < a->dim || s[i] > (1ll << 40)) return fail(PSG_E_SHAPE, "a row stride of %lld elements is below dim=%d or beyond 2^40", (long long)strides[i], a->dim);
+    }
+    const int eb = a->x_dtype == 0 ? 4 : 2, wb = a->weight_dtype == 0 ? 4 : 2;
+    if (!aligned(a->x, eb) || !aligned(a->residual, eb) || !aligned(a->residual_out, eb) || !aligned(a->normed, eb) || !aligned(a->weight, wb) || !aligned(a->scale, 4))
+        return fail(PSG_E_ALIGN, "every operand must be aligned to its elements");
+    NormParams p = {};
+    p.x = a->x, p.residual = a->residual, p.weight = a->weight, p.h = a->residual_out, p.normed = a->normed;
+    p.q = static_cast<uint8_t*>(a->q), p.scale = a->scale;
+    p.x_stride = s[0], p.r_stride = s[1], p.h_stride = s[2], p.n_stride = s[3];
+    p.rows = a->rows, p.dim = a->dim, p.eps = a->eps;
+    p.w_f32 = a->weight_dtype == 0;
+    p.out = !quant ? NORM_NONE : a->out_dtype == PSG_IN_FP8_E4M3FN ? NORM_FP8 : NORM_INT8;
+    const hipError_t e = psg_launch_rmsnorm_quant(p, a->x_dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_rmsnorm_quant launch");
     g_err[0] = 0;
     return 0;
 }

@@ -5,6 +5,8 @@ without leaving the GPU.  torch is used for the output allocations only."""
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -92,3 +94,117 @@ def per_1x32_f4_quant(x: torch.Tensor, shuffle: bool = True, stream=None, out=No
     if rc:
         _lib.check(rc, "psg_quant_mxfp4")
     return packed if packed.dtype == fp4x2 else packed.view(fp4x2), scales if scales.dtype == fp8_e8m0 else scales.view(fp8_e8m0)
+
+
+_norm_plans = {}  # what shapes and types alone decide about a call of rmsnorm_quant, by them
+
+
+def _norm_row_stride(name, t, x):
+    """Elements from a row of ``t`` to the next; ``t`` has the shape, type and device of ``x`` and dense rows."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{name} must be a {tuple(x.shape)} {x.dtype} tensor on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must have dense rows that do not overlap (strides {tuple(t.stride())})")
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _norm_args(x, weight, eps, quant_dtype):
+    """The argument struct of a call, without its addresses and strides."""
+    if quant_dtype is not None and quant_dtype not in _OUT_CODE:
+        raise ValueError(f"quant_dtype must be torch.int8, torch.float8_e4m3fn or None, got {quant_dtype}")
+    if not isinstance(x, torch.Tensor) or x.dtype not in _X_DTYPE:
+        raise TypeError(f"x must be a tensor of fp32, bf16 or fp16, got {getattr(x, 'dtype', type(x).__name__)}")
+    if not x.is_cuda or x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("x must be a 2-D device tensor with at least one column")
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in (x.dtype, torch.float32) or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+        raise ValueError(f"weight must hold {x.shape[1]} elements of {x.dtype} or fp32")
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    a = _lib.RmsnormArgs()
+    a.rows, a.dim = x.shape
+    a.x_dtype, a.weight_dtype = _X_DTYPE[x.dtype], _X_DTYPE[weight.dtype]
+    a.out_dtype = -1 if quant_dtype is None else _OUT_CODE[quant_dtype]
+    a.eps = eps
+    return a
+
+
+def _norm_plan(x, weight, eps, quant_dtype):
+    a = _norm_args(x, weight, eps, quant_dtype)
+    f, any_, rows, dim, eb = _lib.RmsnormArgs, _lib.TYPE_ANY, a.rows, a.dim, x.element_size()
+    typed = {torch.float32: _lib.TYPE_FP32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16}
+    xt, size, optional = typed[x.dtype] + _lib.ROWS, rows << 32 | dim, _lib.OPTIONAL
+    ops = _lib.operands((f.x, eb, xt, size), (f.weight, weight.element_size(), typed[weight.dtype], dim * weight.element_size()), (f.residual, eb, xt + optional, size),
+                        (f.residual_out, eb, xt + optional, size), (f.normed, eb, xt + optional, size), (f.q, 1, any_, rows * dim), (f.scale, 4, _lib.TYPE_FP32, 4 * rows))
+    return (bytes(a),), ops
+
+
+def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None, quant_dtype=torch.float8_e4m3fn,
+                  residual_out: torch.Tensor | None = None, normed: torch.Tensor | None = None, stream=None, out=None):
+    """Residual addition, root-mean-square norm and per-row quantisation in one launch: what a decoder layer has in front of its quantised
+    products.
+
+    ``h = x + residual``, rounded to the type of ``x`` and written to ``residual_out`` (``None``: to ``residual`` itself); ``h = x`` without a residual.
+    ``y = h * weight / sqrt(mean(h^2) + eps)`` in fp32, written to ``normed`` in the type of ``x`` where one is given (what a router or an unquantised layer reads).
+    Returns ``(q [rows, dim] quant_dtype, scale [rows, 1] fp32)`` by the rules of :func:`pertoken_quant` (``scale`` 1 for a row of zeros, NaN as 0, infinities as the largest
+    value, int8 towards zero), but from ``y`` before it is rounded; with ``quant_dtype=None`` the norm alone, and ``normed`` (allocated if it is ``None``) is returned.
+
+    ``x``, ``residual``, ``residual_out`` and ``normed`` are ``[rows, dim]`` of one type (fp32 / bf16 / fp16), each with dense rows any distance apart (a slice of the
+    columns of a wider tensor will do); ``weight`` ``[dim]`` has that type or fp32.  ``residual_out`` may be ``residual`` or ``x``, ``normed`` may be ``x``.  ``rows`` may be
+    0, and ``dim`` any number.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
+    the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
+    # a call with its outputs, on the current device, goes on in native code, which looks at the operands
+    if stream is not None and type(out) in (tuple, list) and len(out) == 2 and type(x) is type(weight) is torch.Tensor and x.is_cuda and x.dim() == 2:
+        q, scale = out
+        h = residual if residual_out is None else residual_out
+        if type(q) is type(scale) is torch.Tensor and q.shape == x.shape and scale.numel() == x.shape[0] and quant_dtype is not None and (
+                residual is not None or h is None) and x.get_device() == torch.cuda.current_device():
+            key = (x.shape, x.dtype, weight.shape, weight.dtype, eps, quant_dtype)
+            plan = _norm_plans.get(key)
+            if plan is None:
+                if len(_norm_plans) >= 256:
+                    _norm_plans.clear()
+                plan = _norm_plans[key] = _norm_plan(x, weight, eps, quant_dtype)
+            rc = _lib._native.launch(_lib.address("psg_rmsnorm_quant"), plan[0], plan[1], stream, x, weight, residual, h, normed, q, scale)
+            if rc != _lib._native.DECLINED:
+                if rc:
+                    _lib.check(rc, "psg_rmsnorm_quant")
+                return q if q.dtype == quant_dtype else q.view(quant_dtype), scale if scale.dim() == 2 and scale.shape[1] == 1 else scale.view(-1, 1)
+    a = _norm_args(x, weight, eps, quant_dtype)
+    rows, dim = x.shape
+    if weight.device != x.device or not weight.is_contiguous():
+        raise ValueError("weight must be contiguous and on the device of x")
+    a.x_stride = _norm_row_stride("x", x, x)
+    a.x, a.weight = x.data_ptr(), weight.data_ptr()
+    if residual is not None:
+        h = residual if residual_out is None else residual_out
+        a.residual_stride, a.residual_out_stride = _norm_row_stride("residual", residual, x), _norm_row_stride("residual_out", h, x)
+        a.residual, a.residual_out = residual.data_ptr(), h.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out is given without a residual")
+    q = scale = None
+    if quant_dtype is None:
+        if out is not None:
+            raise ValueError("out is given with quant_dtype=None: the result is normed")
+        if normed is None:
+            normed = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
+    elif out is None:
+        q, scale = torch.empty((rows, dim), dtype=quant_dtype, device=x.device), torch.empty((rows, 1), dtype=torch.float32, device=x.device)
+    else:
+        q, scale = out
+        _check_out(x, q, scale)
+        if q.shape != x.shape or q.element_size() != 1 or scale.numel() != rows or scale.dtype != torch.float32:
+            raise ValueError("out must be (1-byte [rows, dim], fp32 [rows] or [rows, 1]) tensors")
+    if normed is not None:
+        a.normed_stride = _norm_row_stride("normed", normed, x)
+        a.normed = normed.data_ptr()
+    if q is not None:
+        a.q, a.scale = q.data_ptr(), scale.data_ptr()
+    rc = _lib.launch_on(x.device, _lib.lib().psg_rmsnorm_quant, ctypes.byref(a), _lib.stream_on(stream, x.device))
+    if rc:
+        _lib.check(rc, "psg_rmsnorm_quant")
+    if q is None:
+        return normed
+    return q if q.dtype == quant_dtype else q.view(quant_dtype), scale if scale.shape == (rows, 1) else scale.view(rows, 1)

@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define PSG_ABI_VERSION 7
+#define PSG_ABI_VERSION 8
 
 /* input element types of A and B */
 enum psg_in_dtype { PSG_IN_INT8 = 0, PSG_IN_FP8_E4M3FN = 1, PSG_IN_FP16 = 2, PSG_IN_BF16 = 3,
@@ -452,6 +452,39 @@ int psg_moe_topk_gating(const psg_moe_gating_args *args, void *stream);
  * sort->topk_weights gating->weights (both non-NULL). */
 int psg_moe_softmax_sorting_fused(int32_t tokens, int32_t topk, int32_t experts);
 int psg_moe_softmax_sorting(const psg_moe_gating_args *gating, const psg_moe_sort_args *sort, void *stream);
+
+/*
+ * Residual addition, root-mean-square norm and per-row quantisation in one pass: what stands in front of a quantised product.
+ *   h = x + residual, rounded to the type of x and written to residual_out (h = x with residual NULL; residual_out is then not used)
+ *   y = h * weight / sqrt(mean(h^2) + eps), fp32; normed NULL or y rounded to the type of x
+ *   scale = max|y| / qmax (qmax 448 or 127; 1 for a row of zeros), q = y / scale by the rules of psg_quant_pertoken (NaN -> 0, +-Inf -> +-qmax, int8 towards zero, fp8
+ *   to nearest even), from y before its rounding to fp32
+ * x, residual, residual_out and normed are rows of dim elements, a stride of elements (0 = dim, and at least dim) apart, at addresses and strides that need only be
+ * multiples of an element; q [rows, dim] is dense, scale [rows].  residual_out may be residual or x, normed may be x: every element is read before it is
+ * written.  Other overlaps are not allowed.
+ * x_dtype 0 = fp32, 1 = bf16, 2 = fp16 (the numbering of the quantisers); weight_dtype x_dtype or 0; out_dtype PSG_IN_INT8, PSG_IN_FP8_E4M3FN or -1: no q and scale
+ * (normed is then required).  rows = 0 launches nothing.  dim <= 2^24, eps >= 0.
+ */
+typedef struct psg_rmsnorm_args {
+    const void *x;
+    int64_t x_stride;
+    const void *residual;
+    int64_t residual_stride;
+    void *residual_out;
+    int64_t residual_out_stride;
+    void *normed;
+    int64_t normed_stride;
+    const void *weight;
+    void *q;
+    float *scale;
+    int64_t rows;
+    int32_t dim;
+    int32_t x_dtype, weight_dtype, out_dtype;
+    float eps;
+    int32_t pad0; /* 0 */
+} psg_rmsnorm_args;
+
+int psg_rmsnorm_quant(const psg_rmsnorm_args *args, void *stream);
 
 #ifdef __cplusplus
 }

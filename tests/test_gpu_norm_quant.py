@@ -1,0 +1,205 @@
+"""GPU tests of the norm with quantised rows against its definition in 64 bits.
+
+Tolerances, in units of u = 2^-24 (half a step of fp32): all squares are positive, so their sum is off by at most as many u as a chain of additions is long.  A thread adds at
+most dim / 64 squares one after the other (one wavefront a row; fewer with more threads), then come 6 exchanges and up to 16 partial sums; the mean, the root, the reciprocal and
+two products add at most 8.  The root halves what was before it.  So y and the scale are within (dim / 64 + 40) u relatively, and every output within that and its own rounding.
+"""
+
+import pytest
+import torch
+
+from flydsl_amd import quant_device
+
+pytestmark = pytest.mark.gpu
+FP8 = torch.float8_e4m3fn
+QMAX = {FP8: 448.0, torch.int8: 127.0}
+STEP = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}  # half a step, relative
+
+
+def _inputs(rows, dim, dt, residual, seed, wt=None):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(rows, dim, generator=g) * (1 + 30 * (torch.rand(dim, generator=g) < 0.01))).to(dt)
+    w = (1 + 0.3 * torch.randn(dim, generator=g)).to(wt or dt)
+    r = (3 * torch.randn(rows, dim, generator=g)).to(dt) if residual else None
+    return x.cuda(), w.cuda(), None if r is None else r.cuda()
+
+
+def _exact(x, w, r, eps, qd):
+    h = x if r is None else (x.float() + r.float()).to(x.dtype)
+    d = h.double()
+    y = d * w.double() / (d.square().mean(-1, keepdim=True) + eps).sqrt()
+    s = y.abs().amax(-1, keepdim=True) / QMAX[qd] if qd is not None else None
+    if s is not None:
+        s = torch.where(s == 0, torch.ones_like(s), s)
+    return h, y, s
+
+
+def _check(x, w, r, eps, qd, q, scale, h_out, normed):
+    h, y, s = _exact(x, w, r, eps, qd)
+    tol = (x.shape[1] / 64 + 40) * 2.0**-24
+    if r is not None:
+        assert torch.equal(h_out, h)
+    if normed is not None:
+        # (below the normal range a rounding is off by half a smallest step)
+        tiny = torch.finfo(x.dtype).tiny * 2 * STEP[x.dtype]
+        assert ((normed.double() - y).abs() <= (STEP[x.dtype] * (1 + tol) + tol) * y.abs() + tiny).all()
+    if qd is None:
+        return
+    assert scale.shape == (x.shape[0], 1) and scale.dtype == torch.float32
+    assert ((scale.double() - s).abs() <= tol * s).all()
+    want = y / s
+    off = (q.to(torch.float64) - want).abs()
+    assert (q.to(torch.float64).abs().amax(-1) == torch.where(y.abs().amax(-1) == 0, 0.0, QMAX[qd])).all()  # the maximum of a row is the largest value
+    slack = 4 * 2.0**-24 * want.abs()  # the norm cancels in y / s: a product with the weight, one with the largest value, the quotient
+    if qd == FP8:
+        assert (off <= torch.clamp(2.0**-4 * (want.abs() + slack), min=2.0**-10) + slack).all()
+    else:  # towards zero
+        assert (off < 1 + slack).all() and (q.double().abs() <= want.abs() + slack).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 7), (1, 64), (2, 2051), (67, 4096), (2100, 512), (2049, 1543), (5, 8192), (3, 8200), (2, 33003), (1, 70000)])
+def test_against_the_definition(rows, dim, dt):
+    for residual, qd in ((True, FP8), (False, torch.int8)):
+        x, w, r = _inputs(rows, dim, dt, residual, seed=rows * 7 + dim)
+        keep = None if r is None else r.clone()
+        normed = torch.empty_like(x)
+        q, s = quant_device.rmsnorm_quant(x, w, 1e-5, residual=r, quant_dtype=qd, normed=normed)
+        _check(x, w, keep, 1e-5, qd, q, s, r, normed)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_weight_in_fp32_and_norm_alone(dt):
+    x, w, r = _inputs(33, 1000, dt, True, seed=4, wt=torch.float32)
+    h = torch.empty_like(x)
+    y = quant_device.rmsnorm_quant(x, w, 1e-6, residual=r, residual_out=h, quant_dtype=None)
+    _check(x, w, r, 1e-6, None, None, None, h, y)
+    q, s = quant_device.rmsnorm_quant(x, w, 1e-6, quant_dtype=torch.int8)
+    _check(x, w, None, 1e-6, torch.int8, q, s, None, None)
+
+
+@pytest.mark.parametrize("qd", [FP8, torch.int8])
+@pytest.mark.parametrize("dim", [5, 256, 2056, 9000, 40008])
+def test_special_rows_as_the_quantiser_has_them(dim, qd):
+    """Rows of zeros, NaN and infinities, tiny and huge ones, against the quantiser on the fp32 rows that the norm wrote: the same bytes, and in the ordinary rows, whose
+    values are divided before their rounding here, at most one step beside it."""
+    x, w, _ = _inputs(40, dim, torch.float32, False, seed=dim)
+    x[1] = 0
+    x[2, dim // 2] = float("nan")
+    x[3, dim - 1] = float("inf")
+    x[4] *= 1e-30
+    x[5] *= 1e15
+    x[6, 0] = -float("inf")
+    w[dim // 3] = 0
+    normed = torch.empty_like(x)
+    for eps in (1e-6, 0.0):
+        q, s = quant_device.rmsnorm_quant(x, w, eps, quant_dtype=qd, normed=normed)
+        pad = torch.nn.functional.pad(normed, (0, -dim % 8))  # (the quantiser wants multiples of 8; zeros change nothing)
+        q2, s2 = quant_device.pertoken_quant(pad, quant_dtype=qd)
+        assert torch.equal(s, s2)
+        q2 = q2[:, :dim]
+        odd = [1, 2, 3, 4, 6]
+        assert torch.equal(q.view(torch.uint8)[odd], q2.view(torch.uint8)[odd])
+        a, b = q.float(), q2.float()
+        assert ((a - b).abs() <= torch.clamp(2.0**-3 * b.abs(), min=2.0**-9) if qd == FP8 else (a - b).abs() <= 1).all()
+    bad = torch.ones(dim, device="cuda")
+    bad[0] = float("inf")  # an infinite weight: that column saturates, the others stay
+    q, s = quant_device.rmsnorm_quant(x, bad, 1e-6, quant_dtype=qd, normed=normed)
+    q2, s2 = quant_device.pertoken_quant(torch.nn.functional.pad(normed, (0, -dim % 8)), quant_dtype=qd)
+    assert torch.equal(s, s2) and torch.equal(q.view(torch.uint8), q2.view(torch.uint8)[:, :dim])
+    assert (q[:3, 0].float() == 0).sum() == 2 and q[0, 0].float().abs() == QMAX[qd]
+
+
+def test_slices_of_wider_tensors_and_rows_in_place():
+    rows, dim = 50, 1027
+    x, w, r = _inputs(rows, dim, torch.bfloat16, True, seed=1)
+    wide = {k: torch.full((rows, dim + 29), 7.0, dtype=torch.bfloat16, device="cuda") for k in ("x", "r", "h", "n")}
+    wide["x"][:, 3 : 3 + dim], wide["r"][:, 11 : 11 + dim] = x, r
+    v = {k: t[:, o : o + dim] for (k, t), o in zip(wide.items(), (3, 11, 5, 0))}
+    q, s = quant_device.rmsnorm_quant(v["x"], w, residual=v["r"], residual_out=v["h"], normed=v["n"])
+    _check(x, w, r, 1e-6, FP8, q, s, v["h"], v["n"])
+    assert torch.equal(v["x"], x) and torch.equal(v["r"], r)
+    for k, o in zip(wide, (3, 11, 5, 0)):  # nothing beside the slices
+        assert (wide[k][:, :o] == 7).all() and (wide[k][:, o + dim :] == 7).all()
+    # the sum in place of the residual or of x, the norm in place of x: also where a row is longer than what the registers hold
+    for d in (dim, 41000):
+        x, w, r = _inputs(4, d, torch.float16, True, seed=2)
+        a, b = x.clone(), r.clone()
+        q, s = quant_device.rmsnorm_quant(a, w, residual=b, normed=a)
+        _check(x, w, r, 1e-6, FP8, q, s, b, a)
+        a = x.clone()
+        q, s = quant_device.rmsnorm_quant(a, w, residual=r, residual_out=a)
+        _check(x, w, r, 1e-6, FP8, q, s, a, None)
+        a = x.clone()
+        q, s = quant_device.rmsnorm_quant(a, w, normed=a)
+        _check(x, w, None, 1e-6, FP8, q, s, None, a)
+
+
+def test_rows_far_apart():
+    """Offsets of rows beyond 32 bits."""
+    far = torch.empty(3 * 1_300_000_000, dtype=torch.bfloat16, device="cuda").as_strided((3, 264), (1_300_000_000, 1))
+    x, w, _ = _inputs(3, 264, torch.bfloat16, False, seed=3)
+    far.copy_(x)
+    normed = torch.empty_like(x)
+    q, s = quant_device.rmsnorm_quant(far, w, normed=normed)
+    _check(x, w, None, 1e-6, FP8, q, s, None, normed)
+
+
+def test_no_rows_and_reused_outputs():
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q, s = quant_device.rmsnorm_quant(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda"), w)
+    assert q.shape == (0, 64) and s.shape == (0, 1)
+    x, w, _ = _inputs(9, 64, torch.bfloat16, False, seed=5)
+    out = torch.empty(9, 64, dtype=torch.uint8, device="cuda"), torch.empty(9, device="cuda")
+    q, s = quant_device.rmsnorm_quant(x, w, stream=torch.cuda.current_stream(), out=out)
+    assert q.data_ptr() == out[0].data_ptr() and s.data_ptr() == out[1].data_ptr() and q.dtype == FP8
+    _check(x, w, None, 1e-6, FP8, q, s, None, None)
+
+
+def test_graph_replays_and_another_stream():
+    x, w, r = _inputs(20, 4096, torch.bfloat16, True, seed=6)
+    out = torch.empty(20, 4096, dtype=FP8, device="cuda"), torch.empty(20, 1, device="cuda")
+    h = torch.empty_like(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        quant_device.rmsnorm_quant(x, w, residual=r, residual_out=h, stream=side, out=out)
+    for k in range(3):
+        x.copy_(torch.roll(x, 1, 0) * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(x, w, r, 1e-6, FP8, out[0], out[1], h, None)
+        again = quant_device.rmsnorm_quant(x, w, residual=r, residual_out=torch.empty_like(x))  # eager work between the replays
+        assert torch.equal(again[0].view(torch.uint8), out[0].view(torch.uint8)) and torch.equal(again[1], out[1])
+
+
+def test_refusals():
+    x, w, r = _inputs(4, 64, torch.bfloat16, True, seed=7)
+    out = torch.empty(4, 64, dtype=torch.uint8, device="cuda"), torch.empty(4, device="cuda")
+    f = quant_device.rmsnorm_quant
+    for stream in (None, torch.cuda.current_stream()):
+        with pytest.raises(ValueError, match="residual must be"):
+            f(x, w, residual=r[:3], out=out, stream=stream)
+        with pytest.raises(ValueError, match="residual must be"):
+            f(x, w, residual=r.half(), out=out, stream=stream)
+        with pytest.raises(ValueError, match="normed must be"):
+            f(x, w, normed=torch.empty(4, 65, dtype=torch.bfloat16, device="cuda"), out=out, stream=stream)
+        with pytest.raises(ValueError, match="out must be"):
+            f(x, w, out=(out[0][:3], out[1]), stream=stream)
+        with pytest.raises(ValueError, match="out must be"):
+            f(x, w, out=(out[0], out[1][:3]), stream=stream)
+        with pytest.raises(ValueError, match="weight must"):
+            f(x, w[:32], out=out, stream=stream)
+        with pytest.raises(ValueError, match="weight must"):
+            f(x, w.half(), out=out, stream=stream)
+        with pytest.raises(ValueError, match="without a residual"):
+            f(x, w, residual_out=r, out=out, stream=stream)
+    with pytest.raises(ValueError, match="dense rows"):
+        f(x.t().contiguous().t(), w)
+    with pytest.raises(ValueError, match="dense rows"):
+        f(x[:1].expand(4, 64), w)
+    with pytest.raises(ValueError, match="eps"):
+        f(x, w, -1.0)
+    with pytest.raises(ValueError, match="quant_dtype=None"):
+        f(x, w, quant_dtype=None, out=out)
