@@ -70,6 +70,7 @@ EXPORTS = (
     "psg_moe_softmax_sorting",
     "psg_moe_softmax_sorting_fused",
     "psg_rmsnorm_quant",
+    "psg_gemm_w4a16",
 )
 
 
@@ -252,6 +253,23 @@ class RmsnormArgs(ctypes.Structure):
     ]
 
 
+class W4A16Args(ctypes.Structure):
+    _fields_ = [
+        ("c", ctypes.c_void_p),
+        ("a", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("M", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("epilogue", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -298,7 +316,7 @@ def lib() -> ctypes.CDLL:
     handle.psg_moe_softmax_sorting_fused.restype = ctypes.c_int
     handle.psg_moe_softmax_sorting_fused.argtypes = [ctypes.c_int32] * 3
     for name in ("psg_gemm_a8w8", "psg_gemm_mxfp4", "psg_gemm_a8w8_static", "psg_moe_gemm", "psg_moe_mx_gemm", "psg_moe_sorting", "psg_moe_topk_gating",
-                 "psg_rmsnorm_quant"):
+                 "psg_rmsnorm_quant", "psg_gemm_w4a16"):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

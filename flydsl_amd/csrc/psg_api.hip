@@ -11,6 +11,7 @@
 #include "psg_common.h"
 #include "moe_gating.h"
 #include "moe_rows.h"
+#include "gemm_w4a16.h"
 #include "norm_quant.h"
 #include "tile_order.h"
 
@@ -39,6 +40,7 @@ hipError_t psg_launch_tile_order(int tiles_m, int tiles_n, int group_m, int32_t*
 hipError_t psg_launch_quant_pertoken(const void* x, int x_dtype, void* y, float* scale, int M, int K, int out_fp8, hipStream_t stream);
 hipError_t psg_launch_quant_mxfp4(const void* x, int x_dtype, void* packed, void* scales, int M, int R, int K, int shuffled,
                                   hipStream_t stream);
+hipError_t psg_launch_w4a16(const W4Params& p, int group, hipStream_t stream);
 hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream);
 
 // Scratch of the entry point that allocates nothing (psg_gemm_a8w8_static): the split-K partial sums of the tiled
@@ -1351,6 +1353,32 @@ int psg_rmsnorm_quant(const psg_rmsnorm_args* a, void* stream) {
     p.out = !quant ? NORM_NONE : a->out_dtype == PSG_IN_FP8_E4M3FN ? NORM_FP8 : NORM_INT8;
     const hipError_t e = psg_launch_rmsnorm_quant(p, a->x_dtype, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_rmsnorm_quant launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_gemm_w4a16(const psg_w4a16_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (!a->c || !a->a || !a->w || !a->scales) return fail(PSG_E_NULL, "c, a, w and scales must be non-NULL");
+    if (a->epilogue != PSG_EPI_NONE && !a->bias) return fail(PSG_E_NULL, "bias must be non-NULL when epilogue != none");
+    if (a->dtype != PSG_OUT_BF16 && a->dtype != PSG_OUT_FP16) return fail(PSG_E_DTYPE, "dtype %d unknown", a->dtype);
+    if (a->epilogue < PSG_EPI_NONE || a->epilogue > PSG_EPI_BIAS_GELU) return fail(PSG_E_DTYPE, "epilogue %d unknown", a->epilogue);
+    if (a->group != 32 && a->group != 64 && a->group != 128) return fail(PSG_E_SHAPE, "group=%d must be 32, 64 or 128", a->group);
+    if (a->M < 1 || a->M > 65536) return fail(PSG_E_SHAPE, "M=%d outside [1, 65536]", a->M);
+    if (a->N < 16 || a->N % 16) return fail(PSG_E_SHAPE, "N=%d must be a positive multiple of 16", a->N);
+    if (a->K < a->group || a->K % a->group) return fail(PSG_E_SHAPE, "K=%d must be a positive multiple of group=%d", a->K, a->group);
+    // (offsets into W, the scales and A's rows are 32-bit)
+    if ((uint64_t)a->N * (uint64_t)((a->K + 127ll) / 128) * 64ull >= OOB || (uint64_t)a->M * (uint64_t)a->K * 2ull >= OOB) return fail(PSG_E_SHAPE, "w or a exceeds the 4 GiB descriptor range");
+    if (!aligned(a->a, 16) || !aligned(a->w, 16)) return fail(PSG_E_ALIGN, "a and w must be 16-byte aligned");
+    if (!aligned(a->c, 8) || !aligned(a->scales, 8)) return fail(PSG_E_ALIGN, "c and scales must be 8-byte aligned");
+    if (!aligned(a->zeros, 2)) return fail(PSG_E_ALIGN, "zeros must be 2-byte aligned");
+    if (a->epilogue != PSG_EPI_NONE && !aligned(a->bias, 8)) return fail(PSG_E_ALIGN, "bias must be 8-byte aligned");
+    W4Params p = {};
+    p.c = a->c, p.a = a->a, p.w = static_cast<const uint8_t*>(a->w), p.scales = static_cast<const uint16_t*>(a->scales), p.zeros = static_cast<const uint8_t*>(a->zeros);
+    p.bias = static_cast<const uint16_t*>(a->bias);
+    p.M = a->M, p.N = a->N, p.K = a->K, p.out = a->dtype, p.epi = a->epilogue;
+    const hipError_t e = psg_launch_w4a16(p, a->group, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_gemm_w4a16 launch");
     g_err[0] = 0;
     return 0;
 }

@@ -136,3 +136,35 @@ def preshuffle_b(b_t: torch.Tensor) -> torch.Tensor:
     n, k = b_t.shape[-2:]
     assert n % 16 == 0 and k % 64 == 0, f"need N%16==0 and K%64==0, got N={n} K={k}"
     return b_t.reshape(n // 16, 16, k // 64, 4, 16).permute(0, 2, 3, 1, 4).contiguous()
+
+
+def shuffle_weight_w4a16(codes: torch.Tensor) -> torch.Tensor:
+    """4-bit codes ``[N, K]`` (one 0..15 per byte) -> the packed order of the group-scaled products, ``[N, ceil(K/128)*64]`` bytes: 1 KB blocks of 16 rows x 128
+    elements in which lane ``16 g + r`` of a wavefront reads 16 bytes of row ``r``, dword ``j`` of them elements ``32 j + 8 g .. + 7``, the even ones in the nibbles of the
+    lower half of the dword, the odd ones in those of the upper half.  ``N % 16 == 0``, ``K % 32 == 0``; elements past K are zeros."""
+    n, k = codes.shape
+    if codes.dtype != torch.uint8 or n % 16 or k % 32:
+        raise ValueError(f"expected uint8 codes [N, K] with N % 16 == 0 and K % 32 == 0, got {tuple(codes.shape)} {codes.dtype}")
+    if codes.numel() and int(codes.max()) > 15:
+        raise ValueError("codes must lie in [0, 15]")
+    kp = (k + 127) // 128 * 128
+    padded = torch.nn.functional.pad(codes, (0, kp - k))
+    #                   n/16    n%16  k/128     j  g  i/2 i%2
+    v = padded.reshape(n // 16, 16, kp // 128, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 6, 5)
+    return (v[..., 0::2] | (v[..., 1::2] << 4)).contiguous().view(n, kp // 2)
+
+
+def shuffle_group_scales(scales: torch.Tensor) -> torch.Tensor:
+    """Group scales ``[N, K/group]`` -> ``[N/16, K/group, 16]``, what the group-scaled products read."""
+    n, g = scales.shape
+    if n % 16:
+        raise ValueError(f"{n} rows of scales: a multiple of 16 is required")
+    return scales.reshape(n // 16, 16, g).transpose(1, 2).contiguous()
+
+
+def shuffle_group_zeros(zeros: torch.Tensor) -> torch.Tensor:
+    """Zero points ``[N, K/group]`` (0..15, one per byte) -> ``[N/16, K/group, 8]`` bytes, two neighbouring rows in one, the even one in the low nibble."""
+    if zeros.dtype != torch.uint8 or (zeros.numel() and int(zeros.max()) > 15):
+        raise ValueError("zero points must be uint8 in [0, 15]")
+    z = shuffle_group_scales(zeros)
+    return (z[..., 0::2] | (z[..., 1::2] << 4)).contiguous()

@@ -175,3 +175,24 @@ def per_1x32_f8_quant(x):
     sf = e8m0_to_f32(sc).clamp_min(1e-30)
     x_q = (blocks / sf.view(-1, 1)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(shape).contiguous()
     return x_q, sc.view(torch.uint8).reshape(*shape[:-1], shape[-1] // 32).contiguous()
+
+
+def pergroup_w4_quant(w: torch.Tensor, group_size: int = 128, zero_points: bool = False, scale_dtype=torch.bfloat16):
+    """4-bit quantisation of a weight ``[N, K]`` with one scale per ``group_size`` consecutive elements of a row.  Returns ``(codes [N, K] uint8 in 0..15, scales
+    [N, K/group] scale_dtype, zeros [N, K/group] uint8 or None)``; a code stands for ``scale * (code - zero)``, with ``zero = 8`` without zero points.
+
+    With zero points the group's range, extended to hold 0, is spread over the 16 codes; without, its largest magnitude is 7.5 steps (half a step is clipped at the
+    positive end).  The scale is rounded to ``scale_dtype`` before the codes are made; a group of zeros has scale 1.  ``w`` must be finite."""
+    n, k = w.shape
+    if k % group_size:
+        raise ValueError(f"K={k} must be a multiple of group_size={group_size}")
+    v = w.float().reshape(n, k // group_size, group_size)
+    if zero_points:
+        lo, hi = v.amin(-1, keepdim=True).clamp(max=0), v.amax(-1, keepdim=True).clamp(min=0)
+        scale = ((hi - lo) / 15).to(scale_dtype)
+    else:
+        scale = (v.abs().amax(-1, keepdim=True) / 7.5).to(scale_dtype)
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    zero = torch.round(-lo / scale.float()).clamp(0, 15) if zero_points else torch.full_like(scale, 8, dtype=torch.float32)
+    codes = (torch.round(v / scale.float()) + zero).clamp(0, 15).to(torch.uint8).reshape(n, k)
+    return codes, scale.squeeze(-1).contiguous(), zero.to(torch.uint8).squeeze(-1).contiguous() if zero_points else None

@@ -1,0 +1,156 @@
+"""GPU tests of the products with 4-bit weights and group scales against their definition in 64 bits.
+
+Exact inputs: activations are whole numbers up to 8 and scales powers of two, so that every partial sum (at most K * 8 * 31 < 2^24) is exact in fp32 whatever its order: the output
+is the definition, rounded once to 16 bits, to the bit.
+Random inputs: with u = 2^-23 for every addition in whatever order, a group's sum of codes and the sum of activations times 16 + zero are off by at most group * u * 31 * sum|a| each, the
+groups' sums by another (K / group + 8) u of their magnitudes; then the rounding to 16 bits, and what the activation function makes of the error (its slope is at most 1.13)
+and its own evaluation (2^-20, of exp2 and a reciprocal).
+"""
+
+import pytest
+import torch
+
+from flydsl_amd import layout, quant
+from kernels.gemm.w4a16_gemm import compile_w4a16_gemm
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+HALF = {"bf16": 2.0**-8, "fp16": 2.0**-11}
+
+
+def _weights(n, k, group, dt, zero_points, seed, exact):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    if exact:
+        scale = torch.exp2(-torch.randint(4, 7, (n, k // group), generator=g).float()).to(dt)
+    else:
+        scale = (0.002 + 0.01 * torch.rand(n, k // group, generator=g)).to(dt)
+    zero = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zero_points else None
+    return codes, scale, zero
+
+
+def _deq(codes, scale, zero, group):
+    z = torch.full(scale.shape, 8.0, dtype=torch.float64) if zero is None else zero.double()
+    return (codes.double() - z.repeat_interleave(group, 1)) * scale.double().repeat_interleave(group, 1)
+
+
+def _act(y, epi):
+    if epi == "bias_relu":
+        return y.clamp(min=0)
+    if epi == "bias_silu":
+        return y * torch.sigmoid(y)
+    if epi == "bias_gelu":
+        return 0.5 * y * (1 + torch.tanh(0.7978845608 * (y + 0.044715 * y**3)))
+    return y
+
+
+def _run(a, codes, scale, zero, bias, group, dtype, epi, guard=3):
+    m, k = a.shape
+    n = codes.shape[0]
+    fn = compile_w4a16_gemm(N=n, K=k, group_size=group, in_dtype=dtype, zero_points=zero is not None, epilogue=epi)
+    c = torch.full((m + guard, n), -77.0, dtype=DT[dtype], device="cuda")
+    z = None if zero is None else layout.shuffle_group_zeros(zero).cuda()
+    args = a.cuda(), layout.shuffle_weight_w4a16(codes).cuda(), layout.shuffle_group_scales(scale).cuda(), z, None if bias is None else bias.cuda(), m
+    print(f"w4a16 M={m} N={n} K={k} group={group} {dtype} {epi}", flush=True)
+    fn(c, *args, torch.cuda.current_stream())
+    again = torch.empty_like(c[:m])
+    fn(again, *args)  # the Python checks, the current stream
+    torch.cuda.synchronize()
+    assert (c[m:] == -77).all()
+    assert torch.equal(c[:m].view(torch.int16), again.view(torch.int16))
+    return c[:m].cpu()
+
+
+SIZES = [(1, 16, 128), (1, 4096, 4096), (2, 2064, 1152), (5, 1040, 2176), (16, 48, 11008), (17, 512, 640), (32, 7168, 2048), (33, 272, 512), (100, 1024, 1024), (3, 28672, 256), (16, 8208, 384)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("group,zero_points,dtype", [(128, False, "bf16"), (128, True, "fp16"), (64, True, "bf16"), (64, False, "fp16"), (32, False, "fp16"), (32, True, "bf16")])
+def test_exact_sums(m, n, k, group, zero_points, dtype):
+    if group < 128:
+        k -= 128 - group if k > 128 else 0  # rows that end inside a block
+    dt = DT[dtype]
+    codes, scale, zero = _weights(n, k, group, dt, zero_points, m + n + k, True)
+    a = torch.randint(-8, 9, (m, k), generator=torch.Generator().manual_seed(m)).to(dt)
+    got = _run(a, codes, scale, zero, None, group, dtype, "none")
+    want = (a.double() @ _deq(codes, scale, zero, group).t()).float()  # exact in fp32
+    assert torch.equal(got, want.to(dt))
+
+
+@pytest.mark.parametrize("epi", ["none", "bias", "bias_relu", "bias_silu", "bias_gelu"])
+@pytest.mark.parametrize("m,n,k,group,zero_points,dtype", [(1, 1024, 4096, 128, True, "bf16"), (9, 528, 2080, 32, True, "fp16"), (31, 320, 960, 64, False, "bf16")])
+def test_random_values_and_epilogues(m, n, k, group, zero_points, dtype, epi):
+    dt = DT[dtype]
+    codes, scale, zero = _weights(n, k, group, dt, zero_points, 5, False)
+    g = torch.Generator().manual_seed(6)
+    a, bias = torch.randn(m, k, generator=g).to(dt), (0.5 * torch.randn(n, generator=g)).to(dt)
+    got = _run(a, codes, scale, zero, None if epi == "none" else bias, group, dtype, epi).double()
+    w = _deq(codes, scale, zero, group)
+    y = a.double() @ w.t()
+    u = 2.0**-23
+    mags = (a.double().abs().view(m, -1, group).sum(-1)) @ scale.double().t()
+    slack = 2 * group * u * 31 * mags + (k // group + 8) * u * (a.double().abs() @ w.abs().t())
+    if epi != "none":
+        y = y + bias.double()
+        slack = slack + u * y.abs()
+    want = _act(y, epi)
+    slack = 1.13 * slack + (2.0**-20 * y.abs() if epi in ("bias_silu", "bias_gelu") else 0)
+    assert ((got - want).abs() <= HALF[dtype] * (want.abs() + slack) + slack + 2.0**-25).all()
+
+
+def test_quantised_weights_and_outlier_rows():
+    """What the quantiser makes, with an activation row of zeros and one that is not finite beside the others."""
+    g = torch.Generator().manual_seed(8)
+    w = 0.02 * torch.randn(256, 1024, generator=g)
+    a = torch.randn(6, 1024, generator=g).to(torch.bfloat16)
+    a[1] = 0
+    a[4, 7] = float("nan")
+    for zero_points in (False, True):
+        codes, scale, zero = quant.pergroup_w4_quant(w, 64, zero_points)
+        got = _run(a, codes, scale, zero, None, 64, "bf16", "none").float()
+        keep = [0, 2, 3, 5]
+        want = (a[keep].double() @ _deq(codes, scale, zero, 64).t()).float()
+        assert (got[1] == 0).all() and torch.isnan(got[4]).all()
+        assert (got[keep] - want).abs().max() <= 2.0**-7 * want.abs().max()
+        # and the weights are what they were quantised from: 15 or 16 steps over a group's range of about 5 deviations, sqrt(1/12) of a step each
+        full = a[keep].double() @ w.double().t()
+        assert (got[keep] - full).norm() / full.norm() < 0.13
+
+
+def test_graph_replays():
+    m, n, k = 4, 1024, 2048
+    fn = compile_w4a16_gemm(N=n, K=k, group_size=128)
+    codes, scale, _ = _weights(n, k, 128, torch.bfloat16, False, 3, True)
+    w, s = layout.shuffle_weight_w4a16(codes).cuda(), layout.shuffle_group_scales(scale).cuda()
+    a = torch.randint(-8, 9, (m, k)).to(torch.bfloat16).cuda()
+    c, eager = (torch.empty(m, n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        fn(c, a, w, s, None, None, m, side)
+    for _ in range(3):
+        a.copy_(torch.randint(-8, 9, (m, k)).to(torch.bfloat16))
+        graph.replay()
+        fn(eager, a, w, s, None, None, m)
+        torch.cuda.synchronize()
+        assert torch.equal(c, eager)
+        want = (a.cpu().double() @ _deq(codes, scale, None, 128).t()).float().to(torch.bfloat16)
+        assert torch.equal(c.cpu(), want)
+
+
+def test_refusals():
+    fn = compile_w4a16_gemm(N=64, K=256, zero_points=True, epilogue="bias")
+    b = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device="cuda")
+    good = dict(C=b(4, 64), A=b(4, 256), W=b(64, 128, dt=torch.uint8), scales=b(4, 2, 16), zeros=b(4, 2, 8, dt=torch.uint8), bias=b(64))
+    for stream in (None, torch.cuda.current_stream()):
+        fn(*good.values(), 4, stream)
+        for name, bad in [("C", b(3, 64)), ("A", b(4, 255)), ("W", b(63, 128, dt=torch.uint8)), ("scales", b(4, 2, 15)), ("zeros", b(4, 2, 7, dt=torch.uint8)), ("bias", b(63)),
+                          ("A", b(4, 256, dt=torch.float16)), ("scales", b(4, 2, 16, dt=torch.float16)), ("zeros", None), ("bias", None), ("W", b(64, 256, dt=torch.uint8)[:, ::2]),
+                          ("A", b(4, 512)[:, :256])]:
+            with pytest.raises(ValueError, match=name):
+                fn(*{**good, name: bad}.values(), 4, stream)
+        with pytest.raises(ValueError, match="aligned"):
+            fn(*{**good, "A": b(4 * 256 + 4)[4:]}.values(), 4, stream)
+        with pytest.raises(ValueError, match="outside"):
+            fn(*good.values(), 0, stream)
