@@ -71,6 +71,7 @@ EXPORTS = (
     "psg_moe_softmax_sorting_fused",
     "psg_rmsnorm_quant",
     "psg_gemm_w4a16",
+    "psg_gemm_grouped",
 )
 
 
@@ -270,6 +271,25 @@ class W4A16Args(ctypes.Structure):
     ]
 
 
+class GroupedArgs(ctypes.Structure):
+    _fields_ = [
+        ("c", ctypes.c_void_p),
+        ("a", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("scale_a", ctypes.c_void_p),
+        ("scale_b", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("M", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("tile_rows", ctypes.c_int32),
+        ("pad0", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -316,7 +336,7 @@ def lib() -> ctypes.CDLL:
     handle.psg_moe_softmax_sorting_fused.restype = ctypes.c_int
     handle.psg_moe_softmax_sorting_fused.argtypes = [ctypes.c_int32] * 3
     for name in ("psg_gemm_a8w8", "psg_gemm_mxfp4", "psg_gemm_a8w8_static", "psg_moe_gemm", "psg_moe_mx_gemm", "psg_moe_sorting", "psg_moe_topk_gating",
-                 "psg_rmsnorm_quant", "psg_gemm_w4a16"):
+                 "psg_rmsnorm_quant", "psg_gemm_w4a16", "psg_gemm_grouped"):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

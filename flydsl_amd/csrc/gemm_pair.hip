@@ -5,12 +5,14 @@
 // 8192x4096x4096 106.7 / 121.4 / 107.8, 8192x8192x1024 78.9 / 85.1 / 69.3, 1024x8192x2048 25.6 / 22.3 / 19.5, 1500x11264x4096 86.1 / 84.9 / 71.8, 5120x5120x8320
 // 170 / 201 / 181; int8 4096x8192x2048 65.2 / 67.9 / 60.4, 4096x28672x8192 701 / 720 / 688 (the estimates of pick_plain_tile see it the other way round, 674 / 692, and take the larger tile); bf16 1500x5264x4096 84.4 / 64.6 / 57.7, 5133x5120x8320 348 / 371 / 346.
 // Same bits.
+// With GroupParams the rows are those of one group of a grouped product (gemm_grouped.hip) and W and its scales that group's.
+#include "group_tiles.h"
 #include "pair_loop.h"
 
 namespace {
 
-template <int KIND, int STORE>
-__global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p) {
+template <int KIND, int STORE, class... GROUPS>
+__global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p, GROUPS... groups) {
     using acc_t = typename Acc<KIND>::type;
     using P = Pair<KIND>;
     constexpr int MR = P::MR, NR = P::NR, TM = P::TM, TN = P::TN;
@@ -22,9 +24,19 @@ __global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p) {
     const int tid = threadIdx.x;
     const int wave = wave_id();
     const int lane = tid & 63, li = lane & 15, lg = lane >> 4;
-    int tm, tn;
-    tile_coords((int)blockIdx.x, (p.M + TM - 1) / TM, (p.N + TN - 1) / TN, p.group_m, tm, tn);
-    const int m0 = tm * TM, n0 = tn * TN;
+    int tm, tn, m0;
+    if constexpr (sizeof...(GROUPS) == 1) {
+        GroupTile t;
+        if (!group_tile((groups, ...), p.M, TM, (int)blockIdx.x, (p.N + TN - 1) / TN, lane, t)) return;
+        m0 = t.row, tn = t.n_tile;
+        p.M = t.row + t.rows;  // the group's end
+        p.b += (uint64_t)t.e * (uint64_t)p.N * (uint64_t)p.K * (SCALED ? 1u : 2u);
+        if constexpr (SCALED) p.sb += (uint64_t)t.e * (uint64_t)p.N;
+    } else {
+        tile_coords((int)blockIdx.x, (p.M + TM - 1) / TM, (p.N + TN - 1) / TN, p.group_m, tm, tn);
+        m0 = tm * TM;
+    }
+    const int n0 = tn * TN;
     const uint32_t K = SCALED ? (uint32_t)p.K : (uint32_t)p.K * 2u;  // bytes of a row
     const int steps = (int)((K + TK - 1) / TK), per = STORE == STORE_ACC ? (steps + p.splits - 1) / p.splits : steps;
     uint32_t k0 = STORE == STORE_ACC ? blockIdx.y * (uint32_t)(per * TK) : 0u;
@@ -109,6 +121,25 @@ void go(const A8W8Params& p, int store, dim3 grid, hipStream_t stream) {
 }
 
 }  // namespace
+
+// The grouped product on these tiles: bf16 by STORE_C, fp16 by STORE_C_GENERIC
+hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream) {
+    g.most = (int)group_tiles_most(p.M, g.groups, 128);
+    const dim3 grid((unsigned)g.most * (unsigned)((p.N + 255) / 256));
+#define PSG_GROUPED(KIND_)                                                                                                                             \
+    case KIND_:                                                                                                                                        \
+        if (p.out == OUT_BF16) hipLaunchKernelGGL((k_pair<KIND_, STORE_C, GroupParams>), grid, dim3(256), 0, stream, p, g);                             \
+        else hipLaunchKernelGGL((k_pair<KIND_, STORE_C_GENERIC, GroupParams>), grid, dim3(256), 0, stream, p, g);                                       \
+        return hipGetLastError();
+    switch (kind) {
+        PSG_GROUPED(KIND_INT8)
+        PSG_GROUPED(KIND_FP8)
+        PSG_GROUPED(KIND_FP16)
+        PSG_GROUPED(KIND_BF16)
+    }
+#undef PSG_GROUPED
+    return hipErrorInvalidValue;
+}
 
 // store: STORE_ACC (p.splits slices), STORE_C or STORE_C_GENERIC
 hipError_t psg_launch_pair(const A8W8Params& p, int kind, int store, hipStream_t stream) {

@@ -12,6 +12,7 @@
 #include "moe_gating.h"
 #include "moe_rows.h"
 #include "gemm_w4a16.h"
+#include "group_tiles.h"
 #include "norm_quant.h"
 #include "tile_order.h"
 
@@ -41,6 +42,8 @@ hipError_t psg_launch_quant_pertoken(const void* x, int x_dtype, void* y, float*
 hipError_t psg_launch_quant_mxfp4(const void* x, int x_dtype, void* packed, void* scales, int M, int R, int K, int shuffled,
                                   hipStream_t stream);
 hipError_t psg_launch_w4a16(const W4Params& p, int group, hipStream_t stream);
+int psg_grouped_tile(int64_t rows, int groups);
+hipError_t psg_launch_grouped(const A8W8Params& p, const GroupParams& g, int kind, int bm, hipStream_t stream);
 hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream);
 
 // Scratch of the entry point that allocates nothing (psg_gemm_a8w8_static): the split-K partial sums of the tiled
@@ -1379,6 +1382,36 @@ int psg_gemm_w4a16(const psg_w4a16_args* a, void* stream) {
     p.M = a->M, p.N = a->N, p.K = a->K, p.out = a->dtype, p.epi = a->epilogue;
     const hipError_t e = psg_launch_w4a16(p, a->group, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_gemm_w4a16 launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (!a->c || !a->a || !a->w || !a->offsets) return fail(PSG_E_NULL, "c, a, w and offsets must be non-NULL");
+    if (a->in_dtype < PSG_IN_INT8 || a->in_dtype > PSG_IN_BF16) return fail(PSG_E_DTYPE, "in_dtype %d unknown", a->in_dtype);
+    if (a->out_dtype != PSG_OUT_BF16 && a->out_dtype != PSG_OUT_FP16) return fail(PSG_E_DTYPE, "out_dtype %d unknown", a->out_dtype);
+    const bool is16 = a->in_dtype == PSG_IN_FP16 || a->in_dtype == PSG_IN_BF16;
+    const int64_t eb = is16 ? 2 : 1;
+    if (!is16 && (!a->scale_a || !a->scale_b)) return fail(PSG_E_NULL, "scale_a and scale_b must be non-NULL for 8-bit inputs");
+    if (a->M < 1 || a->M > (1 << 22)) return fail(PSG_E_SHAPE, "M=%d outside [1, 2^22]", a->M);
+    if (a->groups < 1 || a->groups > 4096) return fail(PSG_E_SHAPE, "groups=%d outside [1, 4096]", a->groups);
+    if (a->N < 16 || a->N % 16) return fail(PSG_E_SHAPE, "N=%d must be a positive multiple of 16", a->N);
+    if (a->K < 64 / eb || (a->K * eb) % 64) return fail(PSG_E_SHAPE, "K=%d must be a positive multiple of %d", a->K, (int)(64 / eb));
+    if ((uint64_t)a->N * (uint64_t)a->K * (uint64_t)eb >= OOB) return fail(PSG_E_SHAPE, "N*K bytes exceed the 4 GiB descriptor range");
+    if (128ull * (uint64_t)a->K * (uint64_t)eb >= OOB || 128ull * (uint64_t)a->N * 2ull >= OOB) return fail(PSG_E_SHAPE, "128 rows of a or c exceed the 4 GiB descriptor range");
+    if (a->tile_rows != 0 && a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64 or 128", a->tile_rows);
+    const int bm = a->tile_rows ? a->tile_rows : psg_grouped_tile(a->M, a->groups);
+    if (group_tiles_most(a->M, a->groups, bm) * ((a->N + 63ll) / 64) > 0x7FFFFFFFll) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
+    if (!aligned(a->a, 16) || !aligned(a->w, 16) || !aligned(a->c, 16)) return fail(PSG_E_ALIGN, "a, w and c must be 16-byte aligned");
+    if (!is16 && (!aligned(a->scale_b, 16) || !aligned(a->scale_a, 4))) return fail(PSG_E_ALIGN, "scale_b must be 16-byte and scale_a 4-byte aligned");
+    if (!aligned(a->offsets, 4)) return fail(PSG_E_ALIGN, "offsets must be 4-byte aligned");
+    A8W8Params p = {};
+    p.c = a->c, p.a = static_cast<const uint8_t*>(a->a), p.b = static_cast<const uint8_t*>(a->w), p.sa = a->scale_a, p.sb = a->scale_b;
+    p.M = a->M, p.N = a->N, p.K = a->K, p.epi = EPI_NONE, p.out = a->out_dtype, p.splits = 1;
+    const GroupParams g = {a->offsets, a->groups, 0};
+    const hipError_t e = psg_launch_grouped(p, g, a->in_dtype, bm, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_gemm_grouped launch");
     g_err[0] = 0;
     return 0;
 }

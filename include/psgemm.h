@@ -510,6 +510,33 @@ typedef struct psg_w4a16_args {
 
 int psg_gemm_w4a16(const psg_w4a16_args *args, void *stream);
 
+/*
+ * Products of rows grouped by expert with the experts' own weights: C[r,:] = A[r,:] W[e]^T (* scale_a[r] * scale_b[e,:]) for offsets[e] <= r < offsets[e+1].
+ *   a [M,K] and c [M,N] row-major; w [groups][N,K] preshuffled, scale_a [M] and scale_b [groups,N] fp32 for 8-bit operands, all as in psg_gemm_a8w8; c bf16 or fp16.
+ *   offsets [groups+1] int32 on the device, not decreasing.  Rows of c outside [offsets[0], offsets[groups]) are left as they are; groups may be empty.  An offset outside [0, M] counts
+ *   as the nearer end, and a group whose end is not above its begin has no rows: no offsets make the kernels read or write outside the operands (where they go back, which
+ *   rows are written is not said).
+ * in_dtype PSG_IN_INT8 .. PSG_IN_BF16; tile_rows 0 (chosen by the mean rows of a group) or 16, 32, 64, 128.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K * bytes % 64 == 0, the bytes of
+ * one weight below 4 GiB.  a, w, c and scale_b 16-byte, scale_a and offsets 4-byte aligned.  Sums as in psg_gemm_a8w8 (int8 exact), of every row in the same order
+ * whatever its group's size.
+ */
+typedef struct psg_grouped_args {
+    void *c;
+    const void *a;
+    const void *w;
+    const float *scale_a;
+    const float *scale_b;
+    const int32_t *offsets;
+    int32_t M, N, K;
+    int32_t groups;
+    int32_t in_dtype;
+    int32_t out_dtype;
+    int32_t tile_rows;
+    int32_t pad0; /* 0 */
+} psg_grouped_args;
+
+int psg_gemm_grouped(const psg_grouped_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
