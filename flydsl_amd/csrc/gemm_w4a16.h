@@ -11,7 +11,6 @@ struct W4Params {
     const uint16_t* bias;  // [N]
     int M, N, K;
     int out, epi;          // OUT_*, EPI_*
-    int ks;                // set by the launcher: K slices of a workgroup (a power of two)
-    int groups;            // set by the launcher: column groups of the launch, unit_q units of 8 columns each,
-    int unit_q, unit_r;    // the first unit_r of them one more
+    int passes, per;       // set by the launcher: passes over the columns, 128-element steps of a wavefront in each
+    int unit_q, unit_r;    // set by the launcher: a workgroup has unit_q units of 8 columns, the first unit_r of them one more
 };

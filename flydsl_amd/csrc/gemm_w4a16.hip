@@ -7,9 +7,10 @@
 // in fp32, and X of a lane's own row is what the same MFMA gives for a weight of ones.  (P is at most 31/16 of the sum with the 16 alone: the difference loses four or five of 24
 // bits, far below the 16-bit output's rounding.)
 //
-// Bound: the weights' way from memory, like the streaming kernel of the wider types (gemm_a8w8_stream.hip), and dealt out like there: columns in units of 8, evenly over the workgroups,
-// a wavefront with up to four units in one or two 16-column windows; the wavefronts of a workgroup are K slices x column groups, their sums meet in LDS in a fixed order, one launch,
-// no workspace.
+// Bound: the weights' way from memory.  The columns are dealt out in units of 8, evenly, one workgroup a CU; its eight wavefronts are eight slices of K.  A wavefront's part of A, 16
+// rows of up to 1024 elements, stays in registers (128 of them) while the workgroup's columns go by in windows of 16, and so do the X of its groups: what moves is W alone, asked for
+// eight steps ahead, windows on end, without a barrier.  The slices' sums meet in LDS in a fixed order: one launch, no workspace.  Longer rows take several passes over the
+// columns, each with its part of A.
 //
 // Layout: W in blocks of 16 rows x 128 elements, 1 KB: lane l = 16 g + r of a wavefront reads 16 bytes, row r, dword j of them elements 32 j + 8 g .. + 7, what
 // it multiplies in MFMA j; the even ones are the nibbles of the lower half of the dword, the odd ones those of the upper half, so that two of them are a mask away from a
@@ -19,19 +20,14 @@
 
 namespace {
 
-// eight codes -> eight operands 16 + q
-template <bool BF16>
-__device__ __forceinline__ v4i widen(int w) {
-    constexpr int UP = BF16 ? 3 : 6;  // from the lowest nibble to the bits of the mantissa that count 1..8 beside 16
-    constexpr int MASK = BF16 ? 0x00780078 : 0x03C003C0, BASE = BF16 ? 0x41804180 : 0x4C004C00;
-    v4i r;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        const int s = UP - 4 * t;
-        r[t] = ((s >= 0 ? w << s : (int)((unsigned)w >> -s)) & MASK) | BASE;
-    }
-    return r;
-}
+// Constants in registers of the two files: an instruction that masks and joins takes one from each, and the compiler would otherwise make two of it, a literal each
+template <int MASK, int BASE>
+struct Join {
+    int mask = MASK, base = BASE;
+    __device__ __forceinline__ Join() { asm("" : "+s"(mask), "+v"(base)); }
+    __device__ __forceinline__ int operator()(int x) const { return (x & mask) | base; }
+};
+__device__ __forceinline__ int shift(int x, int left) { return left >= 0 ? x << left : (int)((unsigned)x >> -left); }
 
 template <bool BF16>
 __device__ __forceinline__ v4f mfma16(v4i w, v4i a, v4f c) {
@@ -39,145 +35,166 @@ __device__ __forceinline__ v4f mfma16(v4i w, v4i a, v4f c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, a), c, 0, 0, 0);
 }
 
-// MB: 16-row blocks of A.  NWIN: 16-column windows of a wavefront.  GS: elements of a group.  ZP: zero points.  CH: 128-element steps that are asked for together.
-template <bool BF16, int MB, int NWIN, int GS, bool ZP, int NWAVES, int CH>
-__global__ void __launch_bounds__(NWAVES * 64) k_w4a16(W4Params p) {
+constexpr int W4_WAVES = 8;
+
+// MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  R: windows that are asked for ahead.
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int R>
+__global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     constexpr int GPS = 128 / GS, MPG = GS / 32;  // groups of a step, MFMAs of a group
-    __shared__ v4f part[NWAVES][NWIN * MB * 64];
+    extern __shared__ v4f part[];                 // [wavefront][window][16-row block][lane]
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
-    const int ksh = __builtin_ctz(p.ks), gpw = NWAVES >> ksh;  // column groups of a workgroup
     auto unit_begin = [&](int g) { return g * p.unit_q + (g < p.unit_r ? g : p.unit_r); };
     // an XCD owns one range of columns: workgroups go round the XCDs
-    const int bid = (gridDim.x & 7) == 0 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
-    const int grp = bid * gpw + (wave >> ksh), m0 = (int)blockIdx.y * MB * 16, M = p.M - m0;
-    const int K = p.K, steps = (K + 127) >> 7, groups = K / GS;
-    const int per = (steps + p.ks - 1) >> ksh, s0 = (wave & (p.ks - 1)) * per, s1 = s0 + per < steps ? s0 + per : steps;
-    const int n_begin = grp < p.groups ? unit_begin(grp) * 8 : 0, n_end = grp < p.groups ? unit_begin(grp + 1) * 8 : 0;
+    const int wg = (gridDim.x & 7) == 0 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
+    const int n_begin = unit_begin(wg) * 8, n_end = unit_begin(wg + 1) * 8, windows = (n_end - n_begin + 15) >> 4;
+    const int m0 = (int)blockIdx.y * MB * 16, M = p.M - m0, K = p.K, steps = (K + 127) >> 7, groups = K / GS;
 
-    v4f acc[NWIN][MB];
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w, (uint64_t)p.N * (uint64_t)steps * 64ull), rs = make_rsrc(p.scales, (uint64_t)p.N * (uint64_t)groups * 2ull),
+                                 rz = make_rsrc(ZP ? p.zeros : p.w, (uint64_t)p.N * (uint64_t)groups / 2ull),
+                                 ra = make_rsrc(static_cast<const uint16_t*>(p.a) + (uint64_t)m0 * (uint64_t)K, (uint64_t)M * (uint64_t)K * 2ull);
+    // a lane reads row n of W, and the scales of the four columns from c on that it holds of C; a window is 16 rows on
+    const int n_lane = n_begin + li, c_lane = n_begin + lg * 4;
+    const uint32_t w_lane = (uint32_t)(n_lane >> 4) * (uint32_t)steps * 1024u + (uint32_t)(lg * 256 + (n_lane & 15) * 16);
+    const uint32_t s_lane = (uint32_t)(c_lane >> 4) * (uint32_t)groups * 32u + (uint32_t)(c_lane & 15) * 2u;
+    uint32_t a_lane[MB];
 #pragma unroll
-    for (int w = 0; w < NWIN; w++)
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) acc[w][mb] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int mb = 0; mb < MB; mb++) a_lane[mb] = mb * 16 + li < M ? (uint32_t)(mb * 16 + li) * (uint32_t)K * 2u + (uint32_t)lg * 16u : OOB;
+    const Join<BF16 ? 0x00780078 : 0x03C003C0, BF16 ? 0x41804180 : 0x4C004C00> code;  // a code in the bits of the mantissa that count 1 to 8 beside 16
+    const Join<0x00780000, 0x41800000> zero;                                           // the same in fp32
 
-    if (s0 < s1 && n_begin < n_end) {
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w, (uint64_t)p.N * (uint64_t)steps * 64ull), rs = make_rsrc(p.scales, (uint64_t)p.N * (uint64_t)groups * 2ull),
-                                     rz = make_rsrc(ZP ? p.zeros : p.w, (uint64_t)p.N * (uint64_t)groups / 2ull),
-                                     ra = make_rsrc(static_cast<const uint16_t*>(p.a) + (uint64_t)m0 * (uint64_t)K, (uint64_t)M * (uint64_t)K * 2ull);
-        uint32_t w_off[NWIN], s_off[NWIN];
+    for (int pass = 0; pass < p.passes; pass++) {
+        const int s0 = (pass * W4_WAVES + wave) * p.per, s1 = s0 + p.per < steps ? s0 + p.per : steps;
+        v4i w[R][SPW];
+        v2i sc[R][SPW][GPS];
+        int z[R][SPW][ZP ? GPS : 1];
+        auto load = [&](int win, int t, auto I) __attribute__((always_inline)) {
+            constexpr int i = decltype(I)::value;
+            const bool in = win < windows && s0 + t < s1;  // uniform
+            const bool row = in && n_lane + win * 16 < n_end, col = in && c_lane + win * 16 < n_end;
+            w[i][t] = buf_load16_nt(rw, row ? w_lane : OOB, in ? ((uint32_t)win * (uint32_t)steps + (uint32_t)(s0 + t)) * 1024u : 0u);
 #pragma unroll
-        for (int w = 0; w < NWIN; w++) {
-            // a lane reads row n of W, and scales of the four columns that it holds of C
-            const int n = n_begin + w * 16 + li, c = n_begin + w * 16 + lg * 4;
-            w_off[w] = n < n_end ? (uint32_t)(n >> 4) * (uint32_t)steps * 1024u + (uint32_t)(lg * 256 + (n & 15) * 16) : OOB;
-            s_off[w] = c < n_end ? (uint32_t)(c >> 4) * (uint32_t)groups * 32u + (uint32_t)(c & 15) * 2u : OOB;
-        }
-        uint32_t a_off[MB];
+            for (int g = 0; g < GPS; g++) {
+                const int at = (s0 + t) * GPS + g;
+                const bool has = in && at < groups;
+                const uint32_t so = has ? (uint32_t)win * (uint32_t)groups + (uint32_t)at : 0u;
+                sc[i][t][g] = buf_load8(rs, col && has ? s_lane : OOB, so * 32u);
+                if constexpr (ZP) z[i][t][g] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rz, (int)(col && has ? s_lane >> 2 : OOB), (int)(so * 8u), 0);
+            }
+        };
+        v4i a[SPW][4][MB];
 #pragma unroll
-        for (int mb = 0; mb < MB; mb++) a_off[mb] = mb * 16 + li < M ? (uint32_t)(mb * 16 + li) * (uint32_t)K * 2u + (uint32_t)lg * 16u : OOB;
-        const int one = BF16 ? 0x3F803F80 : 0x3C003C00;
-        const v4i ones = {one, one, one, one};
-
-        for (int c0 = s0; c0 < s1; c0 += CH) {
-            v4i a[CH][4][MB], w[CH][NWIN];
-            v2i sc[CH][GPS][NWIN];
-            uint32_t z[CH][GPS][NWIN];
+        for (int t = 0; t < SPW; t++)
 #pragma unroll
-            for (int t = 0; t < CH; t++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int mb = 0; mb < MB; mb++) {
-                        const int k = (c0 + t) * 128 + j * 32;
-                        const bool in = c0 + t < s1 && k < K;  // (K is a multiple of 32)
-                        a[t][j][mb] = buf_load16(ra, in ? a_off[mb] : OOB, in ? (uint32_t)k * 2u : 0u);
-                    }
-#pragma unroll
-            for (int t = 0; t < CH; t++)
-#pragma unroll
-                for (int win = 0; win < NWIN; win++) {
-                    const bool in = c0 + t < s1;
-                    w[t][win] = buf_load16_nt(rw, in ? w_off[win] : OOB, in ? (uint32_t)(c0 + t) * 1024u : 0u);
-#pragma unroll
-                    for (int g = 0; g < GPS; g++) {
-                        const int at = (c0 + t) * GPS + g;
-                        const bool has = in && at < groups;
-                        sc[t][g][win] = buf_load8(rs, has ? s_off[win] : OOB, has ? (uint32_t)at * 32u : 0u);
-                        // (all zero points are less than 2^27 bytes: a quarter of OOB lies behind them too)
-                        if constexpr (ZP) z[t][g][win] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rz, (int)(has ? s_off[win] >> 2 : OOB), has ? at * 8 : 0, 0);
-                    }
+                for (int mb = 0; mb < MB; mb++) {
+                    const int k = (s0 + t) * 128 + j * 32;
+                    const bool in = s0 + t < s1 && k < K;  // (K is a multiple of 32)
+                    a[t][j][mb] = buf_load16(ra, in ? a_lane[mb] : OOB, in ? (uint32_t)k * 2u : 0u);
                 }
-            __builtin_amdgcn_sched_barrier(0);
+        static_for<R>([&](auto I) {
 #pragma unroll
-            for (int t = 0; t < CH; t++)
+            for (int t = 0; t < SPW; t++) load(decltype(I)::value, t, I);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+
+        // X of every group, times -24 without zero points
+        float x[SPW][GPS][MB];
+        const int one = BF16 ? (ZP ? 0x3F803F80 : (int)0xC1C0C1C0) : (ZP ? 0x3C003C00 : (int)0xCE00CE00);
+        const v4i ones = {one, one, one, one};
+#pragma unroll
+        for (int t = 0; t < SPW; t++)
+#pragma unroll
+            for (int g = 0; g < GPS; g++)
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) {
+                    v4f y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int j = g * MPG; j < (g + 1) * MPG; j++) y = mfma16<BF16>(ones, a[t][j][mb], y);
+                    x[t][g][mb] = y[0];
+                }
+
+        auto window = [&](int win, auto I) __attribute__((always_inline)) {
+            constexpr int i = decltype(I)::value;
+            v4f acc[MB];
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) acc[mb] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < SPW; t++) {
 #pragma unroll
                 for (int g = 0; g < GPS; g++) {
-                    v4f x[MB], pr[NWIN][MB];
+                    v4f pr[MB];
 #pragma unroll
-                    for (int mb = 0; mb < MB; mb++) {
-                        x[mb] = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int win = 0; win < NWIN; win++) pr[win][mb] = x[mb];
-                    }
+                    for (int mb = 0; mb < MB; mb++) pr[mb] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int j = g * MPG; j < (g + 1) * MPG; j++) {
+                        v4i b;
 #pragma unroll
-                        for (int mb = 0; mb < MB; mb++) x[mb] = mfma16<BF16>(ones, a[t][j][mb], x[mb]);
+                        for (int q = 0; q < 4; q++) b[q] = code(shift(w[i][t][j], (BF16 ? 3 : 6) - 4 * q));
 #pragma unroll
-                        for (int win = 0; win < NWIN; win++) {
-                            const v4i b = widen<BF16>(w[t][win][j]);
-#pragma unroll
-                            for (int mb = 0; mb < MB; mb++) pr[win][mb] = mfma16<BF16>(b, a[t][j][mb], pr[win][mb]);
-                        }
+                        for (int mb = 0; mb < MB; mb++) pr[mb] = mfma16<BF16>(b, a[t][j][mb], pr[mb]);
                     }
 #pragma unroll
-                    for (int win = 0; win < NWIN; win++)
+                    for (int v = 0; v < 4; v++) {
+                        const float s = from_out16<BF16 ? OUT_BF16 : OUT_FP16>((uint16_t)((uint32_t)sc[i][t][g][v >> 1] >> (16 * (v & 1))));
+                        const float zc = ZP ? __builtin_bit_cast(float, zero(z[i][t][g] << (19 - 4 * v))) : 0.f;
 #pragma unroll
-                        for (int v = 0; v < 4; v++) {
-                            const float s = from_out16<BF16 ? OUT_BF16 : OUT_FP16>((uint16_t)((uint32_t)sc[t][g][win][v >> 1] >> (16 * (v & 1))));
-                            const float zc = ZP ? 16.0f + (float)((z[t][g][win] >> (4 * v)) & 15u) : 24.0f;
-#pragma unroll
-                            for (int mb = 0; mb < MB; mb++) acc[win][mb][v] = __builtin_fmaf(s, __builtin_fmaf(-zc, x[mb][v], pr[win][mb][v]), acc[win][mb][v]);
-                        }
+                        for (int mb = 0; mb < MB; mb++) acc[mb][v] = __builtin_fmaf(s, ZP ? __builtin_fmaf(-zc, x[t][g][mb], pr[mb][v]) : pr[mb][v] + x[t][g][mb], acc[mb][v]);
+                    }
                 }
-        }
+                load(win + R, t, I);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int mb = 0; mb < MB; mb++) {
+                v4f* at = part + ((wave * windows + win) * MB + mb) * 64 + lane;
+                *at = pass ? *at + acc[mb] : acc[mb];
+            }
+        };
+        int w0 = 0;
+        for (; w0 + R <= windows; w0 += R) static_for<R>([&](auto I) { window(w0 + decltype(I)::value, I); });
+        static_for<R - 1>([&](auto I) {
+            if (w0 + decltype(I)::value < windows) window(w0 + decltype(I)::value, I);
+        });
     }
 
-    // the K slices' sums, in their order
-#pragma unroll
-    for (int w = 0; w < NWIN; w++)
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) part[wave][(w * MB + mb) * 64 + lane] = acc[w][mb];
     __syncthreads();
-    for (int t = tid; t < gpw * NWIN * MB * 64; t += NWAVES * 64) {
-        const int g = (t >> 6) / (NWIN * MB), frag = (t >> 6) % (NWIN * MB), gq = bid * gpw + g;
-        const int m = (frag % MB) * 16 + li, n = (gq < p.groups ? unit_begin(gq) * 8 : 0) + (frag / MB) * 16 + lg * 4, ne = gq < p.groups ? unit_begin(gq + 1) * 8 : 0;
-        if (n >= ne || m >= M) continue;
-        v4f sum = part[g << ksh][frag * 64 + lane];
-        for (int j = 1; j < p.ks; j++) sum += part[(g << ksh) + j][frag * 64 + lane];
+    // the slices' sums, in their order
+    for (int t = tid; t < windows * MB * 64; t += W4_WAVES * 64) {
+        const int frag = t >> 6, m = (frag % MB) * 16 + li, n = n_begin + (frag / MB) * 16 + lg * 4;
+        if (n >= n_end || m >= M) continue;
+        v4f sum = part[t];
+#pragma unroll
+        for (int j = 1; j < W4_WAVES; j++) sum += part[j * windows * MB * 64 + t];
         store_c4(p, (size_t)(m0 + m) * (size_t)p.N + (size_t)n, n, sum);
     }
 }
 
-template <bool BF16, int GS, bool ZP>
-hipError_t launch(W4Params p, hipStream_t stream) {
-    constexpr int NWAVES = 8, CH = 4;
-    const int steps = (p.K + 127) / 128, mb = p.M > 16 ? 2 : 1, rows = (p.M + 31) / 32;
-    int ks = NWAVES;
-    while (ks > 1 && ks > steps) ks >>= 1;
-    const int gpw = NWAVES / ks;
-    const long units = p.N / 8, cus = psg_cu_count();
-    const long rounds = (units + 4 * cus * gpw - 1) / (4 * cus * gpw);
-    long tg = cus * gpw * rounds;
-    if (tg > units) tg = units;
-    p.ks = ks, p.groups = (int)tg, p.unit_q = (int)(units / tg), p.unit_r = (int)(units % tg);
-    const bool two = (units + tg - 1) / tg > 2;
-    const dim3 grid((unsigned)((tg + gpw - 1) / gpw), (unsigned)rows);
-    if (mb == 1 && two) hipLaunchKernelGGL((k_w4a16<BF16, 1, 2, GS, ZP, NWAVES, CH>), grid, dim3(NWAVES * 64), 0, stream, p);
-    else if (mb == 1) hipLaunchKernelGGL((k_w4a16<BF16, 1, 1, GS, ZP, NWAVES, CH>), grid, dim3(NWAVES * 64), 0, stream, p);
-    else if (two) hipLaunchKernelGGL((k_w4a16<BF16, 2, 2, GS, ZP, NWAVES, 2>), grid, dim3(NWAVES * 64), 0, stream, p);
-    else hipLaunchKernelGGL((k_w4a16<BF16, 2, 1, GS, ZP, NWAVES, 2>), grid, dim3(NWAVES * 64), 0, stream, p);
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int R>
+hipError_t go(W4Params p, hipStream_t stream) {
+    const int steps = (p.K + 127) / 128;
+    p.passes = (steps + W4_WAVES * SPW - 1) / (W4_WAVES * SPW);
+    p.per = (steps + W4_WAVES * p.passes - 1) / (W4_WAVES * p.passes);
+    // units of 8 columns: at most `most` a workgroup (its sums take 1 KB of LDS a wavefront, window and 16-row block, 64 KB in all), a whole number of workgroups a CU
+    const long units = p.N / 8, cus = psg_cu_count(), most = 16 / MB, rounds = (units + most * cus - 1) / (most * cus), wgs = units < cus * rounds ? units : cus * rounds;
+    p.unit_q = (int)(units / wgs), p.unit_r = (int)(units % wgs);
+    const long windows = (units + wgs - 1) / wgs + 1 >> 1;
+    hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, R>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), (size_t)windows * MB * W4_WAVES * 1024, stream, p);
     return hipGetLastError();
+}
+
+template <bool BF16, int GS, bool ZP>
+hipError_t launch(const W4Params& p, hipStream_t stream) {
+    // steps of K that a wavefront has: the least part of A that holds them, or the largest
+    const int per = ((p.K + 127) / 128 + W4_WAVES - 1) / W4_WAVES;
+    constexpr int AHEAD = GS == 32 ? 4 : 8;  // steps asked for ahead
+    if (p.M <= 16) {
+        if (per <= 2) return go<BF16, 1, GS, ZP, 2, AHEAD / 2>(p, stream);
+        if (per <= 4 || GS == 32) return go<BF16, 1, GS, ZP, 4, AHEAD / 4>(p, stream);
+        return go<BF16, 1, GS, ZP, GS == 32 ? 4 : 8, 1>(p, stream);
+    }
+    if (per <= 2 || GS == 32) return go<BF16, 2, GS, ZP, 2, AHEAD / 2>(p, stream);
+    return go<BF16, 2, GS, ZP, GS == 32 ? 2 : 4, GS == 32 ? AHEAD / 2 : AHEAD / 4>(p, stream);
 }
 
 template <bool BF16, int GS>
