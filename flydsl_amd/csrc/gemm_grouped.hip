@@ -70,6 +70,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
         constexpr int S = decltype(I)::value & 1, set = decltype(I)::value % SETS;
         load_a(kt + 3, (set + 3) % SETS);
         load_w(kt + 3, (set + 3) % SETS);
+        // (addresses in front, MFMAs behind: one that writes a register has two wait states to the vector instruction that wrote it last)
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 1");
 #pragma unroll
         for (int mi = 0; mi < MR; mi++) {
             const v4i alo = *reinterpret_cast<const v4i*>(&lds[S][lds_off(mi * 16 + li, lg)]), ahi = *reinterpret_cast<const v4i*>(&lds[S][lds_off(mi * 16 + li, 4 + lg)]);

@@ -7,16 +7,24 @@
 // in fp32, and X of a lane's own row is what the same MFMA gives for a weight of ones.  (P is at most 31/16 of the sum with the 16 alone: the difference loses four or five of 24
 // bits, far below the 16-bit output's rounding.)
 //
-// Bound: the weights' way from memory.  The columns are dealt out in units of 8, evenly, one workgroup a CU; its eight wavefronts are eight slices of K.  A wavefront's part of A, 16
-// rows of up to 1024 elements, stays in registers (128 of them) while the workgroup's columns go by in windows of 16, and so do the X of its groups: what moves is W alone, asked for
-// eight steps ahead, windows on end, without a barrier.  The slices' sums meet in LDS in a fixed order: one launch, no workspace.  Longer rows take several passes over the
-// columns, each with its part of A.
+// Bound: the weights' way from memory, and at a few MB of them the 3 us that a launch takes whatever it reads.  The columns are dealt out in units of 8, evenly, over one workgroup a CU;
+// its eight wavefronts are eight slices of K.  A wavefront's part of A (SPW steps of 128 elements of the 16 rows) stays in registers while the workgroup's columns go by in windows of 16,
+// the sums X of its groups too: what moves is W alone, the next window asked for as this one's registers become free, without a barrier.  The slices' sums meet in LDS in a fixed order:
+// one launch, no workspace.  Rows too long for the registers take several passes over the columns; the next pass's part of A comes into LDS meanwhile, and W does not wait
+// at their ends.
+//   * A comes row by row, by DMA, only the rows there are: as fragments, 16 rows times 64 bytes an instruction and those of absent rows too, they took the address units longer than
+//     the weights (16x6144x4096 8.1 us against 6.2, 1x2048x2048 5.0 / 3.4).
+//   * A lane of every 16 reads the scales (and zero points) of one group for its four columns; the others take them from it by DPP.  One load a window instead of one a group (5x1040x2080,
+//     groups of 32, 6.0 / 4.8).
+//   * Reading A once and not once for every four units of columns: 16x28672x8192 58 -> 25, 5.0 TB/s.
+//   Deeper prefetch (two windows), sixteen wavefronts and A read from LDS for every window were level or slower.
 //
 // Layout: W in blocks of 16 rows x 128 elements, 1 KB: lane l = 16 g + r of a wavefront reads 16 bytes, row r, dword j of them elements 32 j + 8 g .. + 7, what
 // it multiplies in MFMA j; the even ones are the nibbles of the lower half of the dword, the odd ones those of the upper half, so that two of them are a mask away from a
 // packed pair.  Rows end on whole blocks (elements past K are not looked at: A reads as zero there and X with it).  Scales [N/16][K/group][16], zero points the same as
 // nibbles, lower one first: a lane's four columns are 8 and 2 bytes.
 #include "gemm_w4a16.h"
+#include "lds_dma.h"
 
 namespace {
 
@@ -35,94 +43,142 @@ __device__ __forceinline__ v4f mfma16(v4i w, v4i a, v4f c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, a), c, 0, 0, 0);
 }
 
-constexpr int W4_WAVES = 8;
+// lane n of every 16
+template <int N>
+__device__ __forceinline__ int of_lane(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x150 + N, 0xF, 0xF, true); }
 
-// MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  R: windows that are asked for ahead.
-template <bool BF16, int MB, int GS, bool ZP, int SPW, int R>
+constexpr int W4_WAVES = 8, W4_LDS = 160 * 1024;
+
+// MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  SH: those that come through LDS at a time.  MANY: several
+// passes.
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY>
 __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
-    constexpr int GPS = 128 / GS, MPG = GS / 32;  // groups of a step, MFMAs of a group
-    extern __shared__ v4f part[];                 // [wavefront][window][16-row block][lane]
+    constexpr int NW = W4_WAVES;
+    constexpr int GPS = 128 / GS, MPG = GS / 32;              // groups of a step, MFMAs of a group
+    constexpr int CPR = SH * 16, PATCH = MB * 16 * CPR * 16;  // 16-byte pieces of a staged row, bytes of a wavefront's patch
+    static_assert(SPW * GPS <= 16, "a load of scales holds 16 groups");
+    static_assert(!MANY || SH == SPW, "the next pass's part of A lies in the patch");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[MANY ? W4_LDS : NW * PATCH];
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
     auto unit_begin = [&](int g) { return g * p.unit_q + (g < p.unit_r ? g : p.unit_r); };
     // an XCD owns one range of columns: workgroups go round the XCDs
     const int wg = (gridDim.x & 7) == 0 ? (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3)) : (int)blockIdx.x;
     const int n_begin = unit_begin(wg) * 8, n_end = unit_begin(wg + 1) * 8, windows = (n_end - n_begin + 15) >> 4;
-    const int m0 = (int)blockIdx.y * MB * 16, M = p.M - m0, K = p.K, steps = (K + 127) >> 7, groups = K / GS;
+    const int m0 = (int)blockIdx.y * MB * 16, M = p.M - m0 < MB * 16 ? p.M - m0 : MB * 16, K = p.K, steps = (K + 127) >> 7, groups = K / GS;
 
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w, (uint64_t)p.N * (uint64_t)steps * 64ull), rs = make_rsrc(p.scales, (uint64_t)p.N * (uint64_t)groups * 2ull),
                                  rz = make_rsrc(ZP ? p.zeros : p.w, (uint64_t)p.N * (uint64_t)groups / 2ull),
-                                 ra = make_rsrc(static_cast<const uint16_t*>(p.a) + (uint64_t)m0 * (uint64_t)K, (uint64_t)M * (uint64_t)K * 2ull);
-    // a lane reads row n of W, and the scales of the four columns from c on that it holds of C; a window is 16 rows on
+                                 ra = make_rsrc_uniform(static_cast<const uint16_t*>(p.a) + (uint64_t)m0 * (uint64_t)K, (uint64_t)M * (uint64_t)K * 2ull);
+    // a lane reads row n of W; of the scales it reads group li's for the four columns from c on that it holds of C; a window is 16 rows on
     const int n_lane = n_begin + li, c_lane = n_begin + lg * 4;
     const uint32_t w_lane = (uint32_t)(n_lane >> 4) * (uint32_t)steps * 1024u + (uint32_t)(lg * 256 + (n_lane & 15) * 16);
-    const uint32_t s_lane = (uint32_t)(c_lane >> 4) * (uint32_t)groups * 32u + (uint32_t)(c_lane & 15) * 2u;
-    uint32_t a_lane[MB];
-#pragma unroll
-    for (int mb = 0; mb < MB; mb++) a_lane[mb] = mb * 16 + li < M ? (uint32_t)(mb * 16 + li) * (uint32_t)K * 2u + (uint32_t)lg * 16u : OOB;
+    const uint32_t s_lane = (uint32_t)(c_lane >> 4) * (uint32_t)groups * 32u + (uint32_t)(c_lane & 15) * 2u + (uint32_t)li * 32u;
     const Join<BF16 ? 0x00780078 : 0x03C003C0, BF16 ? 0x41804180 : 0x4C004C00> code;  // a code in the bits of the mantissa that count 1 to 8 beside 16
     const Join<0x00780000, 0x41800000> zero;                                           // the same in fp32
+    uint8_t* const patch = lds + wave * PATCH;
+    // [window][16-row block][lane], wavefronts `apart`: in the patch, free again once A is in registers, or beside it
+    const int apart = MANY ? windows * MB * 64 : PATCH / 16;
+    v4f* const all = reinterpret_cast<v4f*>(MANY ? lds + NW * PATCH : lds);
+    auto first = [&](int pass) { return (pass * NW + wave) * p.per; };
+    auto last = [&](int pass) { const int e = first(pass) + p.per; return e < steps ? e : steps; };
 
-    for (int pass = 0; pass < p.passes; pass++) {
-        const int s0 = (pass * W4_WAVES + wave) * p.per, s1 = s0 + p.per < steps ? s0 + p.per : steps;
-        v4i w[R][SPW];
-        v2i sc[R][SPW][GPS];
-        int z[R][SPW][ZP ? GPS : 1];
-        auto load = [&](int win, int t, auto I) __attribute__((always_inline)) {
-            constexpr int i = decltype(I)::value;
-            const bool in = win < windows && s0 + t < s1;  // uniform
-            const bool row = in && n_lane + win * 16 < n_end, col = in && c_lane + win * 16 < n_end;
-            w[i][t] = buf_load16_nt(rw, row ? w_lane : OOB, in ? ((uint32_t)win * (uint32_t)steps + (uint32_t)(s0 + t)) * 1024u : 0u);
+    v4i w[SPW];
+    v2i sc;
+    int z = 0;
+    int l_pass = 0, l_win = 0;  // what is asked for next: windows on end, pass after pass
+    auto load_w = [&](int t) __attribute__((always_inline)) {
+        const int s = first(l_pass) + t;
+        const bool in = (MANY ? l_pass < p.passes : l_win < windows) && s < last(l_pass);  // uniform
+        w[t] = buf_load16_nt(rw, in && n_lane + l_win * 16 < n_end ? w_lane : OOB, in ? ((uint32_t)l_win * (uint32_t)steps + (uint32_t)s) * 1024u : 0u);
+    };
+    auto load_s = [&]() __attribute__((always_inline)) {
+        const int at = first(l_pass) * GPS, e = last(l_pass) * GPS < groups ? last(l_pass) * GPS : groups;
+        const bool in = MANY ? l_pass < p.passes : l_win < windows, has = in && at + li < e && c_lane + l_win * 16 < n_end;
+        const uint32_t so = in ? (uint32_t)l_win * (uint32_t)groups + (uint32_t)at : 0u;
+        sc = buf_load8(rs, has ? s_lane : OOB, so * 32u);
+        // (all zero points are less than 2^27 bytes: a quarter of OOB lies behind them too)
+        if constexpr (ZP) z = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rz, (int)(has ? s_lane >> 2 : OOB), (int)(so * 8u), 0);
+        l_win++;
+        if (MANY && l_win == windows) l_win = 0, l_pass++;
+    };
+    // part of A, SH steps at a time: rows by DMA into the wavefront's patch (16-byte pieces XORed with the row), from there in fragments
+    const int pieces = (M * CPR + 63) >> 6;
+    auto stage = [&](int pass, int h) __attribute__((always_inline)) {
+        const int k0 = (first(pass) + h * SH) * 128, ke = last(pass) * 128 < K ? last(pass) * 128 : K;
+        for (int i = 0; i < pieces; i++) {
+            const int q = i * 64 + lane, row = q / CPR, k = k0 + ((q % CPR) ^ (row & 15)) * 8;
+            dma16(ra, (uint32_t)(uintptr_t)patch + (uint32_t)i * 1024u, row < M && k < ke ? (uint32_t)row * (uint32_t)K * 2u + (uint32_t)k * 2u : OOB, 0u);
+        }
+    };
+    stage(0, 0);
 #pragma unroll
-            for (int g = 0; g < GPS; g++) {
-                const int at = (s0 + t) * GPS + g;
-                const bool has = in && at < groups;
-                const uint32_t so = has ? (uint32_t)win * (uint32_t)groups + (uint32_t)at : 0u;
-                sc[i][t][g] = buf_load8(rs, col && has ? s_lane : OOB, so * 32u);
-                if constexpr (ZP) z[i][t][g] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rz, (int)(col && has ? s_lane >> 2 : OOB), (int)(so * 8u), 0);
-            }
-        };
+    for (int t = 0; t < SPW; t++) load_w(t);
+    load_s();
+    __builtin_amdgcn_sched_barrier(0);
+
+    for (int pass = 0; pass < (MANY ? p.passes : 1); pass++) {
         v4i a[SPW][4][MB];
+        // the part has landed once only what was asked for behind it, a window of W at least, is on its way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SPW + (ZP ? 2 : 1)) : "memory");
 #pragma unroll
-        for (int t = 0; t < SPW; t++)
+        for (int h = 0; h < SPW / SH; h++) {
+            if (h) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                stage(pass, h);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int t = 0; t < SH; t++)
 #pragma unroll
-                for (int mb = 0; mb < MB; mb++) {
-                    const int k = (s0 + t) * 128 + j * 32;
-                    const bool in = s0 + t < s1 && k < K;  // (K is a multiple of 32)
-                    a[t][j][mb] = buf_load16(ra, in ? a_lane[mb] : OOB, in ? (uint32_t)k * 2u : 0u);
-                }
-        static_for<R>([&](auto I) {
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int t = 0; t < SPW; t++) load(decltype(I)::value, t, I);
-        });
-        __builtin_amdgcn_sched_barrier(0);
+                    for (int mb = 0; mb < MB; mb++) {
+                        const int r = mb * 16 + li < M ? mb * 16 + li : M - 1;  // (rows past M: any, they are not written)
+                        a[h * SH + t][j][mb] = *reinterpret_cast<const v4i*>(patch + r * (CPR * 16) + (((t * 16 + j * 4 + lg) ^ (r & 15)) << 4));
+                    }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (MANY && pass + 1 < p.passes) stage(pass + 1, 0);
 
         // X of every group, times -24 without zero points
         float x[SPW][GPS][MB];
         const int one = BF16 ? (ZP ? 0x3F803F80 : (int)0xC1C0C1C0) : (ZP ? 0x3C003C00 : (int)0xCE00CE00);
         const v4i ones = {one, one, one, one};
 #pragma unroll
-        for (int t = 0; t < SPW; t++)
+        for (int t = 0; t < SPW; t++) {
+            v4f y[GPS][MB];
 #pragma unroll
             for (int g = 0; g < GPS; g++)
 #pragma unroll
                 for (int mb = 0; mb < MB; mb++) {
-                    v4f y = {0.f, 0.f, 0.f, 0.f};
+                    y[g][mb] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int j = g * MPG; j < (g + 1) * MPG; j++) y = mfma16<BF16>(ones, a[t][j][mb], y);
-                    x[t][g][mb] = y[0];
+                    for (int j = g * MPG; j < (g + 1) * MPG; j++) y[g][mb] = mfma16<BF16>(ones, a[t][j][mb], y[g][mb]);
                 }
+            // (all four rows of a result are the same; whole until they are there, so that no later MFMA's registers overlap one that is on its way)
+#pragma unroll
+            for (int g = 0; g < GPS; g++)
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) asm volatile("" : "+v"(y[g][mb]));
+            asm volatile("s_nop 7");
+#pragma unroll
+            for (int g = 0; g < GPS; g++)
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) x[t][g][mb] = y[g][mb][0];
+            __builtin_amdgcn_sched_barrier(0);
+        }
 
-        auto window = [&](int win, auto I) __attribute__((always_inline)) {
-            constexpr int i = decltype(I)::value;
+        for (int win = 0; win < windows; win++) {
+            v4f* const at = all + wave * apart + win * MB * 64 + lane;
             v4f acc[MB];
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) acc[mb] = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int t = 0; t < SPW; t++) {
-#pragma unroll
-                for (int g = 0; g < GPS; g++) {
+            for (int mb = 0; mb < MB; mb++) acc[mb] = MANY && pass ? at[mb * 64] : (v4f){0.f, 0.f, 0.f, 0.f};
+            const v2i sc_ = sc;
+            const int z_ = z;
+            static_for<SPW>([&](auto T) {
+                constexpr int t = decltype(T)::value;
+                static_for<GPS>([&](auto G) {
+                    constexpr int g = decltype(G)::value, q0 = t * GPS + g;
                     v4f pr[MB];
 #pragma unroll
                     for (int mb = 0; mb < MB; mb++) pr[mb] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -130,71 +186,76 @@ __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
                     for (int j = g * MPG; j < (g + 1) * MPG; j++) {
                         v4i b;
 #pragma unroll
-                        for (int q = 0; q < 4; q++) b[q] = code(shift(w[i][t][j], (BF16 ? 3 : 6) - 4 * q));
+                        for (int q = 0; q < 4; q++) b[q] = code(shift(w[t][j], (BF16 ? 3 : 6) - 4 * q));
 #pragma unroll
                         for (int mb = 0; mb < MB; mb++) pr[mb] = mfma16<BF16>(b, a[t][j][mb], pr[mb]);
                     }
+                    const int s2[2] = {of_lane<q0>(sc_[0]), of_lane<q0>(sc_[1])};
+                    const int z4 = ZP ? of_lane<q0>(z_) : 0;
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const float s = from_out16<BF16 ? OUT_BF16 : OUT_FP16>((uint16_t)((uint32_t)sc[i][t][g][v >> 1] >> (16 * (v & 1))));
-                        const float zc = ZP ? __builtin_bit_cast(float, zero(z[i][t][g] << (19 - 4 * v))) : 0.f;
+                        const float s = from_out16<BF16 ? OUT_BF16 : OUT_FP16>((uint16_t)((uint32_t)s2[v >> 1] >> (16 * (v & 1))));
+                        const float zc = ZP ? __builtin_bit_cast(float, zero(z4 << (19 - 4 * v))) : 0.f;
 #pragma unroll
                         for (int mb = 0; mb < MB; mb++) acc[mb][v] = __builtin_fmaf(s, ZP ? __builtin_fmaf(-zc, x[t][g][mb], pr[mb][v]) : pr[mb][v] + x[t][g][mb], acc[mb][v]);
                     }
-                }
-                load(win + R, t, I);
+                });
+                load_w(t);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+            });
+            load_s();
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) {
-                v4f* at = part + ((wave * windows + win) * MB + mb) * 64 + lane;
-                *at = pass ? *at + acc[mb] : acc[mb];
-            }
-        };
-        int w0 = 0;
-        for (; w0 + R <= windows; w0 += R) static_for<R>([&](auto I) { window(w0 + decltype(I)::value, I); });
-        static_for<R - 1>([&](auto I) {
-            if (w0 + decltype(I)::value < windows) window(w0 + decltype(I)::value, I);
-        });
+            for (int mb = 0; mb < MB; mb++) at[mb * 64] = acc[mb];
+        }
     }
 
     __syncthreads();
     // the slices' sums, in their order
-    for (int t = tid; t < windows * MB * 64; t += W4_WAVES * 64) {
+    for (int t = tid; t < windows * MB * 64; t += NW * 64) {
         const int frag = t >> 6, m = (frag % MB) * 16 + li, n = n_begin + (frag / MB) * 16 + lg * 4;
         if (n >= n_end || m >= M) continue;
-        v4f sum = part[t];
+        v4f sum = all[t];
 #pragma unroll
-        for (int j = 1; j < W4_WAVES; j++) sum += part[j * windows * MB * 64 + t];
+        for (int j = 1; j < NW; j++) sum += all[j * apart + t];
         store_c4(p, (size_t)(m0 + m) * (size_t)p.N + (size_t)n, n, sum);
     }
 }
 
-template <bool BF16, int MB, int GS, bool ZP, int SPW, int R>
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY>
 hipError_t go(W4Params p, hipStream_t stream) {
     const int steps = (p.K + 127) / 128;
     p.passes = (steps + W4_WAVES * SPW - 1) / (W4_WAVES * SPW);
     p.per = (steps + W4_WAVES * p.passes - 1) / (W4_WAVES * p.passes);
-    // units of 8 columns: at most `most` a workgroup (its sums take 1 KB of LDS a wavefront, window and 16-row block, 64 KB in all), a whole number of workgroups a CU
-    const long units = p.N / 8, cus = psg_cu_count(), most = 16 / MB, rounds = (units + most * cus - 1) / (most * cus), wgs = units < cus * rounds ? units : cus * rounds;
+    // a workgroup has LDS for the sums of so many windows of 16 columns, which begin at a multiple of 8
+    constexpr int PATCH = MB * SH * 4096, windows = MANY ? (W4_LDS - W4_WAVES * PATCH) / (W4_WAVES * MB * 1024) : PATCH / (MB * 1024), most = 2 * windows - 1;
+    const long units = p.N / 8, cus = psg_cu_count(), rounds = (units + most * cus - 1) / (most * cus), wgs = units < cus * rounds ? units : cus * rounds;
     p.unit_q = (int)(units / wgs), p.unit_r = (int)(units % wgs);
-    const long windows = (units + wgs - 1) / wgs + 1 >> 1;
-    hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, R>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), (size_t)windows * MB * W4_WAVES * 1024, stream, p);
+    hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, SH, MANY>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), 0, stream, p);
     return hipGetLastError();
 }
 
 template <bool BF16, int GS, bool ZP>
 hipError_t launch(const W4Params& p, hipStream_t stream) {
-    // steps of K that a wavefront has: the least part of A that holds them, or the largest
-    const int per = ((p.K + 127) / 128 + W4_WAVES - 1) / W4_WAVES;
-    constexpr int AHEAD = GS == 32 ? 4 : 8;  // steps asked for ahead
-    if (p.M <= 16) {
-        if (per <= 2) return go<BF16, 1, GS, ZP, 2, AHEAD / 2>(p, stream);
-        if (per <= 4 || GS == 32) return go<BF16, 1, GS, ZP, 4, AHEAD / 4>(p, stream);
-        return go<BF16, 1, GS, ZP, GS == 32 ? 4 : 8, 1>(p, stream);
+    const int per = ((p.K + 127) / 128 + W4_WAVES - 1) / W4_WAVES;  // steps of a wavefront
+    // 17 to 32 rows read W once where A fits the registers, else 16 rows at a time: 32x7168x2048 8.1 / 5.9, 32x4096x4096 8.6 / 6.8; in several passes of 32 rows 32x8192x8192 took 22.8, like this 19.9,
+    // 32x28672x4096 in groups of 32 47 / 34
+    if (p.M > 16) {
+        if (per <= 2) return go<BF16, 2, GS, ZP, 2, 2, false>(p, stream);
+        if constexpr (GS == 128) {
+            if (per <= 4) return go<BF16, 2, GS, ZP, 4, 2, false>(p, stream);
+        }
     }
-    if (per <= 2 || GS == 32) return go<BF16, 2, GS, ZP, 2, AHEAD / 2>(p, stream);
-    return go<BF16, 2, GS, ZP, GS == 32 ? 2 : 4, GS == 32 ? AHEAD / 2 : AHEAD / 4>(p, stream);
+    if (per <= 2) return go<BF16, 1, GS, ZP, 2, 2, false>(p, stream);
+    if (per <= 4) return go<BF16, 1, GS, ZP, 4, 4, false>(p, stream);
+    // eight steps fit with the sums of eight groups, not with those of 16 (the build spilled: 4x5120x6144 in groups of 64 29 us, in passes 9)
+    if constexpr (GS == 128) {
+        if (per <= 8) return go<BF16, 1, GS, ZP, 8, 4, false>(p, stream);
+    }
+    // Passes of four steps leave LDS for four windows a workgroup, passes of two for twelve.  us four / two: 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but more windows a CU
+    // 16x28672x8192 in groups of 64 36.7 / 33.6, five and six steps, which two divide better, 4x5120x6144 10.0 / 9.0, 1x6144x6144 9.9 / 8.7, and groups of 32 with zero points,
+    // which take all registers, 2x8192x10240 16.9 / 14.9
+    if (per <= 6 || p.N > 56 * psg_cu_count() || (GS == 32 && ZP)) return go<BF16, 1, GS, ZP, 2, 2, true>(p, stream);
+    return go<BF16, 1, GS, ZP, 4, 4, true>(p, stream);
 }
 
 template <bool BF16, int GS>

@@ -1,6 +1,6 @@
 """GPU tests of the products with 4-bit weights and group scales against their definition in 64 bits.
 
-Exact inputs: activations are whole numbers up to 8 and scales powers of two, so that every partial sum (at most K * 8 * 31 < 2^24) is exact in fp32 whatever its order: the output
+Exact inputs: activations are whole numbers up to 8 and scales powers of two, so that every partial sum (at most K * 8 * 15 steps of a quarter of the largest scale, below 2^24) is exact in fp32 whatever its order: the output
 is the definition, rounded once to 16 bits, to the bit.
 Random inputs: with u = 2^-23 for every addition in whatever order, a group's sum of codes and the sum of activations times 16 + zero are off by at most group * u * 31 * sum|a| each, the
 groups' sums by another (K / group + 8) u of their magnitudes; then the rounding to 16 bits, and what the activation function makes of the error (its slope is at most 1.13)
@@ -61,7 +61,8 @@ def _run(a, codes, scale, zero, bias, group, dtype, epi, guard=3):
     return c[:m].cpu()
 
 
-SIZES = [(1, 16, 128), (1, 4096, 4096), (2, 2064, 1152), (5, 1040, 2176), (16, 48, 11008), (17, 512, 640), (32, 7168, 2048), (33, 272, 512), (100, 1024, 1024), (3, 28672, 256), (16, 8208, 384)]
+SIZES = [(1, 16, 128), (1, 4096, 4096), (2, 2064, 1152), (5, 1040, 2176), (16, 48, 11008), (17, 512, 640), (32, 7168, 2048), (33, 272, 512), (100, 1024, 1024), (3, 28672, 256), (16, 8208, 384), (20, 1040, 4096), (16, 2064, 8192),
+         (8, 528, 6144), (3, 32992, 5120), (1, 16, 32768), (9, 14352, 7168)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
