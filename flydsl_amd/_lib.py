@@ -374,6 +374,7 @@ def address(name: str) -> int:
 
 TYPE_ANY, TYPE_INT32, TYPE_FP32, TYPE_BF16, TYPE_FP16 = range(5)
 OPTIONAL = 256  # added to a type: None may stand in the operand's place
+EXACT = 1024  # added to a type: exactly that many bytes
 ROWS = 512  # added to a type: the operand is [rows, columns] (``rows << 32 | columns`` in the place of the bytes) with dense rows any distance apart, which the struct holds behind the address
 
 
@@ -419,6 +420,19 @@ def stream_on(stream, device) -> int:
 
         return int(torch.cuda.current_stream(device).cuda_stream)
     return stream_handle(stream)
+
+
+_devices = 0
+
+
+def is_current(index: int) -> bool:
+    """Whether ``index`` is the current device, where kernels are loaded and launched."""
+    global _devices
+    import torch
+
+    if not _devices:
+        _devices = torch.cuda.device_count()
+    return _devices == 1 or torch.cuda.current_device() == index
 
 
 def launch_on(device, fn, *args) -> int:

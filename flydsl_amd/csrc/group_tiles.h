@@ -10,6 +10,13 @@ struct GroupParams {
     int most;  // set by the launcher: tiles along M that the grid was made for (offsets that go back may say more)
 };
 
+// Rows of a tile (16, 32, 64 or 128), and whether K is cut into slices (16 rows only)
+struct GroupedPlan {
+    int bm;
+    bool sliced;
+};
+GroupedPlan psg_grouped_plan(int64_t rows, int groups, int N, int64_t kbytes);
+hipError_t psg_launch_grouped(const A8W8Params& p, const GroupParams& g, int kind, GroupedPlan plan, hipStream_t stream);
 hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream);
 
 // Upper bound of the tiles of `bm` rows that the rows of `groups` groups make, for the grid: a group's last tile may be almost empty, a group without rows makes none
@@ -24,6 +31,18 @@ struct GroupTile {
     int n_tile;  // tile along N
 };
 
+// sum over the lanes up to this one: inside rows of 16 by shifts, then the last lane of a row to the one behind it, of the first half to the second (by DPP: six exchanges through
+// LDS would be half a microsecond in front of every tile)
+__device__ __forceinline__ int sum_upto(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // Workgroup `wg` of the launch -> its tile; false for the workgroups that the bound of the grid counts too many.  Every wavefront works it out by itself, a group a lane: no
 // barrier; uniform.  Tiles are walked as in psg_tile_order, eight of them along M at a time, so that an XCD reads a group's weight once.
 __device__ __forceinline__ bool group_tile(const GroupParams& g, int M, int bm, int wg, int n_tiles, int lane, GroupTile& t) {
@@ -35,11 +54,7 @@ __device__ __forceinline__ bool group_tile(const GroupParams& g, int M, int bm, 
         const int end = b < 0 ? 0 : b < M ? b : M;
         rows = end > row ? end - row : 0;
         upto = (int)((unsigned)(rows + bm - 1) / (unsigned)bm);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(upto, d);
-            upto += lane >= d ? v : 0;
-        }
+        upto = sum_upto(upto);
     };
     int row, rows, upto, total = 0;
     look(0, row, rows, upto);

@@ -24,9 +24,9 @@ struct Operand {
     int32_t offset;  // of the address in it
     int32_t item;    // bytes of an element, 0 = any
     int32_t type;    // TYPE_*, plus OPTIONAL where None may stand in the operand's place, ROWS for one that need not be contiguous
-    int64_t need;    // least bytes; ROWS: rows << 32 | columns, which it has exactly
+    int64_t need;    // least bytes (EXACT: just so many); ROWS: rows << 32 | columns, which it has exactly
 };
-enum { TYPE_ANY = 0, TYPE_INT32 = 1, TYPE_FP32 = 2, TYPE_BF16 = 3, TYPE_FP16 = 4, OPTIONAL = 256, ROWS = 512 };
+enum { TYPE_ANY = 0, TYPE_INT32 = 1, TYPE_FP32 = 2, TYPE_BF16 = 3, TYPE_FP16 = 4, OPTIONAL = 256, ROWS = 512, EXACT = 1024 };
 
 bool type_is(const at::Tensor& t, int type) {
     switch (type) {
@@ -116,15 +116,16 @@ PyObject* launch(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (op.arg < 0 || op.arg >= structs || op.offset < 0 || op.offset + (Py_ssize_t)sizeof(void*) > size[op.arg]) return DECLINED;
             const bool rows = op.type & ROWS;
             const at::Tensor* t = operand(a[4 + i], device, rows);
-            if (!t || (op.item && (int64_t)t->element_size() != op.item) || !type_is(*t, op.type & ~(OPTIONAL | ROWS))) return DECLINED;
+            if (!t || (op.item && (int64_t)t->element_size() != op.item) || !type_is(*t, op.type & ~(OPTIONAL | ROWS | EXACT))) return DECLINED;
             if (rows) {
                 const int64_t n = op.need >> 32, cols = op.need & 0xFFFFFFFF;
                 if (t->layout() != at::kStrided || t->dim() != 2 || t->size(0) != n || t->size(1) != cols || (cols > 1 && t->stride(1) != 1) || (n > 1 && t->stride(0) < cols)) return DECLINED;
                 const int64_t apart = n > 1 ? t->stride(0) : 0;
                 if (op.offset + 16 > size[op.arg]) return DECLINED;
                 memcpy(arg[op.arg] + op.offset + 8, &apart, sizeof(apart));
-            } else if (t->numel() * (int64_t)t->element_size() < op.need) {
-                return DECLINED;
+            } else {
+                const int64_t bytes = t->numel() * (int64_t)t->element_size();
+                if (op.type & EXACT ? bytes != op.need : bytes < op.need) return DECLINED;
             }
             void* p = t->data_ptr();
             memcpy(arg[op.arg] + op.offset, &p, sizeof(p));

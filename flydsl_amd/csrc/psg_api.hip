@@ -42,8 +42,6 @@ hipError_t psg_launch_quant_pertoken(const void* x, int x_dtype, void* y, float*
 hipError_t psg_launch_quant_mxfp4(const void* x, int x_dtype, void* packed, void* scales, int M, int R, int K, int shuffled,
                                   hipStream_t stream);
 hipError_t psg_launch_w4a16(const W4Params& p, int group, hipStream_t stream);
-int psg_grouped_tile(int64_t rows, int groups);
-hipError_t psg_launch_grouped(const A8W8Params& p, const GroupParams& g, int kind, int bm, hipStream_t stream);
 hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream);
 
 // Scratch of the entry point that allocates nothing (psg_gemm_a8w8_static): the split-K partial sums of the tiled
@@ -1401,8 +1399,9 @@ int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
     if ((uint64_t)a->N * (uint64_t)a->K * (uint64_t)eb >= OOB) return fail(PSG_E_SHAPE, "N*K bytes exceed the 4 GiB descriptor range");
     if (128ull * (uint64_t)a->K * (uint64_t)eb >= OOB || 128ull * (uint64_t)a->N * 2ull >= OOB) return fail(PSG_E_SHAPE, "128 rows of a or c exceed the 4 GiB descriptor range");
     if (a->tile_rows != 0 && a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64 or 128", a->tile_rows);
-    const int bm = a->tile_rows ? a->tile_rows : psg_grouped_tile(a->M, a->groups);
-    if (group_tiles_most(a->M, a->groups, bm) * ((a->N + 63ll) / 64) > 0x7FFFFFFFll) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
+    const GroupedPlan plan = a->tile_rows ? GroupedPlan{a->tile_rows, false} : psg_grouped_plan(a->M, a->groups, a->N, a->K * eb);
+    const int tn = plan.sliced ? 16 : plan.bm <= 32 ? 64 : 2 * plan.bm;  // columns of a tile
+    if (group_tiles_most(a->M, a->groups, plan.bm) * ((a->N + tn - 1ll) / tn) > 0x7FFFFFFFll) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
     if (!aligned(a->a, 16) || !aligned(a->w, 16) || !aligned(a->c, 16)) return fail(PSG_E_ALIGN, "a, w and c must be 16-byte aligned");
     if (!is16 && (!aligned(a->scale_b, 16) || !aligned(a->scale_a, 4))) return fail(PSG_E_ALIGN, "scale_b must be 16-byte and scale_a 4-byte aligned");
     if (!aligned(a->offsets, 4)) return fail(PSG_E_ALIGN, "offsets must be 4-byte aligned");
@@ -1410,7 +1409,7 @@ int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
     p.c = a->c, p.a = static_cast<const uint8_t*>(a->a), p.b = static_cast<const uint8_t*>(a->w), p.sa = a->scale_a, p.sb = a->scale_b;
     p.M = a->M, p.N = a->N, p.K = a->K, p.epi = EPI_NONE, p.out = a->out_dtype, p.splits = 1;
     const GroupParams g = {a->offsets, a->groups, 0};
-    const hipError_t e = psg_launch_grouped(p, g, a->in_dtype, bm, static_cast<hipStream_t>(stream));
+    const hipError_t e = psg_launch_grouped(p, g, a->in_dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_gemm_grouped launch");
     g_err[0] = 0;
     return 0;

@@ -55,7 +55,7 @@ class GroupedGemm:
 
     def __call__(self, C, A, B, scale_a, scale_b, offsets, M, stream=None):
         """Launch on ``stream`` (``None``: the current stream of the device of ``C``).  ``scale_a`` and ``scale_b`` are only read for 8-bit operands."""
-        if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and C.get_device() == torch.cuda.current_device():
+        if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and _lib.is_current(C.get_device()):
             key = (M, self.tile_rows)
             plan = self._plans.get(key)
             if plan is None:

@@ -56,7 +56,7 @@ class W4A16Gemm:
 
     def __call__(self, C, A, W, scales, zeros, bias, M, stream=None):
         """Launch on ``stream`` (``None``: the current stream of the device of ``C``).  ``zeros`` is only read with zero points, ``bias`` only with an epilogue."""
-        if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and C.get_device() == torch.cuda.current_device():
+        if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and _lib.is_current(C.get_device()):
             plan = self._plans.get(M)
             if plan is None:
                 if len(self._plans) >= 256:

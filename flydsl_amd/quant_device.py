@@ -118,7 +118,7 @@ def _norm_args(x, weight, eps, quant_dtype):
         raise TypeError(f"x must be a tensor of fp32, bf16 or fp16, got {getattr(x, 'dtype', type(x).__name__)}")
     if not x.is_cuda or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("x must be a 2-D device tensor with at least one column")
-    if not isinstance(weight, torch.Tensor) or weight.dtype not in (x.dtype, torch.float32) or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+    if not isinstance(weight, torch.Tensor) or weight.dtype not in (x.dtype, torch.float32) or weight.numel() != x.shape[1]:
         raise ValueError(f"weight must hold {x.shape[1]} elements of {x.dtype} or fp32")
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
@@ -135,9 +135,9 @@ def _norm_plan(x, weight, eps, quant_dtype):
     a = _norm_args(x, weight, eps, quant_dtype)
     f, any_, rows, dim, eb = _lib.RmsnormArgs, _lib.TYPE_ANY, a.rows, a.dim, x.element_size()
     typed = {torch.float32: _lib.TYPE_FP32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16}
-    xt, size, optional = typed[x.dtype] + _lib.ROWS, rows << 32 | dim, _lib.OPTIONAL
-    ops = _lib.operands((f.x, eb, xt, size), (f.weight, weight.element_size(), typed[weight.dtype], dim * weight.element_size()), (f.residual, eb, xt + optional, size),
-                        (f.residual_out, eb, xt + optional, size), (f.normed, eb, xt + optional, size), (f.q, 1, any_, rows * dim), (f.scale, 4, _lib.TYPE_FP32, 4 * rows))
+    xt, size, optional, exact = typed[x.dtype] + _lib.ROWS, rows << 32 | dim, _lib.OPTIONAL, _lib.EXACT
+    ops = _lib.operands((f.x, eb, xt, size), (f.weight, weight.element_size(), typed[weight.dtype] + exact, dim * weight.element_size()), (f.residual, eb, xt + optional, size),
+                        (f.residual_out, eb, xt + optional, size), (f.normed, eb, xt + optional, size), (f.q, 1, any_ + exact, rows * dim), (f.scale, 4, _lib.TYPE_FP32 + exact, 4 * rows))
     return (bytes(a),), ops
 
 
@@ -156,22 +156,22 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     0, and ``dim`` any number.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
     the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
     # a call with its outputs, on the current device, goes on in native code, which looks at the operands
-    if stream is not None and type(out) in (tuple, list) and len(out) == 2 and type(x) is type(weight) is torch.Tensor and x.is_cuda and x.dim() == 2:
+    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is type(weight) is torch.Tensor and quant_dtype is not None and (residual is not None or residual_out is None):
         q, scale = out
         h = residual if residual_out is None else residual_out
-        if type(q) is type(scale) is torch.Tensor and q.shape == x.shape and scale.numel() == x.shape[0] and quant_dtype is not None and (
-                residual is not None or h is None) and x.get_device() == torch.cuda.current_device():
-            key = (x.shape, x.dtype, weight.shape, weight.dtype, eps, quant_dtype)
+        if type(q) is type(scale) is torch.Tensor and x.is_cuda and _lib.is_current(x.get_device()):
+            key = (x.shape, x.dtype, weight.dtype, eps, quant_dtype)
             plan = _norm_plans.get(key)
             if plan is None:
+                a = _norm_plan(x, weight, eps, quant_dtype)
                 if len(_norm_plans) >= 256:
                     _norm_plans.clear()
-                plan = _norm_plans[key] = _norm_plan(x, weight, eps, quant_dtype)
+                plan = _norm_plans[key] = a
             rc = _lib._native.launch(_lib.address("psg_rmsnorm_quant"), plan[0], plan[1], stream, x, weight, residual, h, normed, q, scale)
             if rc != _lib._native.DECLINED:
                 if rc:
                     _lib.check(rc, "psg_rmsnorm_quant")
-                return q if q.dtype == quant_dtype else q.view(quant_dtype), scale if scale.dim() == 2 and scale.shape[1] == 1 else scale.view(-1, 1)
+                return q.view(quant_dtype) if q.dtype is not quant_dtype else q, scale if scale.dim() == 2 and scale.shape[1] == 1 else scale.view(-1, 1)
     a = _norm_args(x, weight, eps, quant_dtype)
     rows, dim = x.shape
     if weight.device != x.device or not weight.is_contiguous():
@@ -195,7 +195,7 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     else:
         q, scale = out
         _check_out(x, q, scale)
-        if q.shape != x.shape or q.element_size() != 1 or scale.numel() != rows or scale.dtype != torch.float32:
+        if q.numel() != x.numel() or q.element_size() != 1 or scale.numel() != rows or scale.dtype != torch.float32:
             raise ValueError("out must be (1-byte [rows, dim], fp32 [rows] or [rows, 1]) tensors")
     if normed is not None:
         a.normed_stride = _norm_row_stride("normed", normed, x)

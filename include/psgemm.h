@@ -516,9 +516,9 @@ int psg_gemm_w4a16(const psg_w4a16_args *args, void *stream);
  *   offsets [groups+1] int32 on the device, not decreasing.  Rows of c outside [offsets[0], offsets[groups]) are left as they are; groups may be empty.  An offset outside [0, M] counts
  *   as the nearer end, and a group whose end is not above its begin has no rows: no offsets make the kernels read or write outside the operands (where they go back, which
  *   rows are written is not said).
- * in_dtype PSG_IN_INT8 .. PSG_IN_BF16; tile_rows 0 (chosen by the mean rows of a group) or 16, 32, 64, 128.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K * bytes % 64 == 0, the bytes of
- * one weight below 4 GiB.  a, w, c and scale_b 16-byte, scale_a and offsets 4-byte aligned.  Sums as in psg_gemm_a8w8 (int8 exact), of every row in the same order
- * whatever its group's size.
+ * in_dtype PSG_IN_INT8 .. PSG_IN_BF16; tile_rows 0 (the library's choice by M, N, K and groups) or 16, 32, 64, 128.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K * bytes % 64 == 0, the bytes of
+ * one weight below 4 GiB.  a, w, c and scale_b 16-byte, scale_a and offsets 4-byte aligned.  Sums as in psg_gemm_a8w8 (int8 exact); within a call every
+ * row's in the same order, whatever its group's size.
  */
 typedef struct psg_grouped_args {
     void *c;
