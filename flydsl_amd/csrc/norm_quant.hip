@@ -9,7 +9,9 @@
 // One pass: the maximum does not need the norm, max|y| = max|h w| / rms with the same rounding (a product with a positive factor is monotone), so the sum of squares and
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
-// Bound: HBM; every operand is read once and every output written once.
+// Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
+// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off four bytes, of an odd width, take up to twice the time (8192 of 2051 48 us, of 2048
+// 25.7): every access of a lane then covers two pieces.
 #include "psg_common.h"
 #include "quant_rows.h"
 #include "norm_quant.h"
@@ -268,13 +270,19 @@ hipError_t launch(const NormParams& p, hipStream_t stream) {
         hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, NT_, KEEP_, WHOLE>), dim3(NT_ == 64 ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows), dim3(NT_ == 64 ? 256 : NT_), 0, stream, p); \
         return hipGetLastError();                                                                                                                \
     }
+    // Threads of a row, us, bf16 to fp8 with a residual.  A wavefront or four: 8192 rows of 1024 13.6 / 16.0, 2048 of 2048 8.7 / 8.8, 777 of 2048 5.3 / 4.4.
     if (nvec <= 256 && p.rows >= 8 * psg_cu_count()) {
         if (nvec <= 64) PSG_NORM(64, 1)
         PSG_NORM(64, 4)
     }
     if (nvec <= 256) PSG_NORM(256, 1)
-    if (nvec <= 512) PSG_NORM(256, 2)
-    if (nvec <= 1024) PSG_NORM(256, 4)
+    // Eight wavefronts or four: with few rows a thread's second vector is what a row waits for, 1 row of 4096 2.9 / 3.1, 256 3.7 / 3.9, 777 7.5 / 7.2, 8192 46.8 / 44.6;
+    // 1 of 8192 3.5 / 4.0, 8192 80.6 / 81.9.
+    if (nvec <= 512 && p.rows > 2 * psg_cu_count()) PSG_NORM(256, 2)
+    if (nvec <= 512) PSG_NORM(512, 1)
+    if (nvec <= 1024) PSG_NORM(512, 2)
+    // Sixteen or eight: 777 of 16384 19.4 / 20.2, 8192 163 / 162; longer rows keep twice as much, and beyond 32768 come back for the rest.
+    if (nvec <= 2048) PSG_NORM(1024, 2)
     PSG_NORM(1024, 4)
 #undef PSG_NORM
 }
