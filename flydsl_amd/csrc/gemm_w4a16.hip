@@ -227,7 +227,7 @@ hipError_t go(W4Params p, hipStream_t stream) {
     p.passes = (steps + W4_WAVES * SPW - 1) / (W4_WAVES * SPW);
     p.per = (steps + W4_WAVES * p.passes - 1) / (W4_WAVES * p.passes);
     // a workgroup has LDS for the sums of so many windows of 16 columns, which begin at a multiple of 8
-    constexpr int PATCH = MB * SH * 4096, windows = MANY ? (W4_LDS - W4_WAVES * PATCH) / (W4_WAVES * MB * 1024) : PATCH / (MB * 1024), most = 2 * windows - 1;
+    constexpr int PATCH = MB * SH * 4096, windows = MANY ? (W4_LDS - W4_WAVES * PATCH) / (W4_WAVES * MB * 1024) : PATCH / (MB * 1024), most = 2 * windows;
     const long units = p.N / 8, cus = psg_cu_count(), rounds = (units + most * cus - 1) / (most * cus), wgs = units < cus * rounds ? units : cus * rounds;
     p.unit_q = (int)(units / wgs), p.unit_r = (int)(units % wgs);
     hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, SH, MANY>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), 0, stream, p);
@@ -237,13 +237,16 @@ hipError_t go(W4Params p, hipStream_t stream) {
 template <bool BF16, int GS, bool ZP>
 hipError_t launch(const W4Params& p, hipStream_t stream) {
     const int per = ((p.K + 127) / 128 + W4_WAVES - 1) / W4_WAVES;  // steps of a wavefront
-    // 17 to 32 rows read W once where A fits the registers, else 16 rows at a time: 32x7168x2048 8.1 / 5.9, 32x4096x4096 8.6 / 6.8; in several passes of 32 rows 32x8192x8192 took 22.8, like this 19.9,
-    // 32x28672x4096 in groups of 32 47 / 34
+    // 17 to 32 rows read W once: where A fits the registers, 16 rows at a time / like this, 32x7168x2048 8.1 / 5.9, 32x4096x4096 8.6 / 6.8; longer rows in passes of two steps, which leave LDS for
+    // two windows a workgroup, 32x8192x8192 22.9 / 16.0, 17x8192x5120 15.5 / 10.3, or of one, for six, 24x12288x6144 22.7 / 18.1, 32x14336x4096 in groups of 32 20.2 / 16.6 (of two 18.7).  With still
+    // more columns 16 rows at a time are level or better (32x28672x8192 47.7 / 55.8).
     if (p.M > 16) {
         if (per <= 2) return go<BF16, 2, GS, ZP, 2, 2, false>(p, stream);
         if constexpr (GS == 128) {
             if (per <= 4) return go<BF16, 2, GS, ZP, 4, 2, false>(p, stream);
         }
+        if (p.N <= 32 * psg_cu_count()) return go<BF16, 2, GS, ZP, 2, 2, true>(p, stream);
+        if (p.N <= 96 * psg_cu_count()) return go<BF16, 2, GS, ZP, 1, 1, true>(p, stream);
     }
     if (per <= 2) return go<BF16, 1, GS, ZP, 2, 2, false>(p, stream);
     if (per <= 4) return go<BF16, 1, GS, ZP, 4, 4, false>(p, stream);
@@ -251,10 +254,10 @@ hipError_t launch(const W4Params& p, hipStream_t stream) {
     if constexpr (GS == 128) {
         if (per <= 8) return go<BF16, 1, GS, ZP, 8, 4, false>(p, stream);
     }
-    // Passes of four steps leave LDS for four windows a workgroup, passes of two for twelve.  us four / two: 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but more windows a CU
+    // 16 rows: passes of four steps leave LDS for four windows a workgroup, passes of two for twelve.  us four / two: 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but more windows a CU
     // 16x28672x8192 in groups of 64 36.7 / 33.6, five and six steps, which two divide better, 4x5120x6144 10.0 / 9.0, 1x6144x6144 9.9 / 8.7, and groups of 32 with zero points,
     // which take all registers, 2x8192x10240 16.9 / 14.9
-    if (per <= 6 || p.N > 56 * psg_cu_count() || (GS == 32 && ZP)) return go<BF16, 1, GS, ZP, 2, 2, true>(p, stream);
+    if (per <= 6 || p.N > 64 * psg_cu_count() || (GS == 32 && ZP)) return go<BF16, 1, GS, ZP, 2, 2, true>(p, stream);
     return go<BF16, 1, GS, ZP, 4, 4, true>(p, stream);
 }
 

@@ -62,7 +62,8 @@ def _run(a, codes, scale, zero, bias, group, dtype, epi, guard=3):
 
 
 SIZES = [(1, 16, 128), (1, 4096, 4096), (2, 2064, 1152), (5, 1040, 2176), (16, 48, 11008), (17, 512, 640), (32, 7168, 2048), (33, 272, 512), (100, 1024, 1024), (3, 28672, 256), (16, 8208, 384), (20, 1040, 4096), (16, 2064, 8192),
-         (8, 528, 6144), (3, 32992, 5120), (1, 16, 32768), (9, 14352, 7168)]
+         (8, 528, 6144), (3, 32992, 5120), (1, 16, 32768), (9, 14352, 7168),
+         (32, 8192, 4096), (17, 8176, 8192), (32, 8208, 6144), (40, 4112, 5120)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
