@@ -108,6 +108,12 @@ __global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p, GROUPS... groups)
                 });
             });
             __syncthreads();
+            if constexpr (sizeof...(GROUPS) == 1) {
+                if ((groups, ...).past) {
+                    pair_store_rows<2>(lds, half, rc, n0, p.N, tid);
+                    return;
+                }
+            }
             pair_store_rows(lds, half, rc, n0, p.N, tid);
         });
     }
@@ -125,6 +131,9 @@ void go(const A8W8Params& p, int store, dim3 grid, hipStream_t stream) {
 // The grouped product on these tiles: bf16 by STORE_C, fp16 by STORE_C_GENERIC
 hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream) {
     g.most = (int)group_tiles_most(p.M, g.groups, 128);
+    // A C that fills the last-level cache (256 MB) goes past it, in whose place weights and rows of A stay: 32768 rows, 4096 x 1536, fp8 233 / 226 us, with what reads C next 314 / 308.  A smaller one
+    // would be missed by its reader: 1500 x 2816, bf16 28.4 / 25.3, but 30.4 / 32.4 with it.
+    g.past = (uint64_t)p.M * (uint64_t)p.N * 2ull >= 256ull << 20;
     const dim3 grid((unsigned)g.most * (unsigned)((p.N + 255) / 256));
 #define PSG_GROUPED(KIND_)                                                                                                                             \
     case KIND_:                                                                                                                                        \

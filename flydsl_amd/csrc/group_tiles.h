@@ -7,6 +7,7 @@
 struct GroupParams {
     const int32_t* offsets;  // [groups + 1]
     int groups;
+    int past;  // set by the launcher (128x256 tiles): C goes past the caches
     int most;  // set by the launcher: tiles along M that the grid was made for (offsets that go back may say more)
 };
 

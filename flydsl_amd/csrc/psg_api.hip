@@ -1408,7 +1408,7 @@ int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
     A8W8Params p = {};
     p.c = a->c, p.a = static_cast<const uint8_t*>(a->a), p.b = static_cast<const uint8_t*>(a->w), p.sa = a->scale_a, p.sb = a->scale_b;
     p.M = a->M, p.N = a->N, p.K = a->K, p.epi = EPI_NONE, p.out = a->out_dtype, p.splits = 1;
-    const GroupParams g = {a->offsets, a->groups, 0};
+    const GroupParams g = {a->offsets, a->groups, 0, 0};
     const hipError_t e = psg_launch_grouped(p, g, a->in_dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_gemm_grouped launch");
     g_err[0] = 0;

@@ -96,6 +96,7 @@ def per_1x32_f4_quant(x: torch.Tensor, shuffle: bool = True, stream=None, out=No
     return packed if packed.dtype == fp4x2 else packed.view(fp4x2), scales if scales.dtype == fp8_e8m0 else scales.view(fp8_e8m0)
 
 
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
 _norm_plans = {}  # what shapes and types alone decide about a call of rmsnorm_quant, by them
 
 
@@ -156,7 +157,7 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     0, and ``dim`` any number.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
     the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
     # a call with its outputs, on the current device, goes on in native code, which looks at the operands
-    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is type(weight) is torch.Tensor and quant_dtype is not None and (residual is not None or residual_out is None):
+    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and type(weight) in _TENSORS and quant_dtype is not None and (residual is not None or residual_out is None):
         q, scale = out
         h = residual if residual_out is None else residual_out
         if type(q) is type(scale) is torch.Tensor and x.is_cuda and _lib.is_current(x.get_device()):

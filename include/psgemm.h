@@ -21,6 +21,9 @@
  *   psg_gemm_mxfp4      kernels/gemm/mxfp4_preshuffle.py:57-488 (launch_gemm / kernel_gemm): fp4/fp6/fp8 A x fp4/fp8 W,
  *                       caller strides, batch over grid.z
  *   psg_gemm_mxfp4_acc  no counterpart: fp32 accumulators of the MXFP4 mainloop, for parity tests
+ *   psg_rmsnorm_quant, psg_gemm_w4a16, psg_gemm_grouped
+ *                       no counterpart of these call shapes: the norm in front of the quantised products, products with 4-bit
+ *                       weights and group scales, and ragged products grouped by expert, beside the quantisers, GEMMs and MoE stages
  *   psg_workspace_bytes no counterpart (the reference's preshuffle GEMM has no split-K path)
  *   psg_tile_coords     the workgroup-id -> tile remap xcd_remap_bx_by
  *                       kernels/common/mma/mfma_preshuffle_pipeline.py:685-729 (host evaluation of the function the

@@ -154,6 +154,8 @@ def test_no_rows_and_reused_outputs():
     q, s = quant_device.rmsnorm_quant(x, w, stream=torch.cuda.current_stream(), out=out)
     assert q.data_ptr() == out[0].data_ptr() and s.data_ptr() == out[1].data_ptr() and q.dtype == FP8
     _check(x, w, None, 1e-6, FP8, q, s, None, None)
+    q, s = quant_device.rmsnorm_quant(x, torch.nn.Parameter(w), stream=torch.cuda.current_stream(), out=out)  # a module's weight
+    _check(x, w, None, 1e-6, FP8, q, s, None, None)
 
 
 def test_graph_replays_and_another_stream():
