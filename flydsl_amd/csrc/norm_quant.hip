@@ -10,8 +10,9 @@
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
 // Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
-// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off four bytes, of an odd width, take up to twice the time (8192 of 2051 48 us, of 2048
-// 25.7): every access of a lane then covers two pieces.
+// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes, of a width that is no multiple
+// of 8, take 1.3 to 1.9 times as long (8192 of 2056 29.4 us, of 2050 to 2054 37 to 43, of 2049 and 2051 43 to 48): an access of a wavefront then covers one line more, and the row's
+// end is read by elements.
 #include "psg_common.h"
 #include "quant_rows.h"
 #include "norm_quant.h"
