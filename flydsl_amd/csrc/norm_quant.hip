@@ -238,8 +238,9 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = times_over<XT == X_BF16 && WT == X_BF16>(v[e], dmax, mhw, rm);
         } else {
+            // (a scale near the smallest number has a few bits only and may be too small by a third: held within +-dmax, where int8 would wrap and fp8 has no number)
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = clean(y[e], dmax) / s;
+            for (int e = 0; e < 8; e++) y[e] = fminf(fmaxf(clean(y[e], dmax) / s, -dmax), dmax);
         }
         const v2i o = p.out == NORM_FP8 ? quant_pack8<1>(y) : quant_pack8<0>(y);
         uint8_t* dst = p.q + qb + (int64_t)vi * 8;

@@ -205,3 +205,21 @@ def test_refusals():
         f(x, w, -1.0)
     with pytest.raises(ValueError, match="quant_dtype=None"):
         f(x, w, quant_dtype=None, out=out)
+
+
+@pytest.mark.parametrize("qd", [torch.int8, FP8])
+def test_scale_near_the_smallest_number(qd):
+    """Rows whose scale has two or three bits: it is off by up to u / 2 (u = 2^-149), the outputs stay within the largest value all the same.  y is off by 2 u (a product rounded to u / 2, times
+    at most 1.25, and rounded again); an output held back at the largest value by as much times u / 2; then the output's own step."""
+    g = torch.Generator().manual_seed(11)
+    x, w = torch.randn(64, 256, generator=g), torch.full((256,), 2.0**-140)
+    assert w[0] > 0
+    y = x.double() * w.double() / x.double().square().mean(-1, keepdim=True).sqrt()
+    assert (x.square().mean(-1).sqrt() - 1).abs().max() < 0.25
+    q, s = quant_device.rmsnorm_quant(x.cuda(), w.cuda(), 0.0, quant_dtype=qd)
+    q, s = q.cpu().double(), s.cpu().double()
+    u = 2.0**-149
+    assert ((s - y.abs().amax(-1, keepdim=True) / QMAX[qd]).abs() <= u).all()
+    assert (q.abs() <= QMAX[qd]).all()
+    step = s if qd == torch.int8 else torch.maximum(y.abs() / 16, s * 2.0**-10)
+    assert ((q * s - y).abs() <= 1.1 * step + (QMAX[qd] / 2 + 3) * u).all()
