@@ -264,14 +264,29 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
     }
 }
 
+// NT threads a row, in launches of 2^31 threads at most: a grid holds no more than 2^32
+template <int XT, int WT, int NT, int KEEP, bool WHOLE>
+hipError_t launch_rows(NormParams p, hipStream_t stream) {
+    constexpr int64_t most = (1ll << 31) / NT, B = XT == X_F32 ? 4 : 2;
+    for (int64_t left = p.rows;; left -= most) {
+        p.rows = left < most ? left : most;
+        hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, NT, KEEP, WHOLE>), dim3(NT == 64 ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows), dim3(NT == 64 ? 256 : NT), 0, stream, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || left <= most) return e;
+        p.x = static_cast<const uint8_t*>(p.x) + most * p.x_stride * B;
+        if (p.residual) {
+            p.residual = static_cast<const uint8_t*>(p.residual) + most * p.r_stride * B;
+            p.h = static_cast<uint8_t*>(p.h) + most * p.h_stride * B;
+        }
+        if (p.normed) p.normed = static_cast<uint8_t*>(p.normed) + most * p.n_stride * B;
+        if (p.out != NORM_NONE) p.q += most * p.dim, p.scale += most;
+    }
+}
+
 template <int XT, int WT, bool WHOLE>
 hipError_t launch(const NormParams& p, hipStream_t stream) {
     const int nvec = (p.dim + 7) / 8;
-#define PSG_NORM(NT_, KEEP_)                                                                                                                     \
-    {                                                                                                                                            \
-        hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, NT_, KEEP_, WHOLE>), dim3(NT_ == 64 ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows), dim3(NT_ == 64 ? 256 : NT_), 0, stream, p); \
-        return hipGetLastError();                                                                                                                \
-    }
+#define PSG_NORM(NT_, KEEP_) return launch_rows<XT, WT, NT_, KEEP_, WHOLE>(p, stream);
     // Threads of a row, us, bf16 to fp8 with a residual.  A wavefront or four: 8192 rows of 1024 13.6 / 16.0, 2048 of 2048 8.7 / 8.8, 777 of 2048 5.3 / 4.4.
     if (nvec <= 256 && p.rows >= 8 * psg_cu_count()) {
         if (nvec <= 64) PSG_NORM(64, 1)

@@ -1401,7 +1401,8 @@ int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
     if (a->tile_rows != 0 && a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64 or 128", a->tile_rows);
     const GroupedPlan plan = a->tile_rows ? GroupedPlan{a->tile_rows, false} : psg_grouped_plan(a->M, a->groups, a->N, a->K * eb);
     const int tn = plan.sliced ? 16 : plan.bm <= 32 ? 64 : 2 * plan.bm;  // columns of a tile
-    if (group_tiles_most(a->M, a->groups, plan.bm) * ((a->N + tn - 1ll) / tn) > 0x7FFFFFFFll) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
+    // (256 threads each: a grid holds less than 2^32)
+    if (group_tiles_most(a->M, a->groups, plan.bm) * ((a->N + tn - 1ll) / tn) >= 1ll << 24) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
     if (!aligned(a->a, 16) || !aligned(a->w, 16) || !aligned(a->c, 16)) return fail(PSG_E_ALIGN, "a, w and c must be 16-byte aligned");
     if (!is16 && (!aligned(a->scale_b, 16) || !aligned(a->scale_a, 4))) return fail(PSG_E_ALIGN, "scale_b must be 16-byte and scale_a 4-byte aligned");
     if (!aligned(a->offsets, 4)) return fail(PSG_E_ALIGN, "offsets must be 4-byte aligned");

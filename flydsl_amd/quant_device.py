@@ -119,6 +119,8 @@ def _norm_args(x, weight, eps, quant_dtype):
         raise TypeError(f"x must be a tensor of fp32, bf16 or fp16, got {getattr(x, 'dtype', type(x).__name__)}")
     if not x.is_cuda or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("x must be a 2-D device tensor with at least one column")
+    if x.shape[0] >= 1 << 31 or x.shape[1] > 1 << 24:
+        raise ValueError(f"x may have up to 2^31 - 1 rows of up to 2^24 elements, got {tuple(x.shape)}")
     if not isinstance(weight, torch.Tensor) or weight.dtype not in (x.dtype, torch.float32) or weight.numel() != x.shape[1]:
         raise ValueError(f"weight must hold {x.shape[1]} elements of {x.dtype} or fp32")
     eps = float(eps)
@@ -154,7 +156,7 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
 
     ``x``, ``residual``, ``residual_out`` and ``normed`` are ``[rows, dim]`` of one type (fp32 / bf16 / fp16), each with dense rows any distance apart (a slice of the
     columns of a wider tensor will do); ``weight`` ``[dim]`` has that type or fp32.  ``residual_out`` may be ``residual`` or ``x``, ``normed`` may be ``x``.  ``rows`` may be
-    0, and ``dim`` any number.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
+    0, and ``dim`` anything up to 2^24.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
     the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
     # a call with its outputs, on the current device, goes on in native code, which looks at the operands
     if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and type(weight) in _TENSORS and quant_dtype is not None and (residual is not None or residual_out is None):

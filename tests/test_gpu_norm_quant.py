@@ -223,3 +223,28 @@ def test_scale_near_the_smallest_number(qd):
     assert (q.abs() <= QMAX[qd]).all()
     step = s if qd == torch.int8 else torch.maximum(y.abs() / 16, s * 2.0**-10)
     assert ((q * s - y).abs() <= 1.1 * step + (QMAX[qd] / 2 + 3) * u).all()
+
+
+def test_more_rows_than_a_launch_holds():
+    rows, at = (1 << 25) + 5, slice((1 << 25) - 3, None)  # 64 threads a row
+    x = torch.randn(rows, 8, dtype=torch.bfloat16, device="cuda")
+    r = torch.randn(rows, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.rand(8, device="cuda") + 0.5
+    q, s = torch.zeros(rows, 8, dtype=torch.int8, device="cuda"), torch.full((rows, 1), -1.0, device="cuda")
+    x0, r0, h0, n0 = x[at].clone(), r[at].clone(), torch.empty(8, 8, dtype=x.dtype, device="cuda"), torch.empty(8, 8, dtype=x.dtype, device="cuda")
+    print(f"norm rows={rows} dim=8", flush=True)
+    quant_device.rmsnorm_quant(x, w, residual=r, normed=x, quant_dtype=torch.int8, out=(q, s))
+    q0, s0 = quant_device.rmsnorm_quant(x0, w, residual=r0, residual_out=h0, normed=n0, quant_dtype=torch.int8)
+    assert torch.equal(q[at], q0) and torch.equal(s[at], s0) and torch.equal(r[at], h0) and torch.equal(x[at], n0)
+    _check(x0, w, r0, 1e-6, torch.int8, q0, s0, h0, n0)
+    assert (s > 0).all() and (torch.maximum(q.amax(-1), -q.amin(-1)) == 127).all()
+
+
+def test_sizes_refused():
+    out = torch.empty(4, 8, dtype=torch.uint8, device="cuda"), torch.empty(4, device="cuda")
+    one = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    for stream in (None, torch.cuda.current_stream()):
+        with pytest.raises(ValueError, match="2\\^31"):
+            quant_device.rmsnorm_quant(one.expand(1 << 31, 1), one[0], out=out, stream=stream)
+        with pytest.raises(ValueError, match="2\\^31"):
+            quant_device.rmsnorm_quant(one.expand(1, (1 << 24) + 1), one.expand(1, (1 << 24) + 1), out=out, stream=stream)

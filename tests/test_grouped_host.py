@@ -34,6 +34,7 @@ def _args(**change):
     (dict(c=0), NULL), (dict(a=0), NULL), (dict(w=0), NULL), (dict(offsets=0), NULL), (dict(scale_a=0), NULL), (dict(scale_b=0, in_dtype=0), NULL), (dict(in_dtype=6), DTYPE), (dict(in_dtype=-1), DTYPE),
     (dict(out_dtype=2), DTYPE), (dict(M=0), SHAPE), (dict(M=(1 << 22) + 1), SHAPE), (dict(groups=0), SHAPE), (dict(groups=4097), SHAPE), (dict(N=40), SHAPE), (dict(K=96), SHAPE),
     (dict(K=0), SHAPE), (dict(N=1 << 18, K=1 << 14), SHAPE), (dict(N=1 << 24, K=64), SHAPE), (dict(N=16, K=1 << 25), SHAPE), (dict(tile_rows=48), SHAPE), (dict(M=1 << 22, N=1 << 20, tile_rows=16), SHAPE),
+    (dict(M=1 << 22, N=1 << 12, tile_rows=16), SHAPE),  # 2^24 workgroups and more
     (dict(a=0x1008), ALIGN), (dict(w=0x1008), ALIGN), (dict(c=0x1008), ALIGN), (dict(scale_b=0x1008), ALIGN), (dict(scale_a=0x1002), ALIGN), (dict(offsets=0x1002), ALIGN),
 ])
 def test_c_entry_refuses(change, code):
