@@ -10,9 +10,8 @@
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
 // Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
-// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes, of a width that is no multiple
-// of 8, take 1.3 to 1.9 times as long (8192 of 2056 29.4 us, of 2050 to 2054 37 to 43, of 2049 and 2051 43 to 48): an access of a wavefront then covers one line more, and the row's
-// end is read by elements.
+// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes cost nothing (8192 of
+// 2048, 2048 to 2056 elements apart, 26.3 to 28.5 us); an end that is no whole vector does a little: 2047 27.6; where it is a thread's second vector, 2056 30.0, 2050 to 2054 33 to 34, 2049 39.9.
 #include "psg_common.h"
 #include "quant_rows.h"
 #include "norm_quant.h"
@@ -22,14 +21,18 @@ namespace {
 // 16-byte pieces at any address that is a multiple of the element (global accesses of this target need no more)
 typedef v4i v4i_any __attribute__((aligned(2)));  // (fp32 elements are on 4 bytes)
 typedef v2i v2i_any __attribute__((aligned(1)));
+typedef int int_any __attribute__((aligned(1)));
+typedef uint16_t half_any __attribute__((aligned(1)));
 
-// Elements [i, i + 8) as they are stored; from `n` on they read as zero
+// Elements [i, i + 8) as they are stored.  Of a row's end, n < 8 of them, its last eight are read: line_up() moves them into their places once every load is on its way (a branch for
+// each element, with a wait of its own, took as long as the rest of the row: 8192 rows of 2047 45.6 us, of 2041 30.8, like this 27.6 and 27.4).  The others among the eight, which their own
+// thread may be writing, are dropped.  Rows of less than eight are read by elements.
 template <int XT, bool WHOLE>
-__device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n) {
+__device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n, int dim) {
     constexpr int B = XT == X_F32 ? 4 : 2;
     Raw8<XT> r;
-    if (WHOLE || n >= 8) {
-        const v4i_any* p = reinterpret_cast<const v4i_any*>(static_cast<const uint8_t*>(base) + i * B);
+    if (WHOLE || dim >= 8) {
+        const v4i_any* p = reinterpret_cast<const v4i_any*>(static_cast<const uint8_t*>(base) + (WHOLE || n >= 8 ? i : i + n - 8) * B);
         r.w[0] = p[0];
         if constexpr (XT == X_F32) r.w[1] = p[1];
     } else {
@@ -45,20 +48,52 @@ __device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n)
     return r;
 }
 
+// the last n of the eight elements to the front, zeros behind them
+template <int XT, bool WHOLE>
+__device__ __forceinline__ void line_up(Raw8<XT>& r, int n, int dim) {
+    if (WHOLE || n >= 8 || dim < 8) return;
+    if constexpr (XT == X_F32) {
+        int v[15];
+#pragma unroll
+        for (int e = 0; e < 15; e++) v[e] = e < 8 ? r.w[e >> 2][e & 3] : 0;
+#pragma unroll
+        for (int k = 4; k > 0; k >>= 1)
+            if ((8 - n) & k) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = e + k < 8 ? v[e + k] : 0;
+            }
+#pragma unroll
+        for (int e = 0; e < 8; e++) r.w[e >> 2][e & 3] = v[e];
+    } else {
+        v4i w = r.w[0];
+        if ((8 - n) & 4) w = (v4i){w[2], w[3], 0, 0};
+        if ((8 - n) & 2) w = (v4i){w[1], w[2], w[3], 0};
+        if ((8 - n) & 1)
+            w = (v4i){(int)__builtin_amdgcn_alignbit((unsigned)w[1], (unsigned)w[0], 16u), (int)__builtin_amdgcn_alignbit((unsigned)w[2], (unsigned)w[1], 16u),
+                      (int)__builtin_amdgcn_alignbit((unsigned)w[3], (unsigned)w[2], 16u), (int)((unsigned)w[3] >> 16)};
+        r.w[0] = w;
+    }
+}
+
+// (a row's end in pieces of 4, 2 and 1)
 template <int XT, bool WHOLE>
 __device__ __forceinline__ void store_row(void* base, int64_t i, int n, const Raw8<XT>& r) {
     constexpr int B = XT == X_F32 ? 4 : 2;
+    uint8_t* at = static_cast<uint8_t*>(base) + i * B;
     if (WHOLE || n >= 8) {
-        v4i_any* p = reinterpret_cast<v4i_any*>(static_cast<uint8_t*>(base) + i * B);
+        v4i_any* p = reinterpret_cast<v4i_any*>(at);
         p[0] = r.w[0];
         if constexpr (XT == X_F32) p[1] = r.w[1];
+    } else if constexpr (XT == X_F32) {
+        v4i w = r.w[0];
+        if (n & 4) *reinterpret_cast<v4i_any*>(at) = w, at += 16, w = r.w[1];
+        if (n & 2) *reinterpret_cast<v2i_any*>(at) = (v2i){w[0], w[1]}, at += 8, w[0] = w[2];
+        if (n & 1) *reinterpret_cast<int*>(at) = w[0];
     } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < n) {
-                if constexpr (XT == X_F32) static_cast<int*>(base)[i + e] = r.w[e >> 2][e & 3];
-                else static_cast<uint16_t*>(base)[i + e] = (uint16_t)((uint32_t)r.w[0][e >> 1] >> (16 * (e & 1)));
-            }
+        v2i w = {r.w[0][0], r.w[0][1]};
+        if (n & 4) *reinterpret_cast<v2i_any*>(at) = w, at += 8, w = (v2i){r.w[0][2], r.w[0][3]};
+        if (n & 2) *reinterpret_cast<int_any*>(at) = w[0], at += 4, w[0] = w[1];
+        if (n & 1) *reinterpret_cast<uint16_t*>(at) = (uint16_t)w[0];
     }
 }
 
@@ -105,7 +140,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
     const int nvec = (p.dim + 7) >> 3;
     const int64_t xb = row * p.x_stride, rb = row * p.r_stride, hb = row * p.h_stride, nb = row * p.n_stride, qb = row * (int64_t)p.dim;
     auto left = [&](int vi) { return p.dim - vi * 8; };
-    auto weights = [&](int vi) __attribute__((always_inline)) { return load_row<WT, WHOLE>(p.weight, (int64_t)vi * 8, left(vi)); };
+    auto weights = [&](int vi) __attribute__((always_inline)) { return load_row<WT, WHOLE>(p.weight, (int64_t)vi * 8, left(vi), p.dim); };
 
     float sum = 0.f, hw[KEEP][8];
     uint32_t mb = 0;
@@ -119,9 +154,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
             mb = u > mb ? u : mb;
         }
     };
-    auto add = [&](const Raw8<XT>& x, const Raw8<XT>& r, int vi, bool live, float* h) __attribute__((always_inline)) {
+    auto add = [&](Raw8<XT> x, Raw8<XT> r, int vi, bool live, float* h) __attribute__((always_inline)) {
+        if (live) line_up<XT, WHOLE>(x, left(vi), p.dim);
         x.values(h);
         if (p.residual) {
+            if (live) line_up<XT, WHOLE>(r, left(vi), p.dim);
             float v[8];
             r.values(v);
 #pragma unroll
@@ -138,10 +175,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
         Raw8<WT> w[KEEP];
         auto at = [&](int it) { return tid + it * NT < nvec ? tid + it * NT : 0; };
 #pragma unroll
-        for (int it = 0; it < KEEP; it++) r[it] = x[it] = load_row<XT, WHOLE>(p.x, xb + (int64_t)at(it) * 8, left(at(it)));
+        for (int it = 0; it < KEEP; it++) r[it] = x[it] = load_row<XT, WHOLE>(p.x, xb + (int64_t)at(it) * 8, left(at(it)), p.dim);
         if (p.residual) {
 #pragma unroll
-            for (int it = 0; it < KEEP; it++) r[it] = load_row<XT, WHOLE>(p.residual, rb + (int64_t)at(it) * 8, left(at(it)));
+            for (int it = 0; it < KEEP; it++) r[it] = load_row<XT, WHOLE>(p.residual, rb + (int64_t)at(it) * 8, left(at(it)), p.dim);
         }
 #pragma unroll
         for (int it = 0; it < KEEP; it++) w[it] = weights(at(it));
@@ -150,6 +187,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
             const bool live = tid + it * NT < nvec;
             float h[8], wv[8];
             add(x[it], r[it], tid + it * NT, live, h);
+            if (live) line_up<WT, WHOLE>(w[it], left(tid + it * NT), p.dim);
             w[it].values(wv);
             if (!live) {
 #pragma unroll
@@ -159,10 +197,12 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
         }
     }
     for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
-        const Raw8<XT> x = load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi));
-        const Raw8<XT> r = p.residual ? load_row<XT, WHOLE>(p.residual, rb + (int64_t)vi * 8, left(vi)) : x;
+        const Raw8<XT> x = load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
+        const Raw8<XT> r = p.residual ? load_row<XT, WHOLE>(p.residual, rb + (int64_t)vi * 8, left(vi), p.dim) : x;
+        Raw8<WT> wr = weights(vi);
+        line_up<WT, WHOLE>(wr, left(vi), p.dim);
         float w[8], h[8], y[8];
-        weights(vi).values(w);
+        wr.values(w);
         add(x, r, vi, true, h);
         take(h, w, y);
     }
@@ -190,9 +230,13 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
 
     // h w of a vector that is not in registers
     auto again = [&](int vi, float* v) __attribute__((always_inline)) {
+        Raw8<XT> h = p.residual ? load_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi), p.dim) : load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
+        Raw8<WT> wr = weights(vi);
+        line_up<XT, WHOLE>(h, left(vi), p.dim);
+        line_up<WT, WHOLE>(wr, left(vi), p.dim);
         float w[8];
-        (p.residual ? load_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi)) : load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi))).values(v);
-        weights(vi).values(w);
+        h.values(v);
+        wr.values(w);
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] *= w[e];
     };
@@ -247,9 +291,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
         if (WHOLE || n >= 8) {
             *reinterpret_cast<v2i_any*>(dst) = o;
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e < n) dst[e] = (uint8_t)((uint32_t)o[e >> 2] >> (8 * (e & 3)));
+            uint32_t b = (uint32_t)o[0];
+            if (n & 4) *reinterpret_cast<int_any*>(dst) = (int)b, dst += 4, b = (uint32_t)o[1];
+            if (n & 2) *reinterpret_cast<half_any*>(dst) = (uint16_t)b, dst += 2, b >>= 16;
+            if (n & 1) *dst = (uint8_t)b;
         }
     };
 #pragma unroll
@@ -308,7 +353,7 @@ hipError_t launch(const NormParams& p, hipStream_t stream) {
 
 // x_dtype: 0 fp32, 1 bf16, 2 fp16.  Requires rows, dim >= 1 and addresses that are multiples of their elements.
 hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream) {
-    // (rows that begin off 16 bytes cost what their lines cost; what WHOLE spares is the code for the end of a row)
+    // (what WHOLE spares is the code for the end of a row: 8192 rows of 2048 28.5 / 29.9 us)
     const bool whole = p.dim % 8 == 0;
 #define PSG_NORM_T(XT_, WT_) return whole ? launch<XT_, WT_, true>(p, stream) : launch<XT_, WT_, false>(p, stream);
     switch (x_dtype) {

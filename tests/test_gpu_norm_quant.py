@@ -248,3 +248,21 @@ def test_sizes_refused():
             quant_device.rmsnorm_quant(one.expand(1 << 31, 1), one[0], out=out, stream=stream)
         with pytest.raises(ValueError, match="2\\^31"):
             quant_device.rmsnorm_quant(one.expand(1, (1 << 24) + 1), one.expand(1, (1 << 24) + 1), out=out, stream=stream)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vecs", [1, 64, 65, 256, 513, 4100])
+def test_every_end_of_a_row(vecs, dt):
+    """Ends of one to seven elements, the residual in place, in launches of few and of many rows; what stands between the rows stays as it is."""
+    for end in range(1, 8):
+        dim = vecs * 8 + end
+        for rows in (3, 2300) if dim < 2048 else (3,):
+            x, w, r = _inputs(rows, dim, dt, True, seed=dim)
+            wide = torch.full((rows, dim + 11), -5.0, dtype=dt, device="cuda")
+            h = wide[:, :dim]
+            h.copy_(r)
+            y = torch.full_like(wide, -6.0)
+            out = torch.empty(rows, dim, dtype=torch.uint8, device="cuda"), torch.empty(rows, 1, device="cuda")
+            q, s = quant_device.rmsnorm_quant(x, w, 1e-6, residual=h, normed=y[:, :dim], out=out, stream=torch.cuda.current_stream())
+            _check(x, w, r, 1e-6, FP8, q, s, h, y[:, :dim])
+            assert (wide[:, dim:] == -5).all() and (y[:, dim:] == -6).all()
