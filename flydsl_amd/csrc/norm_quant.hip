@@ -10,8 +10,8 @@
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
 // Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
-// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes cost nothing (8192 of
-// 2048, 2048 to 2056 elements apart, 26.3 to 28.5 us); an end that is no whole vector does a little: 2047 27.6; where it is a thread's second vector, 2056 30.0, 2050 to 2054 33 to 34, 2049 39.9.
+// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes cost nothing (8192
+// of 2048, 2048 to 2056 elements apart, 26.3 to 28.5 us), off four bytes some, and so does an end that is no whole vector: 2048 24.7, 2056 27.8, 2050 30.4, 2047 30.3, 2049 35.5.
 #include "psg_common.h"
 #include "quant_rows.h"
 #include "norm_quant.h"
@@ -49,9 +49,8 @@ __device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n,
 }
 
 // the last n of the eight elements to the front, zeros behind them
-template <int XT, bool WHOLE>
-__device__ __forceinline__ void line_up(Raw8<XT>& r, int n, int dim) {
-    if (WHOLE || n >= 8 || dim < 8) return;
+template <int XT>
+__device__ __forceinline__ void line_up(Raw8<XT>& r, int n) {
     if constexpr (XT == X_F32) {
         int v[15];
 #pragma unroll
@@ -126,17 +125,15 @@ __device__ __forceinline__ float times_over(float v, float d, float m, float rm)
     return __builtin_copysignf(q, v);
 }
 
-// A row belongs to NT threads: one wavefront (four rows a workgroup, no barrier) or a workgroup.  The first KEEP 8-element vectors of every thread stay in registers; a
+// A row belongs to a workgroup of up to MOST threads.  (Four rows a workgroup, one to a wavefront, without the barrier, were level: 8192 rows of 280 6.9 / 7.3 us, of 512 9.2 / 8.1.)  The first KEEP 8-element vectors of every thread stay in registers; a
 // longer row writes its h, or has it in x, and reads the rest of it once more, every thread what it has written itself.
 // WHOLE: rows are whole vectors.  WT: type of the weight.
-template <int XT, int WT, int NT, int KEEP, bool WHOLE>
-__global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParams p) {
-    __shared__ float red_s[NT / 64];
-    __shared__ uint32_t red_m[NT / 64];
-    const int wave = wave_id();
-    const int64_t row = NT == 64 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
-    if (NT == 64 && row >= p.rows) return;  // a whole wavefront; no barrier follows
-    const int tid = NT == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+template <int XT, int WT, int MOST, int KEEP, bool WHOLE>
+__global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
+    __shared__ float red_s[MOST / 64];
+    __shared__ uint32_t red_m[MOST / 64];
+    const int NT = (int)blockDim.x, tid = (int)threadIdx.x, wave = wave_id();
+    const int64_t row = blockIdx.x;
     const int nvec = (p.dim + 7) >> 3;
     const int64_t xb = row * p.x_stride, rb = row * p.r_stride, hb = row * p.h_stride, nb = row * p.n_stride, qb = row * (int64_t)p.dim;
     auto left = [&](int vi) { return p.dim - vi * 8; };
@@ -154,11 +151,11 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
             mb = u > mb ? u : mb;
         }
     };
-    auto add = [&](Raw8<XT> x, Raw8<XT> r, int vi, bool live, float* h) __attribute__((always_inline)) {
-        if (live) line_up<XT, WHOLE>(x, left(vi), p.dim);
+    // (a vector that begins less than eight elements in front of the row's end, of a row that has eight)
+    auto is_end = [&](int vi) { return !WHOLE && left(vi) < 8 && p.dim >= 8; };
+    auto add = [&](const Raw8<XT>& x, const Raw8<XT>& r, int vi, bool live, float* h) __attribute__((always_inline)) {
         x.values(h);
         if (p.residual) {
-            if (live) line_up<XT, WHOLE>(r, left(vi), p.dim);
             float v[8];
             r.values(v);
 #pragma unroll
@@ -185,9 +182,13 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
 #pragma unroll
         for (int it = 0; it < KEEP; it++) {
             const bool live = tid + it * NT < nvec;
+            if (live && is_end(tid + it * NT)) {
+                line_up<XT>(x[it], left(tid + it * NT));
+                line_up<XT>(r[it], left(tid + it * NT));
+                line_up<WT>(w[it], left(tid + it * NT));
+            }
             float h[8], wv[8];
             add(x[it], r[it], tid + it * NT, live, h);
-            if (live) line_up<WT, WHOLE>(w[it], left(tid + it * NT), p.dim);
             w[it].values(wv);
             if (!live) {
 #pragma unroll
@@ -197,10 +198,14 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
         }
     }
     for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
-        const Raw8<XT> x = load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
-        const Raw8<XT> r = p.residual ? load_row<XT, WHOLE>(p.residual, rb + (int64_t)vi * 8, left(vi), p.dim) : x;
+        Raw8<XT> x = load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
+        Raw8<XT> r = p.residual ? load_row<XT, WHOLE>(p.residual, rb + (int64_t)vi * 8, left(vi), p.dim) : x;
         Raw8<WT> wr = weights(vi);
-        line_up<WT, WHOLE>(wr, left(vi), p.dim);
+        if (is_end(vi)) {
+            line_up<XT>(x, left(vi));
+            line_up<XT>(r, left(vi));
+            line_up<WT>(wr, left(vi));
+        }
         float w[8], h[8], y[8];
         wr.values(w);
         add(x, r, vi, true, h);
@@ -214,15 +219,12 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
             const uint32_t o = (uint32_t)__shfl_xor((int)m, off, 64);
             m = o > m ? o : m;
         }
-        if constexpr (NT > 64) {
-            if ((tid & 63) == 0) red_s[wave] = s, red_m[wave] = m;
-            __syncthreads();
-            s = red_s[0], m = red_m[0];
-#pragma unroll
-            for (int i = 1; i < NT / 64; i++) {
-                s += red_s[i];
-                m = red_m[i] > m ? red_m[i] : m;
-            }
+        if ((tid & 63) == 0) red_s[wave] = s, red_m[wave] = m;
+        __syncthreads();
+        s = red_s[0], m = red_m[0];
+        for (int i = 1; i < NT / 64; i++) {
+            s += red_s[i];
+            m = red_m[i] > m ? red_m[i] : m;
         }
     };
     over_row(sum, mb);
@@ -232,8 +234,10 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
     auto again = [&](int vi, float* v) __attribute__((always_inline)) {
         Raw8<XT> h = p.residual ? load_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi), p.dim) : load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
         Raw8<WT> wr = weights(vi);
-        line_up<XT, WHOLE>(h, left(vi), p.dim);
-        line_up<WT, WHOLE>(wr, left(vi), p.dim);
+        if (is_end(vi)) {
+            line_up<XT>(h, left(vi));
+            line_up<WT>(wr, left(vi));
+        }
         float w[8];
         h.values(v);
         wr.values(w);
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
                 for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(clean(v[e] * rinv, dmax)));
             }
             uint32_t bits = __builtin_bit_cast(uint32_t, m);
-            if constexpr (NT > 64) __syncthreads();  // everybody has read what over_row left
+            __syncthreads();  // everybody has read what over_row left
             over_row(unused, bits);
             amax = __builtin_bit_cast(float, bits);
         }
@@ -309,13 +313,14 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) k_rmsnorm_quant(NormParam
     }
 }
 
-// NT threads a row, in launches of 2^31 threads at most: a grid holds no more than 2^32
-template <int XT, int WT, int NT, int KEEP, bool WHOLE>
-hipError_t launch_rows(NormParams p, hipStream_t stream) {
-    constexpr int64_t most = (1ll << 31) / NT, B = XT == X_F32 ? 4 : 2;
+// `threads` a row, in launches of 2^31 threads at most: a grid holds no more than 2^32
+template <int XT, int WT, int MOST, int KEEP, bool WHOLE>
+hipError_t launch_rows(NormParams p, int threads, hipStream_t stream) {
+    constexpr int64_t B = XT == X_F32 ? 4 : 2;
+    const int64_t most = (1ll << 31) / MOST;
     for (int64_t left = p.rows;; left -= most) {
         p.rows = left < most ? left : most;
-        hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, NT, KEEP, WHOLE>), dim3(NT == 64 ? (unsigned)((p.rows + 3) / 4) : (unsigned)p.rows), dim3(NT == 64 ? 256 : NT), 0, stream, p);
+        hipLaunchKernelGGL((k_rmsnorm_quant<XT, WT, MOST, KEEP, WHOLE>), dim3((unsigned)p.rows), dim3(threads), 0, stream, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || left <= most) return e;
         p.x = static_cast<const uint8_t*>(p.x) + most * p.x_stride * B;
@@ -331,21 +336,18 @@ hipError_t launch_rows(NormParams p, hipStream_t stream) {
 template <int XT, int WT, bool WHOLE>
 hipError_t launch(const NormParams& p, hipStream_t stream) {
     const int nvec = (p.dim + 7) / 8;
-#define PSG_NORM(NT_, KEEP_) return launch_rows<XT, WT, NT_, KEEP_, WHOLE>(p, stream);
-    // Threads of a row, us, bf16 to fp8 with a residual.  A wavefront or four: 8192 rows of 1024 13.6 / 16.0, 2048 of 2048 8.7 / 8.8, 777 of 2048 5.3 / 4.4.
-    if (nvec <= 256 && p.rows >= 8 * psg_cu_count()) {
-        if (nvec <= 64) PSG_NORM(64, 1)
-        PSG_NORM(64, 4)
-    }
-    if (nvec <= 256) PSG_NORM(256, 1)
-    // Eight wavefronts or four: with few rows a thread's second vector is what a row waits for, 1 row of 4096 2.9 / 3.1, 256 3.7 / 3.9, 777 7.5 / 7.2, 8192 46.8 / 44.6;
-    // 1 of 8192 3.5 / 4.0, 8192 80.6 / 81.9.
-    if (nvec <= 512 && p.rows > 2 * psg_cu_count()) PSG_NORM(256, 2)
-    if (nvec <= 512) PSG_NORM(512, 1)
-    if (nvec <= 1024) PSG_NORM(512, 2)
-    // Sixteen or eight: 777 of 16384 19.4 / 20.2, 8192 163 / 162; longer rows keep twice as much, and beyond 32768 come back for the rest.
-    if (nvec <= 2048) PSG_NORM(1024, 2)
-    PSG_NORM(1024, 4)
+    const int64_t cus = psg_cu_count();
+#define PSG_NORM(MOST_, KEEP_) return launch_rows<XT, WT, MOST_, KEEP_, WHOLE>(p, (nvec + KEEP_ * 64 - 1) / (KEEP_ * 64) * 64, stream);
+    // Vectors of a thread; as many wavefronts as the row then fills (all sixteen of 1024 threads where nine have work: 8192 rows of 9042 169 us / 111).  us, bf16 to fp8 with a residual, one vector / two / four:
+    // few and short rows want their loads at once, 4 rows of 1204 3.3 / 3.9 / 4.5, 777 of 2051 5.9 / 6.4 / 7.5; of many rows a CU holds more that way, 8192 of 2048 26.8 / 24.5 / 25.1, of 2880 40.7 / 33.4 / 33.5, of
+    // 5120 70 / 54.6 / 54.2; with the code for a row's end 8192 of 5124 82 / 66 / 59, but 300 5.8 / 6.1 / 6.6.
+    if (nvec <= 64 || (nvec <= 320 && p.rows * nvec <= 1024 * cus)) PSG_NORM(512, 1)
+    if (nvec <= 512 || (nvec <= 1024 && (WHOLE || p.rows <= 4 * cus))) PSG_NORM(512, 2)
+    // Longer ones two / four: 4 of 9042 4.7 / 5.5, 1100 of 12288 20.9 / 22.8, 8192 122 / 125, but with the code for a row's end 8192 of 9715 147 / 136, and 13 to 15 wavefronts leave room for no second
+    // workgroup beside them, 8192 of 14336 157 / 143.
+    if (nvec > 1024 && nvec <= 1536 && (WHOLE || p.rows <= 4 * cus)) PSG_NORM(1024, 2)
+    if (nvec <= 2048) PSG_NORM(512, 4)
+    return launch_rows<XT, WT, 1024, 4, WHOLE>(p, nvec > 4096 ? 1024 : (nvec + 255) / 256 * 64, stream);  // (beyond 32768 elements threads come back for the rest)
 #undef PSG_NORM
 }
 
