@@ -50,13 +50,14 @@ __device__ __forceinline__ int of_lane(int x) { return __builtin_amdgcn_update_d
 constexpr int W4_WAVES = 8, W4_LDS = 160 * 1024;
 
 // MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  SH: those that come through LDS at a time.  MANY: several
-// passes.
-template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY>
+// passes.  ROWS: rows that the patch has room for, 16 MB or (one block of at most so many rows) 8.
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY, int ROWS>
 __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     constexpr int NW = W4_WAVES;
     constexpr int GPS = 128 / GS, MPG = GS / 32;              // groups of a step, MFMAs of a group
-    constexpr int CPR = SH * 16, PATCH = MB * 16 * CPR * 16;  // 16-byte pieces of a staged row, bytes of a wavefront's patch
+    constexpr int CPR = SH * 16, PATCH = ROWS * CPR * 16;  // 16-byte pieces of a staged row, bytes of a wavefront's patch
     static_assert(SPW * GPS <= 16, "a load of scales holds 16 groups");
+    static_assert(ROWS == 16 * MB || (MB == 1 && ROWS == 8), "rows of the patch");
     static_assert(!MANY || SH == SPW, "the next pass's part of A lies in the patch");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[MANY ? W4_LDS : NW * PATCH];
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -221,16 +222,17 @@ __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     }
 }
 
-template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY>
+// (ROWS 8: M <= 8)
+template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY, int ROWS = 16 * MB>
 hipError_t go(W4Params p, hipStream_t stream) {
     const int steps = (p.K + 127) / 128;
     p.passes = (steps + W4_WAVES * SPW - 1) / (W4_WAVES * SPW);
     p.per = (steps + W4_WAVES * p.passes - 1) / (W4_WAVES * p.passes);
     // a workgroup has LDS for the sums of so many windows of 16 columns, which begin at a multiple of 8
-    constexpr int PATCH = MB * SH * 4096, windows = MANY ? (W4_LDS - W4_WAVES * PATCH) / (W4_WAVES * MB * 1024) : PATCH / (MB * 1024), most = 2 * windows;
+    constexpr int PATCH = ROWS * SH * 256, windows = MANY ? (W4_LDS - W4_WAVES * PATCH) / (W4_WAVES * MB * 1024) : PATCH / (MB * 1024), most = 2 * windows;
     const long units = p.N / 8, cus = psg_cu_count(), rounds = (units + most * cus - 1) / (most * cus), wgs = units < cus * rounds ? units : cus * rounds;
     p.unit_q = (int)(units / wgs), p.unit_r = (int)(units % wgs);
-    hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, SH, MANY>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), 0, stream, p);
+    hipLaunchKernelGGL((k_w4a16<BF16, MB, GS, ZP, SPW, SH, MANY, ROWS>), dim3((unsigned)wgs, (unsigned)((p.M + MB * 16 - 1) / (MB * 16))), dim3(W4_WAVES * 64), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -250,8 +252,16 @@ hipError_t launch(const W4Params& p, hipStream_t stream) {
     }
     if (per <= 2) return go<BF16, 1, GS, ZP, 2, 2, false>(p, stream);
     if (per <= 4) return go<BF16, 1, GS, ZP, 4, 4, false>(p, stream);
-    // eight steps fit with the sums of eight groups, not with those of 16 (the build spilled: 4x5120x6144 in groups of 64 29 us, in passes 9)
+    // Five to eight steps in one pass, where the sums of their groups fit beside them: five come through LDS at once, of up to eight rows all of them, else three or four and again as many.  us in
+    // passes of two / in halves / at once: 1x5120x5120 7.8 / 6.9 / 5.9, 16x13824x5120 13.5 / 11.5 / 10.3, 4x5120x6144 in groups of 64 8.4 / 8.1 / 7.4; 1x4096x7168 - / 6.2 / 5.6.  (Eight with 16 groups' sums spill: 4x5120x6144
+    // in groups of 64 29; long rows of eight rows in passes of six or eight were level or spilled.)
+    if constexpr (GS >= 64) {
+        if (per == 5) return go<BF16, 1, GS, ZP, 5, 5, false>(p, stream);
+        if (per == 6 && p.M <= 8) return go<BF16, 1, GS, ZP, 6, 6, false, 8>(p, stream);
+        if (per == 6) return go<BF16, 1, GS, ZP, 6, 3, false>(p, stream);
+    }
     if constexpr (GS == 128) {
+        if (per <= 8 && p.M <= 8) return go<BF16, 1, GS, ZP, 8, 8, false, 8>(p, stream);
         if (per <= 8) return go<BF16, 1, GS, ZP, 8, 4, false>(p, stream);
     }
     // 16 rows: passes of four steps leave LDS for four windows a workgroup, passes of two for twelve.  us four / two: 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but more windows a CU

@@ -79,6 +79,12 @@ def test_exact_sums(m, n, k, group, zero_points, dtype):
     assert torch.equal(got, want.to(dt))
 
 
+@pytest.mark.parametrize("m,n,k", [(16, 1040, 4224), (1, 528, 5120), (40, 272, 5120), (8, 1040, 5248), (9, 1040, 5376), (3, 4112, 6144), (16, 4112, 6144), (8, 528, 6272), (1, 8208, 7168), (7, 1040, 8192), (9, 1040, 8192)])
+@pytest.mark.parametrize("group,zero_points,dtype", [(128, False, "fp16"), (128, True, "bf16"), (64, True, "fp16"), (64, False, "bf16")])
+def test_exact_sums_of_five_to_eight_steps(m, n, k, group, zero_points, dtype):
+    test_exact_sums(m, n, k, group, zero_points, dtype)
+
+
 @pytest.mark.parametrize("epi", ["none", "bias", "bias_relu", "bias_silu", "bias_gelu"])
 @pytest.mark.parametrize("m,n,k,group,zero_points,dtype", [(1, 1024, 4096, 128, True, "bf16"), (9, 528, 2080, 32, True, "fp16"), (31, 320, 960, 64, False, "bf16")])
 def test_random_values_and_epilogues(m, n, k, group, zero_points, dtype, epi):
