@@ -50,14 +50,14 @@ __device__ __forceinline__ int of_lane(int x) { return __builtin_amdgcn_update_d
 constexpr int W4_WAVES = 8, W4_LDS = 160 * 1024;
 
 // MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  SH: those that come through LDS at a time.  MANY: several
-// passes.  ROWS: rows that the patch has room for, 16 MB or (one block of at most so many rows) 8.
+// passes.  ROWS: rows that the patch has room for, 16 MB, or less where M is not more.
 template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY, int ROWS>
 __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     constexpr int NW = W4_WAVES;
     constexpr int GPS = 128 / GS, MPG = GS / 32;              // groups of a step, MFMAs of a group
     constexpr int CPR = SH * 16, PATCH = ROWS * CPR * 16;  // 16-byte pieces of a staged row, bytes of a wavefront's patch
     static_assert(SPW * GPS <= 16, "a load of scales holds 16 groups");
-    static_assert(ROWS == 16 * MB || (MB == 1 && ROWS == 8), "rows of the patch");
+    static_assert(ROWS > 16 * (MB - 1) && ROWS <= 16 * MB && PATCH % 1024 == 0, "rows of the patch, whole instructions of DMA");
     static_assert(!MANY || SH == SPW, "the next pass's part of A lies in the patch");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[MANY ? W4_LDS : NW * PATCH];
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     }
 }
 
-// (ROWS 8: M <= 8)
+// (ROWS below 16 MB: M <= ROWS)
 template <bool BF16, int MB, int GS, bool ZP, int SPW, int SH, bool MANY, int ROWS = 16 * MB>
 hipError_t go(W4Params p, hipStream_t stream) {
     const int steps = (p.K + 127) / 128;
@@ -244,7 +244,12 @@ hipError_t launch(const W4Params& p, hipStream_t stream) {
     // more columns 16 rows at a time are level or better (32x28672x8192 47.7 / 55.8).
     if (p.M > 16) {
         if (per <= 2) return go<BF16, 2, GS, ZP, 2, 2, false>(p, stream);
-        if constexpr (GS == 128) {
+        // three and four steps in one pass, where they fit the registers: of up to 24 rows three come through LDS at once, 24x2048x2560 in halves / like this 6.1 / 5.1, 20x6144x2560 in groups of 64 in passes / like
+        // this 7.8 / 6.4, 20x4096x2880 of 32 6.6 / 5.4; four in halves, in groups of 64 in passes / like this 28x28672x4096 27.5 / 17.7, 28x8192x4096 8.7 / 8.3
+        if constexpr (GS > 32 || !ZP) {
+            if (per == 3 && p.M <= 24) return go<BF16, 2, GS, ZP, 3, 3, false, 24>(p, stream);
+        }
+        if constexpr (GS == 128 || (GS == 64 && !ZP)) {
             if (per <= 4) return go<BF16, 2, GS, ZP, 4, 2, false>(p, stream);
         }
         if (p.N <= 32 * psg_cu_count()) return go<BF16, 2, GS, ZP, 2, 2, true>(p, stream);

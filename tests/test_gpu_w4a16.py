@@ -85,6 +85,12 @@ def test_exact_sums_of_five_to_eight_steps(m, n, k, group, zero_points, dtype):
     test_exact_sums(m, n, k, group, zero_points, dtype)
 
 
+@pytest.mark.parametrize("m,n,k", [(17, 528, 2176), (23, 1040, 2688), (24, 4112, 2944), (25, 528, 2944), (32, 1040, 3200), (24, 272, 4096)])
+@pytest.mark.parametrize("group,zero_points,dtype", [(128, True, "bf16"), (64, False, "bf16"), (64, True, "fp16"), (32, False, "bf16"), (32, True, "fp16")])
+def test_exact_sums_of_three_and_four_steps(m, n, k, group, zero_points, dtype):
+    test_exact_sums(m, n, k, group, zero_points, dtype)
+
+
 @pytest.mark.parametrize("epi", ["none", "bias", "bias_relu", "bias_silu", "bias_gelu"])
 @pytest.mark.parametrize("m,n,k,group,zero_points,dtype", [(1, 1024, 4096, 128, True, "bf16"), (9, 528, 2080, 32, True, "fp16"), (31, 320, 960, 64, False, "bf16")])
 def test_random_values_and_epilogues(m, n, k, group, zero_points, dtype, epi):
