@@ -236,27 +236,35 @@ hipError_t go(W4Params p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// The steps of a wavefront's part of A are built to the number: a step too many is a window's MFMAs for nothing, at every window.  us with two or four for one or three / to the number:
+// 1x28672x1024 7.6 / 5.9, 16x28672x2560 12.5 / 10.7, 4x4096x1024 3.3 / 3.1, 32x28672x1024 10.4 / 8.1, 8x18432x7168 19.3 / 16.4.
 template <bool BF16, int GS, bool ZP>
 hipError_t launch(const W4Params& p, hipStream_t stream) {
     const int per = ((p.K + 127) / 128 + W4_WAVES - 1) / W4_WAVES;  // steps of a wavefront
-    // 17 to 32 rows read W once: where A fits the registers, 16 rows at a time / like this, 32x7168x2048 8.1 / 5.9, 32x4096x4096 8.6 / 6.8; longer rows in passes of two steps, which leave LDS for
-    // two windows a workgroup, 32x8192x8192 22.9 / 16.0, 17x8192x5120 15.5 / 10.3, or of one, for six, 24x12288x6144 22.7 / 18.1, 32x14336x4096 in groups of 32 20.2 / 16.6 (of two 18.7).  With still
-    // more columns 16 rows at a time are level or better (32x28672x8192 47.7 / 55.8).
+    const int64_t cus = psg_cu_count();
+    // 17 to 32 rows read W once: where A fits the registers, 16 rows at a time / like this, 32x7168x2048 8.1 / 5.9, 32x4096x4096 8.6 / 6.8
     if (p.M > 16) {
-        if (per <= 2) return go<BF16, 2, GS, ZP, 2, 2, false>(p, stream);
-        // three and four steps in one pass, where they fit the registers: of up to 24 rows three come through LDS at once, 24x2048x2560 in halves / like this 6.1 / 5.1, 20x6144x2560 in groups of 64 in passes / like
-        // this 7.8 / 6.4, 20x4096x2880 of 32 6.6 / 5.4; four in halves, in groups of 64 in passes / like this 28x28672x4096 27.5 / 17.7, 28x8192x4096 8.7 / 8.3
+        if (per == 1) return go<BF16, 2, GS, ZP, 1, 1, false>(p, stream);
+        if (per == 2) return go<BF16, 2, GS, ZP, 2, 2, false>(p, stream);
+        // of up to 24 rows three steps come through LDS at once, 24x2048x2560 in halves / like this 6.1 / 5.1, 20x6144x2560 in groups of 64 in passes / like this 7.8 / 6.4, 20x4096x2880 of 32 6.6 / 5.4;
+        // four in halves, in groups of 64 in passes / like this 28x28672x4096 27.5 / 17.7, 28x8192x4096 8.7 / 8.3
         if constexpr (GS > 32 || !ZP) {
             if (per == 3 && p.M <= 24) return go<BF16, 2, GS, ZP, 3, 3, false, 24>(p, stream);
         }
         if constexpr (GS == 128 || (GS == 64 && !ZP)) {
             if (per <= 4) return go<BF16, 2, GS, ZP, 4, 2, false>(p, stream);
         }
-        if (p.N <= 32 * psg_cu_count()) return go<BF16, 2, GS, ZP, 2, 2, true>(p, stream);
-        if (p.N <= 96 * psg_cu_count()) return go<BF16, 2, GS, ZP, 1, 1, true>(p, stream);
+        // longer rows in passes of two steps, which leave LDS for two windows a workgroup, 16 rows at a time / like this 32x8192x8192 22.9 / 16.0, 17x8192x5120 15.5 / 10.3, of up to 24 rows for four, passes of
+        // one / of two 24x12288x6144 19.4 / 14.9, 17x16384x8192 28.1 / 22.9; or of one, for six, 16 rows at a time / of one 32x14336x4096 in groups of 32 20.2 / 16.6 (of two 18.7).  With still more columns 16 rows
+        // at a time are level or better (32x28672x8192 47.7 / 55.8).
+        if (p.N <= 32 * cus) return go<BF16, 2, GS, ZP, 2, 2, true>(p, stream);
+        if (p.M <= 24 && p.N <= 64 * cus) return go<BF16, 2, GS, ZP, 2, 2, true, 24>(p, stream);
+        if (p.N <= 96 * cus) return go<BF16, 2, GS, ZP, 1, 1, true>(p, stream);
     }
-    if (per <= 2) return go<BF16, 1, GS, ZP, 2, 2, false>(p, stream);
-    if (per <= 4) return go<BF16, 1, GS, ZP, 4, 4, false>(p, stream);
+    if (per == 1) return go<BF16, 1, GS, ZP, 1, 1, false>(p, stream);
+    if (per == 2) return go<BF16, 1, GS, ZP, 2, 2, false>(p, stream);
+    if (per == 3) return go<BF16, 1, GS, ZP, 3, 3, false>(p, stream);
+    if (per == 4) return go<BF16, 1, GS, ZP, 4, 4, false>(p, stream);
     // Five to eight steps in one pass, where the sums of their groups fit beside them: five come through LDS at once, of up to eight rows all of them, else three or four and again as many.  us in
     // passes of two / in halves / at once: 1x5120x5120 7.8 / 6.9 / 5.9, 16x13824x5120 13.5 / 11.5 / 10.3, 4x5120x6144 in groups of 64 8.4 / 8.1 / 7.4; 1x4096x7168 - / 6.2 / 5.6.  (Eight with 16 groups' sums spill: 4x5120x6144
     // in groups of 64 29; long rows of eight rows in passes of six or eight were level or spilled.)
@@ -266,13 +274,18 @@ hipError_t launch(const W4Params& p, hipStream_t stream) {
         if (per == 6) return go<BF16, 1, GS, ZP, 6, 3, false>(p, stream);
     }
     if constexpr (GS == 128) {
-        if (per <= 8 && p.M <= 8) return go<BF16, 1, GS, ZP, 8, 8, false, 8>(p, stream);
+        if (per == 7 && p.M <= 8) return go<BF16, 1, GS, ZP, 7, 7, false, 8>(p, stream);
+        if (per == 8 && p.M <= 8) return go<BF16, 1, GS, ZP, 8, 8, false, 8>(p, stream);
         if (per <= 8) return go<BF16, 1, GS, ZP, 8, 4, false>(p, stream);
     }
-    // 16 rows: passes of four steps leave LDS for four windows a workgroup, passes of two for twelve.  us four / two: 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but more windows a CU
-    // 16x28672x8192 in groups of 64 36.7 / 33.6, five and six steps, which two divide better, 4x5120x6144 10.0 / 9.0, 1x6144x6144 9.9 / 8.7, and groups of 32 with zero points,
-    // which take all registers, 2x8192x10240 16.9 / 14.9
-    if (per <= 6 || p.N > 64 * psg_cu_count() || (GS == 32 && ZP)) return go<BF16, 1, GS, ZP, 2, 2, true>(p, stream);
+    // Longer rows in as few passes of up to four steps as there are, which leave LDS for four windows a workgroup, three steps where that is what the passes come to or for eight windows, two for twelve.  us four / three:
+    // 1x8192x9216 10.5 / 9.3, 16x20480x9216 27.5 / 23.5, 13x1536x8256 in groups of 32 10.3 / 8.7; two / three 3x18432x13824 32.4 / 28.7, 16x17408x16384 42.7 / 37.9, 16x13824x5120 in groups of 32 with zero
+    // points 18.0 / 17.3; four / two 16x12288x7168 13.1 / 14.5, 9x3584x18944 12.8 / 14.4, 1x8192x28672 23.3 / 27.3; but groups of 32 with zero points, whose four steps take all registers, 2x8192x10240 16.9 / 14.9
+    // (three 17.1).
+    const int passes = (per + 3) / 4, each = (per + passes - 1) / passes;
+    const bool all_registers = GS == 32 && ZP, wide = p.N > 64 * cus;
+    if ((each == 3 || (wide && !all_registers)) && p.N <= 128 * cus) return go<BF16, 1, GS, ZP, 3, 3, true>(p, stream);
+    if (wide || all_registers) return go<BF16, 1, GS, ZP, 2, 2, true>(p, stream);
     return go<BF16, 1, GS, ZP, 4, 4, true>(p, stream);
 }
 

@@ -91,6 +91,13 @@ def test_exact_sums_of_three_and_four_steps(m, n, k, group, zero_points, dtype):
     test_exact_sums(m, n, k, group, zero_points, dtype)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 528, 896), (16, 28688, 1024), (33, 1040, 1024), (17, 528, 768), (8, 4112, 2816), (16, 28688, 2560), (7, 1040, 7168), (1, 528, 9216), (16, 4112, 8832), (9, 16912, 9216), (3, 17424, 8320),
+                                   (24, 8720, 6144), (17, 528, 5248), (20, 16400, 4224)])
+@pytest.mark.parametrize("group,zero_points,dtype", [(128, False, "bf16"), (64, True, "bf16"), (32, False, "fp16"), (32, True, "bf16")])
+def test_exact_sums_of_other_steps_and_passes(m, n, k, group, zero_points, dtype):
+    test_exact_sums(m, n, k, group, zero_points, dtype)
+
+
 @pytest.mark.parametrize("epi", ["none", "bias", "bias_relu", "bias_silu", "bias_gelu"])
 @pytest.mark.parametrize("m,n,k,group,zero_points,dtype", [(1, 1024, 4096, 128, True, "bf16"), (9, 528, 2080, 32, True, "fp16"), (31, 320, 960, 64, False, "bf16")])
 def test_random_values_and_epilogues(m, n, k, group, zero_points, dtype, epi):
