@@ -271,9 +271,9 @@ __global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
             amax = __builtin_bit_cast(float, bits);
         }
         s = amax / dmax;
-        if (s == 0.0f) s = 1.0f;
-        if (tid == 0) p.scale[row] = s;
         exact = !special && s >= 0x1p-80f && s <= 0x1p100f && mhw >= 0x1p-80f && mhw <= 0x1p100f;
+        if (s == 0.0f) s = 1.0f;  // (a row of zeros, or of values whose scale is rounded to zero, and their codes with it)
+        if (tid == 0) p.scale[row] = s;
     }
     auto finish = [&](int vi, const float* v) __attribute__((always_inline)) {
         const int n = left(vi);

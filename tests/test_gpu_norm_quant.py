@@ -266,3 +266,20 @@ def test_every_end_of_a_row(vecs, dt):
             q, s = quant_device.rmsnorm_quant(x, w, 1e-6, residual=h, normed=y[:, :dim], out=out, stream=torch.cuda.current_stream())
             _check(x, w, r, 1e-6, FP8, q, s, h, y[:, :dim])
             assert (wide[:, dim:] == -5).all() and (y[:, dim:] == -6).all()
+
+
+def test_scale_that_is_rounded_to_zero():
+    """A row whose values are below the smallest scale has scale 1, and codes of what the values are then, none, however far from zero h is: 2^-142 / 448 is below half of the smallest
+    number, 2^-149.  2^-142 / 127 = 2^-148.99 is rounded to it, and 2^-142 / 2^-149 = 128 is held at 127."""
+    h = torch.full((3, 8), 2.0**62, device="cuda")
+    h[:, 1::2] *= -1
+    h[1] = 0
+    w = torch.full((8,), 2.0**-142, device="cuda")
+    for qd in (FP8, torch.int8):
+        normed = torch.empty_like(h)
+        q, s = quant_device.rmsnorm_quant(h, w, quant_dtype=qd, normed=normed)
+        assert torch.equal(normed, h * 2.0**-62 * w)
+        if qd == FP8:
+            assert (s == 1).all() and (q.float() == 0).all()
+        else:
+            assert s.view(-1).tolist() == [2.0**-149, 1.0, 2.0**-149] and torch.equal(q.float(), h * (127 * 2.0**-62))
