@@ -9,6 +9,7 @@
 // One pass: the maximum does not need the norm, max|y| = max|h w| / rms with the same rounding (a product with a positive factor is monotone), so the sum of squares and
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
+// A row whose squares are beyond fp32 or below it (h from about 2^58 on; below 2^-50 with an eps below 2^-60) is read a second and a third time, scaled by powers of two.
 // Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
 // with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes cost nothing (8192
 // of 2048, 2048 to 2056 elements apart, 26.3 to 28.5 us), off four bytes some, and so does an end that is no whole vector: 2048 24.7, 2056 27.8, 2050 30.4, 2047 30.3, 2049 35.5.
@@ -228,10 +229,12 @@ __global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
         }
     };
     over_row(sum, mb);
-    const float rinv = 1.0f / __builtin_sqrtf(sum / (float)p.dim + p.eps);
+    const float mean = sum / (float)p.dim + p.eps;
+    float rinv = 1.0f / __builtin_sqrtf(mean);
+    int up = 0;  // h is taken times 2^up, rinv is of that
 
     // h w of a vector that is not in registers
-    auto again = [&](int vi, float* v) __attribute__((always_inline)) {
+    auto again = [&](int vi, float* v, bool product) __attribute__((always_inline)) {
         Raw8<XT> h = p.residual ? load_row<XT, WHOLE>(p.h, hb + (int64_t)vi * 8, left(vi), p.dim) : load_row<XT, WHOLE>(p.x, xb + (int64_t)vi * 8, left(vi), p.dim);
         Raw8<WT> wr = weights(vi);
         if (is_end(vi)) {
@@ -241,9 +244,66 @@ __global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
         float w[8];
         h.values(v);
         wr.values(w);
+        if (up) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = __builtin_ldexpf(v[e], up);
+        }
+        if (!product) return;
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] *= w[e];
     };
+
+    // Rows whose squares, whose sum of them or whose products with the weight leave fp32's range, though y does not, are taken once more: the sum of (h 2^-80)^2 or (h 2^100)^2, all of
+    // whose terms that matter are normal numbers, then h 2^up with a root mean square from 1/2 to 1, so that its products leave the range only where y does.  What the first sum
+    // is short of, squares below 2^-149, is less than 2^-125 and is nothing beside an eps from 2^-60 on.  (Infinities and NaN of h stay: their sum is none either way.)
+    const bool far_sum = mean == __builtin_inff() || (sum < 0x1p-100f && p.eps < 0x1p-60f);
+    // (What asks for it costs every launch 0.05 to 0.12 us: 67 rows of 8192 4.58 / 4.67, 8192 level.)
+    if (__builtin_expect(far_sum || mb == 0x7F800000u || (mb < 0x17800000u && sum > 0.f && mean < 0.25f), 0)) {  // (the bits of infinity and of 2^-80)
+        float sq = sum, unused_s = 0.f;
+        uint32_t m = 0;
+        if (sum == __builtin_inff()) up = -80;
+        else if (sum < 0x1p-100f) up = 100;
+        const int first = up;
+        if (first) {
+            sq = 0.f;
+            for (int vi = tid; vi < nvec; vi += NT) {
+                float h[8];
+                again(vi, h, false);
+#pragma unroll
+                for (int e = 0; e < 8; e++) sq = __builtin_fmaf(h[e], h[e], sq);
+            }
+            __syncthreads();  // everybody has read what over_row left
+            over_row(sq, m);
+        }
+        const double ms = __builtin_ldexp((double)sq, -2 * first) / p.dim + (double)p.eps;
+        up = 0;
+        if (ms > 0.0 && sq < __builtin_inff()) {
+            const double rms = __builtin_sqrt(ms);
+            up = -__builtin_amdgcn_frexp_exp(rms);
+            rinv = (float)(1.0 / __builtin_ldexp(rms, up));
+            mb = 0;
+            auto largest = [&](const float* v) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t u = __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu;
+                    mb = u > mb ? u : mb;
+                }
+            };
+#pragma unroll
+            for (int it = 0; it < KEEP; it++)
+                if (tid + it * NT < nvec) {
+                    again(tid + it * NT, hw[it], true);
+                    largest(hw[it]);
+                }
+            for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
+                float v[8];
+                again(vi, v, true);
+                largest(v);
+            }
+            __syncthreads();
+            over_row(unused_s, mb);
+        }
+    }
 
     const float dmax = p.out == NORM_FP8 ? 448.0f : 127.0f;
     float s = 1.0f;
@@ -261,7 +321,7 @@ __global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
                 for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(clean(hw[it][e] * rinv, dmax)));
             for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
                 float v[8];
-                again(vi, v);
+                again(vi, v, true);
 #pragma unroll
                 for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(clean(v[e] * rinv, dmax)));
             }
@@ -308,7 +368,7 @@ __global__ void __launch_bounds__(MOST) k_rmsnorm_quant(NormParams p) {
     }
     for (int vi = tid + KEEP * NT; vi < nvec; vi += NT) {
         float v[8];
-        again(vi, v);
+        again(vi, v, true);
         finish(vi, v);
     }
 }

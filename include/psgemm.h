@@ -462,6 +462,7 @@ int psg_moe_softmax_sorting(const psg_moe_gating_args *gating, const psg_moe_sor
  *   y = h * weight / sqrt(mean(h^2) + eps), fp32; normed NULL or y rounded to the type of x
  *   scale = max|y| / qmax (qmax 448 or 127; 1 for a row of zeros), q = y / scale by the rules of psg_quant_pertoken (NaN -> 0, +-Inf -> +-qmax, int8 towards zero, fp8
  *   to nearest even), from y before its rounding to fp32
+ * The squares of h, their sum and h * weight may be beyond fp32 or below its smallest number where y is not: such rows are taken again, scaled by powers of two.
  * x, residual, residual_out and normed are rows of dim elements, a stride of elements (0 = dim, and at least dim) apart, at addresses and strides that need only be
  * multiples of an element; q [rows, dim] is dense, scale [rows].  residual_out may be residual or x, normed may be x: every element is read before it is
  * written.  Other overlaps are not allowed.

@@ -283,3 +283,52 @@ def test_scale_that_is_rounded_to_zero():
             assert (s == 1).all() and (q.float() == 0).all()
         else:
             assert s.view(-1).tolist() == [2.0**-149, 1.0, 2.0**-149] and torch.equal(q.float(), h * (127 * 2.0**-62))
+
+
+def _far(rows, dim, dt, residual, seed, exponents):
+    x, w, r = _inputs(rows, dim, dt, residual, seed)
+    by = torch.tensor([2.0**e for e in exponents], dtype=torch.float64, device="cuda").unsqueeze(1)
+    return (x.double() * by).to(dt), w, None if r is None else (r.double() * by).to(dt)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [1, 7, 256, 4096, 5003, 9000, 12296, 40008, 40011])
+def test_rows_whose_squares_leave_the_range(dim, dt):
+    """h from 2^-120 to 2^118 beside ordinary rows: the squares, or their sum, are beyond fp32, the norm is not.  (With an eps, rows far below its root are h w / sqrt(eps), exact as far
+    as the products are normal numbers.)"""
+    for eps, exponents in ((0.0, (0, 59, 64, 90, 118, -50, -60, -64, -90, -120, 0, 30)), (1e-6, (0, 59, 64, 90, 118, -20, -50, -60, -70, 1, 0, 30))):
+        for residual, qd in ((True, FP8), (False, torch.int8)):
+            x, w, r = _far(12, dim, dt, residual, dim, exponents)
+            keep, normed = None if r is None else r.clone(), torch.empty_like(x)
+            q, s = quant_device.rmsnorm_quant(x, w, eps, residual=r, quant_dtype=qd, normed=normed)
+            _check(x, w, keep, eps, qd, q, s, r, normed)
+
+
+@pytest.mark.parametrize("dim", [2048, 41003])
+def test_rows_whose_squares_leave_the_range_in_place(dim):
+    exponents = (64, 0, -70, 110)
+    for residual in (False, True):
+        x, w, r = _far(4, dim, torch.bfloat16, residual, 3, exponents)
+        a = x.clone()
+        q, s = quant_device.rmsnorm_quant(a, w, 0.0, residual=None if r is None else r.clone(), normed=a)
+        _check(x, w, None if r is None else r, 0.0, FP8, q, s, (x.float() + r.float()).to(x.dtype) if residual else None, a)
+    a = x.clone()
+    q, s = quant_device.rmsnorm_quant(a, w, 0.0, residual=r, residual_out=a)
+    _check(x, w, r, 0.0, FP8, q, s, a, None)
+
+
+def test_products_with_the_weight_that_leave_the_range():
+    """h and y are numbers of fp32, h w is beyond the largest or below the smallest."""
+    x, _, _ = _inputs(6, 300, torch.float32, False, 5)
+    for e, f in ((55, 80), (30, 100), (-45, -60)):
+        h, w = x * 2.0**e, (torch.rand(300, generator=torch.Generator().manual_seed(1)) + 0.5).cuda() * 2.0**f
+        normed = torch.empty_like(h)
+        q, s = quant_device.rmsnorm_quant(h, w, 0.0, normed=normed)
+        _check(h, w, None, 0.0, FP8, q, s, None, normed)
+    # a scale below 2^-80: y is divided, with two roundings of y, three of the scale and one of the quotient
+    h, w = x * 2.0**-45, torch.full((300,), 2.0**-105, device="cuda")
+    q, s = quant_device.rmsnorm_quant(h, w, 0.0)
+    _, y, want = _exact(h, w, None, 0.0, FP8)
+    assert ((s.double() - want).abs() <= (300 / 64 + 40) * 2.0**-24 * want).all()
+    slack = 6 * 2.0**-24 * (y / want).abs()
+    assert ((q.double() - y / want).abs() <= torch.clamp(2.0**-4 * ((y / want).abs() + slack), min=2.0**-10) + slack).all()
