@@ -5,6 +5,7 @@ most dim / 64 squares one after the other (one wavefront a row; fewer with more 
 two products add at most 8.  The root halves what was before it.  So y and the scale are within (dim / 64 + 40) u relatively, and every output within that and its own rounding.
 """
 
+import numpy
 import pytest
 import torch
 
@@ -332,3 +333,14 @@ def test_products_with_the_weight_that_leave_the_range():
     assert ((s.double() - want).abs() <= (300 / 64 + 40) * 2.0**-24 * want).all()
     slack = 6 * 2.0**-24 * (y / want).abs()
     assert ((q.double() - y / want).abs() <= torch.clamp(2.0**-4 * ((y / want).abs() + slack), min=2.0**-10) + slack).all()
+
+
+def test_eps_that_is_no_python_number():
+    """A tensor or an array is read at every call."""
+    x, w, _ = _inputs(3, 256, torch.bfloat16, False, 6)
+    out = torch.empty(3, 256, dtype=FP8, device="cuda"), torch.empty(3, 1, device="cuda")
+    for eps in (torch.tensor(1e-6), numpy.array(1e-6)):
+        for value in (1e-6, 4.0):
+            eps[...] = value
+            q, s = quant_device.rmsnorm_quant(x, w, eps, stream=torch.cuda.current_stream(), out=out)
+            _check(x, w, None, value, FP8, q, s, None, None)
