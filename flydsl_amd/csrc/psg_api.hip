@@ -1336,6 +1336,7 @@ int psg_rmsnorm_quant(const psg_rmsnorm_args* a, void* stream) {
     if (!a->x || !a->weight) return fail(PSG_E_NULL, "x and weight must be non-NULL");
     if (quant ? !a->q || !a->scale : !a->normed) return fail(PSG_E_NULL, quant ? "q and scale must be non-NULL" : "normed must be non-NULL without a quantised output");
     if (a->residual && !a->residual_out) return fail(PSG_E_NULL, "residual_out must be non-NULL with a residual");
+    if (a->residual && a->normed == a->residual_out) return fail(PSG_E_SHAPE, "normed and residual_out are the same rows: one of the two would be lost");
     const int64_t strides[4] = {a->x_stride, a->residual_stride, a->residual_out_stride, a->normed_stride};
     int64_t s[4];
     for (int i = 0; i < 4; i++) {

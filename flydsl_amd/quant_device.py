@@ -156,7 +156,7 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     value, int8 towards zero), but from ``y`` before it is rounded; with ``quant_dtype=None`` the norm alone, and ``normed`` (allocated if it is ``None``) is returned.
 
     ``x``, ``residual``, ``residual_out`` and ``normed`` are ``[rows, dim]`` of one type (fp32 / bf16 / fp16), each with dense rows any distance apart (a slice of the
-    columns of a wider tensor will do); ``weight`` ``[dim]`` has that type or fp32.  ``residual_out`` may be ``residual`` or ``x``, ``normed`` may be ``x``.  ``rows`` may be
+    columns of a wider tensor will do); ``weight`` ``[dim]`` has that type or fp32.  ``residual_out`` may be ``residual`` or ``x``, ``normed`` may be ``x``, but not both the same.  ``rows`` may be
     0, and ``dim`` anything up to 2^24.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
     the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
     # a call with its outputs, on the current device, goes on in native code, which looks at the operands

@@ -464,8 +464,8 @@ int psg_moe_softmax_sorting(const psg_moe_gating_args *gating, const psg_moe_sor
  *   to nearest even), from y before its rounding to fp32
  * The squares of h, their sum and h * weight may be beyond fp32 or below its smallest number where y is not: such rows are taken again, scaled by powers of two.
  * x, residual, residual_out and normed are rows of dim elements, a stride of elements (0 = dim, and at least dim) apart, at addresses and strides that need only be
- * multiples of an element; q [rows, dim] is dense, scale [rows].  residual_out may be residual or x, normed may be x: every element is read before it is
- * written.  Other overlaps are not allowed.
+ * multiples of an element; q [rows, dim] is dense, scale [rows].  residual_out may be residual or x, normed may be x (not both x: normed at the address of
+ * residual_out is refused): every element is read before it is written.  Other overlaps are not allowed.
  * x_dtype 0 = fp32, 1 = bf16, 2 = fp16 (the numbering of the quantisers); weight_dtype x_dtype or 0; out_dtype PSG_IN_INT8, PSG_IN_FP8_E4M3FN or -1: no q and scale
  * (normed is then required).  rows = 0 launches nothing.  dim <= 2^24, eps >= 0.
  */

@@ -51,3 +51,10 @@ def test_host_tensors_and_wrong_arguments_are_refused():
         quant_device.rmsnorm_quant(x.double(), w)
     with pytest.raises(TypeError, match="fp32, bf16 or fp16"):
         quant_device.rmsnorm_quant(None, w, out=out, stream=7)
+
+
+def test_both_16_bit_outputs_in_one_place_are_refused():
+    handle = _lib.lib()
+    for change in (dict(residual=0x2000, residual_out=0x1000, normed=0x1000), dict(residual=0x2000, residual_out=0x2000, normed=0x2000), dict(residual=0x2000, residual_out=0x3000, normed=0x3000, out_dtype=-1)):
+        assert handle.psg_rmsnorm_quant(ctypes.byref(_args(**change)), None) == SHAPE
+        assert b"lost" in handle.psg_last_error()
