@@ -5,6 +5,7 @@ without leaving the GPU.  torch is used for the output allocations only."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -112,6 +113,14 @@ def _norm_row_stride(name, t, x):
     return t.stride(0) if t.shape[0] > 1 else 0
 
 
+def _allocating_for(stream, device):
+    """Outputs of a launch on ``stream`` come from that stream's memory: a block of the current stream's may still be in use by what is queued there."""
+    handle = _lib.stream_on(stream, device)
+    if handle == torch.cuda.current_stream(device).cuda_stream:
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device))
+
+
 def _norm_args(x, weight, eps, quant_dtype):
     """The argument struct of a call, without its addresses and strides."""
     if quant_dtype is not None and quant_dtype not in _OUT_CODE:
@@ -158,7 +167,8 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     ``x``, ``residual``, ``residual_out`` and ``normed`` are ``[rows, dim]`` of one type (fp32 / bf16 / fp16), each with dense rows any distance apart (a slice of the
     columns of a wider tensor will do); ``weight`` ``[dim]`` has that type or fp32.  ``residual_out`` may be ``residual`` or ``x``, ``normed`` may be ``x``, but not both the same.  ``rows`` may be
     0, and ``dim`` anything up to 2^24.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
-    the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``."""
+    the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``; without ``out`` the outputs are allocated for that stream, as torch
+    allocates what is made with it as the current one."""
     # a call with its outputs, on the current device, goes on in native code, which looks at the operands
     if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and type(weight) in _TENSORS and quant_dtype is not None and (residual is not None or residual_out is None) and type(eps) in _NUMBERS:
         q, scale = out
@@ -193,9 +203,11 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
         if out is not None:
             raise ValueError("out is given with quant_dtype=None: the result is normed")
         if normed is None:
-            normed = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
+            with _allocating_for(stream, x.device):
+                normed = torch.empty((rows, dim), dtype=x.dtype, device=x.device)
     elif out is None:
-        q, scale = torch.empty((rows, dim), dtype=quant_dtype, device=x.device), torch.empty((rows, 1), dtype=torch.float32, device=x.device)
+        with _allocating_for(stream, x.device):
+            q, scale = torch.empty((rows, dim), dtype=quant_dtype, device=x.device), torch.empty((rows, 1), dtype=torch.float32, device=x.device)
     else:
         q, scale = out
         _check_out(x, q, scale)

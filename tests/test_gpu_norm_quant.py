@@ -344,3 +344,19 @@ def test_eps_that_is_no_python_number():
             eps[...] = value
             q, s = quant_device.rmsnorm_quant(x, w, eps, stream=torch.cuda.current_stream(), out=out)
             _check(x, w, None, value, FP8, q, s, None, None)
+
+
+def test_outputs_are_allocated_for_the_stream_of_the_launch():
+    x, w, _ = _inputs(2048, 2048, torch.bfloat16, False, 8)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    made = {0: torch.cuda.default_stream().cuda_stream, side: side.cuda_stream, side.cuda_stream: side.cuda_stream, None: torch.cuda.current_stream().cuda_stream}
+    for stream, handle in made.items():
+        q, s = quant_device.rmsnorm_quant(x, w, stream=stream)
+        y = quant_device.rmsnorm_quant(x, w, quant_dtype=None, stream=stream)
+        torch.cuda.synchronize()
+        _check(x, w, None, 1e-6, FP8, q, s, None, y)
+        segments = torch.cuda.memory_snapshot()
+        for t in (q, s, y):
+            at = [g["stream"] for g in segments if g["address"] <= t.data_ptr() < g["address"] + g["total_size"]]
+            assert at == [handle]
