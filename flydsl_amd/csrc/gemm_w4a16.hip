@@ -47,6 +47,38 @@ __device__ __forceinline__ v4f mfma16(v4i w, v4i a, v4f c) {
 template <int N>
 __device__ __forceinline__ int of_lane(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x150 + N, 0xF, 0xF, true); }
 
+// Row `row` of A times the four columns of W from n on, by all lanes of a wavefront: fp32 products with (q - z) s, which is exact (4 bits and a sign times 11), lanes eight elements of K each in turn.
+template <bool BF16, int GS, bool ZP>
+__device__ __forceinline__ v4f plain_sums(const W4Params& p, uint64_t row, int n, int steps, int groups, int lane) {
+    constexpr int OUT = BF16 ? OUT_BF16 : OUT_FP16;
+    const uint16_t* const a = static_cast<const uint16_t*>(p.a) + row * (uint64_t)p.K;
+    v4f d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int c = lane; c < p.K / 8; c += 64) {
+        const v4i a8 = *reinterpret_cast<const v4i*>(a + (size_t)c * 8);
+        const uint64_t g = (uint64_t)(n >> 4) * (uint64_t)groups + (uint64_t)(c * 8 / GS);
+        // block, lane group and dword of these eight elements
+        const uint8_t* const w = p.w + ((uint64_t)(n >> 4) * (uint64_t)steps + (uint64_t)(c >> 4)) * 1024u + (uint32_t)((c & 3) * 256 + ((c >> 2) & 3) * 4);
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const int r = (n & 15) + v;
+            const uint32_t q8 = *reinterpret_cast<const uint32_t*>(w + r * 16);
+            const float s = from_out16<OUT>(p.scales[g * 16 + r]);
+            const int z = ZP ? p.zeros[g * 8 + (r >> 1)] >> (4 * (r & 1)) & 15 : 8;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int q = (int)(q8 >> (e & 1 ? 14 + 2 * e : 2 * e)) & 15;
+                d[v] = __builtin_fmaf(from_out16<OUT>((uint16_t)((uint32_t)a8[e >> 1] >> (16 * (e & 1)))), (float)(q - z) * s, d[v]);
+            }
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+        for (int v = 0; v < 4; v++) d[v] += __shfl_xor(d[v], off, 64);
+    return d;
+}
+
 constexpr int W4_WAVES = 8, W4_LDS = 160 * 1024;
 
 // MB: 16-row blocks of A.  GS: elements of a group.  ZP: zero points.  SPW: 128-element steps of a wavefront's part of A.  SH: those that come through LDS at a time.  MANY: several
@@ -214,11 +246,25 @@ __global__ void __launch_bounds__(W4_WAVES * 64, 2) k_w4a16(W4Params p) {
     // the slices' sums, in their order
     for (int t = tid; t < windows * MB * 64; t += NW * 64) {
         const int frag = t >> 6, m = (frag % MB) * 16 + li, n = n_begin + (frag / MB) * 16 + lg * 4;
-        if (n >= n_end || m >= M) continue;
+        const bool live = n < n_end && m < M;
         v4f sum = all[t];
 #pragma unroll
         for (int j = 1; j < NW; j++) sum += all[j * apart + t];
-        store_c4(p, (size_t)(m0 + m) * (size_t)p.N + (size_t)n, n, sum);
+        const size_t at = (size_t)(m0 + m) * (size_t)p.N + (size_t)n;
+        if (live) store_c4(p, at, n, sum);
+        // Sums that are not finite (all of a wavefront is here): P and 16 X meet as infinities where A has one, or where a group of finite rows passes fp32 by the 16 alone.  Such
+        // values are taken and stored once more as the definition has them, the sum of A ((q - z) s), lanes along K: 16x28672x8192 25 us, with an infinity in one row 79, in all 780.  (Asking
+        // costs 0.1 us a launch: 1x2048x2048 3.33 / 3.43, 16x28672x8192 level; in front of the stores 0.17.)
+        const float mags = (fabsf(sum[0]) + fabsf(sum[1])) + (fabsf(sum[2]) + fabsf(sum[3]));
+        for (uint64_t bad = __ballot(live && !(mags < __builtin_inff())); __builtin_expect(bad != 0, 0); bad &= bad - 1) {
+            const int l = __builtin_ctzll(bad);
+            const v4f d = plain_sums<BF16, GS, ZP>(p, (uint64_t)(m0 + __builtin_amdgcn_readlane(m, l)), __builtin_amdgcn_readlane(n, l), steps, groups, lane);
+            if (lane == l) {
+#pragma unroll
+                for (int v = 0; v < 4; v++) sum[v] = fabsf(sum[v]) < __builtin_inff() ? sum[v] : d[v];
+                store_c4(p, at, n, sum);
+            }
+        }
     }
 }
 

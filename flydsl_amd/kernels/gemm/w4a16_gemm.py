@@ -8,8 +8,8 @@
 ``shuffle_group_scales`` and ``shuffle_group_zeros``, laid out once (``flydsl_amd.quant.pergroup_w4_quant`` makes the codes); without zero points a code counts from 8 and
 ``zeros`` is ``None``.
 
-A row of ``A`` with an infinity, or with bf16 values of which 31 times the sum over a group passes the fp32 range, gives NaN in its row of ``C`` (the sums of ``16 + code`` and of 16 are
-subtracted); other rows are as without it.
+Infinities and NaN of ``A`` go where the sum of ``A * (scale * (code - zero))`` in fp32 has them, rows beside them are as without; such values are taken one at a time, so a batch full of
+them is slow.
 
 It is made for decode: the weights are read once for every 32 rows, whatever ``M``.
 """

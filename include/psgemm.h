@@ -492,6 +492,7 @@ int psg_rmsnorm_quant(const psg_rmsnorm_args *args, void *stream);
 
 /*
  * Products of a few rows with 4-bit weights: C[m,n] = sum_k A[m,k] s[n, k/group] (q[n,k] - z[n, k/group]) (+ bias, activation), sums in fp32.
+ * Infinities, NaN and sums beyond fp32 are those of the terms A ((q - z) s).
  *   a [M,K], c [M,N], bias [N] and the scales share one 16-bit type, dtype = enum psg_out_dtype (bf16 or fp16); q 0..15; z 0..15 from zeros, or 8 with zeros NULL.
  *   w: blocks of 16 rows x 128 elements [N/16][ceil(K/128)][4 g][16 r][16 bytes], dword j of the 16 bytes the elements 32 j + 8 g + i of row r, i = 0..7: even i in bits
  *   [2 i, 2 i + 4), odd i in bits [16 + 2 (i - 1), + 4); what elements past K hold does not matter.  scales [N/16][K/group][16]; zeros [N/16][K/group][8 bytes], column

@@ -175,3 +175,31 @@ def test_refusals():
             fn(*{**good, "A": b(4 * 256 + 4)[4:]}.values(), 4, stream)
         with pytest.raises(ValueError, match="outside"):
             fn(*good.values(), 0, stream)
+
+
+@pytest.mark.parametrize("m,n,k,group,zero_points,dtype", [(6, 528, 1024, 128, False, "bf16"), (6, 272, 2080, 32, True, "fp16"), (20, 1040, 2560, 64, False, "bf16"), (31, 528, 4096, 128, True, "bf16"), (9, 2064, 9216, 128, True, "bf16"),
+                                                         (22, 1040, 6144, 32, False, "fp16"), (40, 272, 5120, 64, True, "bf16")])
+def test_infinities_and_sums_beyond_fp32(m, n, k, group, zero_points, dtype):
+    """An infinity in a row of A is one in the columns whose weight of it is not zero; finite rows have finite products, also where a group's sum of 16 + code is beyond fp32.  Rows beside them are what
+    they are without."""
+    dt = DT[dtype]
+    codes, scale, zero = _weights(n, k, group, dt, zero_points, m + n, True)
+    a = torch.randint(-8, 9, (m, k), generator=torch.Generator().manual_seed(m)).to(dt)
+    inf = float("inf")
+    a[0, 7], a[1, k - 1] = inf, -inf
+    a[3, 5], a[3, k // 2] = inf, inf
+    a[m - 1, 0], a[m - 1, 33] = inf, -inf
+    if dtype == "bf16":
+        a[4] = 0
+        a[4, 1:4], a[4, k - 2] = 2.0**124, -(2.0**124)  # times up to 31 beyond 2^128, times (q - z) s at most 2^124 4 15 / 16
+    got = _run(a, codes, scale, zero, None, group, dtype, "none")
+    w = _deq(codes, scale, zero, group)
+    rows = [i for i in range(m) if torch.isfinite(a[i]).all()]
+    want = torch.empty(m, n, dtype=torch.float64)
+    want[rows] = a[rows].double() @ w.t()
+    for i in set(range(m)) - set(rows):  # (the library's product may take an infinity times zero out of a sum)
+        want[i] = (a[i].double() * w)[:, ~torch.isfinite(a[i])].sum(1)
+    want = want.float().to(dt)
+    assert torch.isfinite(want[rows]).all() and torch.isinf(want[[0, 1]]).any() and torch.isnan(want[m - 1]).any()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))
