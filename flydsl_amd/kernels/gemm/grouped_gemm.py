@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -24,6 +25,10 @@ from ... import _lib
 
 _IN = {"fp8": (1, torch.float8_e4m3fn), "int8": (1, torch.int8), "fp16": (2, torch.float16), "bf16": (2, torch.bfloat16)}
 _OUT = {"bf16": (torch.bfloat16, _lib.TYPE_BF16), "fp16": (torch.float16, _lib.TYPE_FP16)}
+
+
+class _Forced(threading.local):
+    tile_rows = 0  # rows of a tile; 0: the library's choice (another for tests)
 
 
 class GroupedGemm:
@@ -34,7 +39,15 @@ class GroupedGemm:
         self._eb, self._scaled = _IN[in_dtype][0], _IN[in_dtype][0] == 1
         self._lib = _lib.lib()
         self._plans = {}  # (argument struct without its addresses, operands) by M
-        self.tile_rows = 0  # rows of a tile; 0: the library's choice (another for tests)
+        self._forced = _Forced()  # (one launcher serves all callers of its sizes: what a thread forces is its own)
+
+    @property
+    def tile_rows(self):
+        return self._forced.tile_rows
+
+    @tile_rows.setter
+    def tile_rows(self, rows):
+        self._forced.tile_rows = rows
 
     def _args(self, M):
         if M < 1 or M > 1 << 22:
@@ -56,7 +69,7 @@ class GroupedGemm:
     def __call__(self, C, A, B, scale_a, scale_b, offsets, M, stream=None):
         """Launch on ``stream`` (``None``: the current stream of the device of ``C``).  ``scale_a`` and ``scale_b`` are only read for 8-bit operands."""
         if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and _lib.is_current(C.get_device()):
-            key = (M, self.tile_rows)
+            key = (M, self._forced.tile_rows)
             plan = self._plans.get(key)
             if plan is None:
                 if len(self._plans) >= 256:

@@ -55,3 +55,27 @@ def test_host_tensors_are_refused():
             fn(None, *good[1:], 10, stream)
         with pytest.raises(ValueError, match="outside"):
             fn(*good, 0, stream)
+
+
+def test_tile_rows_are_those_of_the_thread_that_set_them():
+    """The launcher is one for all callers of its sizes; what a thread forces is its own, also in the plans that are kept."""
+    import threading
+
+    fn = compile_grouped_gemm(N=64, K=192, groups=4)
+    fn.tile_rows = 32
+    try:
+        seen = []
+
+        def other():
+            seen.append(fn.tile_rows)
+            seen.append(fn._args(10).tile_rows)
+            fn.tile_rows = 64
+            seen.append(fn._args(10).tile_rows)
+
+        t = threading.Thread(target=other)
+        t.start()
+        t.join()
+        assert seen == [0, 0, 64] and fn.tile_rows == 32 and fn._args(10).tile_rows == 32
+    finally:
+        fn.tile_rows = 0
+    assert fn._args(10).tile_rows == 0
