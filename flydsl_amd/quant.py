@@ -182,7 +182,8 @@ def pergroup_w4_quant(w: torch.Tensor, group_size: int = 128, zero_points: bool 
     [N, K/group] scale_dtype, zeros [N, K/group] uint8 or None)``; a code stands for ``scale * (code - zero)``, with ``zero = 8`` without zero points.
 
     With zero points the group's range, extended to hold 0, is spread over the 16 codes; without, its largest magnitude is 7.5 steps (half a step is clipped at the
-    positive end).  The scale is rounded to ``scale_dtype`` before the codes are made; a group of zeros has scale 1.  ``w`` must be finite."""
+    positive end).  The scale is rounded to ``scale_dtype`` before the codes are made; a group of zeros has scale 1.  ``w`` must be finite, and so the scales in
+    ``scale_dtype`` (ValueError otherwise)."""
     n, k = w.shape
     if k % group_size:
         raise ValueError(f"K={k} must be a multiple of group_size={group_size}")
@@ -192,6 +193,8 @@ def pergroup_w4_quant(w: torch.Tensor, group_size: int = 128, zero_points: bool 
         scale = ((hi - lo) / 15).to(scale_dtype)
     else:
         scale = (v.abs().amax(-1, keepdim=True) / 7.5).to(scale_dtype)
+    if not torch.isfinite(scale).all():
+        raise ValueError(f"w must be finite, and its groups' scales numbers of {scale_dtype}")
     scale = torch.where(scale == 0, torch.ones_like(scale), scale)
     zero = torch.round(-lo / scale.float()).clamp(0, 15) if zero_points else torch.full_like(scale, 8, dtype=torch.float32)
     codes = (torch.round(v / scale.float()) + zero).clamp(0, 15).to(torch.uint8).reshape(n, k)

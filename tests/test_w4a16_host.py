@@ -114,3 +114,19 @@ def test_host_tensors_are_refused():
         fn(None, b(1, 256), None, None, None, None, 1)
     with pytest.raises(ValueError, match="outside"):
         fn(None, None, None, None, None, None, 0)
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_quantiser_refuses_scales_that_are_none(zero_points):
+    """A group whose scale is beyond the type of the scales would stand for NaN."""
+    w = torch.ones(16, 128)
+    w[5, 7] = -8e5  # over 7.5 steps; with zero points the next row, over 15: beyond 65504
+    w[6, 7] = 8e5 if zero_points else 0.0
+    w[6, 8] = -8e5 if zero_points else 0.0
+    with pytest.raises(ValueError, match="float16"):
+        quant.pergroup_w4_quant(w, 64, zero_points, torch.float16)
+    codes, scale, zero = quant.pergroup_w4_quant(w, 64, zero_points, torch.bfloat16)
+    assert torch.isfinite(scale).all()
+    w[1, 1] = float("inf")
+    with pytest.raises(ValueError, match="finite"):
+        quant.pergroup_w4_quant(w, 64, zero_points)
