@@ -177,11 +177,12 @@ hipError_t launch(const A8W8Params& p, GroupParams g, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// Whether W goes past the caches: where most groups are one tile, so that nothing is read twice, and two such products, as a layer has them at least, have more weights than the last-level
-// cache (256 MB).  us through the caches / past them: 64 rows on 32 experts, 3584 x 4096, fp8 75.0 / 69.8 (6.3 TB/s), 512 79.3 / 75.3, bf16 256 on 64, 2048 x 2048 96 / 87; but
-// two tiles a group, 512 rows in tiles of 16, 85 / 92, and weights that the cache holds, 16 rows on 8, 2048 x 4096 13.8 / 15.0.
+// Whether W goes past the caches: where most groups are one tile, so that little is read twice, and two such products, as a layer has them at least, have more weights than the last-level
+// cache (256 MB).  us through the caches / past them, fp8, 3584 x 4096 on 32 experts, by the rows that a group has for every row of its tile: tiles of 16, 1/2 83.8 / 77.8, 3/4 85.1 / 84.2, 1 90.3 / 96.2,
+// 3/2 101 / 124; of 32, 1/2 86.2 / 81.1, 3/4 91.8 / 91.3, 1 97.5 / 107; of 64, 1/2 92.0 / 87.2, 3/4 101.4 / 102.0, 1 106 / 118; as many on fewer experts, W of 84 MB 16.6 / 18.3, 112 20.3 / 20.9, 140 27.5 / 27.3,
+// 168 33.6 / 31.4; int8 2048 x 768 on 128, 2048 rows 45.8 / 40.9, 4200 49.9 / 45.5; bf16 2048 x 2048 on 64, 256 rows 99.8 / 91.0, 1100 107.4 / 99.6.
 bool goes_past(const A8W8Params& p, const GroupParams& g, int bm, int bytes) {
-    return 2ll * g.groups * p.N * p.K * bytes > 256ll << 20 && 2ll * p.M <= (int64_t)bm * g.groups;
+    return 2ll * g.groups * p.N * p.K * bytes > 256ll << 20 && 4ll * p.M <= 3ll * bm * g.groups;
 }
 
 template <int KIND>

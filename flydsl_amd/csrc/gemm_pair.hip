@@ -131,9 +131,11 @@ void go(const A8W8Params& p, int store, dim3 grid, hipStream_t stream) {
 // The grouped product on these tiles: bf16 by STORE_C, fp16 by STORE_C_GENERIC
 hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream) {
     g.most = (int)group_tiles_most(p.M, g.groups, 128);
-    // A C that fills the last-level cache (256 MB) goes past it, in whose place weights and rows of A stay: 32768 rows, 4096 x 1536, fp8 233 / 226 us, with what reads C next 314 / 308.  A smaller one
-    // would be missed by its reader: 1500 x 2816, bf16 28.4 / 25.3, but 30.4 / 32.4 with it.
-    g.past = (uint64_t)p.M * (uint64_t)p.N * 2ull >= 256ull << 20;
+    // C goes past the caches where C, A and the weights are more than five eighths of the last level (256 MB), so that of two such products on end one has put out what the other left: weights and
+    // rows of A stay in C's place.  us through the caches / past them, with what reads C next, by their MB together: bf16 2816 x 1088 on 17, 110 27.3 / 28.0, 143 62.2 / 63.0; fp8 4096 x 1536 on 8, 67 29.8 / 30.3,
+    // on 16, 134 53.5 / 54.1, on 32, 230 79.2 / 72.6, 268 104.7 / 102.8, 420 243 / 234, 496 315 / 301; bf16 4096 x 4096 on 4, 192 147.1 / 145.8, on 8, 512 943 / 938.
+    const int64_t bytes = kind == KIND_INT8 || kind == KIND_FP8 ? 1 : 2, weights = (int64_t)(g.groups < p.M ? g.groups : p.M) * p.N * p.K * bytes;
+    g.past = weights + (int64_t)p.M * p.K * bytes + (int64_t)p.M * p.N * 2 > 160ll << 20;
     const dim3 grid((unsigned)g.most * (unsigned)((p.N + 255) / 256));
 #define PSG_GROUPED(KIND_)                                                                                                                             \
     case KIND_:                                                                                                                                        \
