@@ -4,8 +4,8 @@
 //
 // with z = 16 + zero point (24 without zero points: codes 0..15 stand for -8..7).  A code q is made an operand of the matrix cores by two instructions for two of them: shifted to
 // the upper bits of a mantissa, masked and joined with the exponent of 16 it is the 16-bit number 16 + q exactly, in bf16 as in fp16.  The 16 and the zero point come off the group's sum
-// in fp32, and X of a lane's own row is what the same MFMA gives for a weight of ones.  (P is at most 31/16 of the sum with the 16 alone: the difference loses four or five of 24
-// bits, far below the 16-bit output's rounding.)
+// in fp32, and X of a lane's own row is what the same MFMA gives for a weight of ones.  (Both parts are at most 31 times the group's sum of |A|, of which an fp32 addition loses 2^-24; the terms
+// A (q - z) are at most 8 times it, 15 with zero points: the 16 costs up to two bits, far below the 16-bit output's rounding but where terms of both signs cancel.)
 //
 // Bound: the weights' way from memory, and at a few MB of them the 3 us that a launch takes whatever it reads.  The columns are dealt out in units of 8, evenly, over one workgroup a CU;
 // its eight wavefronts are eight slices of K.  A wavefront's part of A (SPW steps of 128 elements of the 16 rows) stays in registers while the workgroup's columns go by in windows of 16,

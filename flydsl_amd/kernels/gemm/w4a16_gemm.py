@@ -11,7 +11,7 @@
 Infinities and NaN of ``A`` go where the sum of ``A * (scale * (code - zero))`` in fp32 has them, rows beside them are as without; such values are taken one at a time, so a batch full of
 them is slow.
 
-It is made for decode: the weights are read once for every 32 rows, whatever ``M``.
+It is made for decode: the weights are read once for every 32 rows, or for every 16 where ``N`` and ``K`` are large (more than 96 columns a compute unit on rows too long for one pass).
 """
 
 from __future__ import annotations

@@ -497,7 +497,8 @@ int psg_rmsnorm_quant(const psg_rmsnorm_args *args, void *stream);
  *   w: blocks of 16 rows x 128 elements [N/16][ceil(K/128)][4 g][16 r][16 bytes], dword j of the 16 bytes the elements 32 j + 8 g + i of row r, i = 0..7: even i in bits
  *   [2 i, 2 i + 4), odd i in bits [16 + 2 (i - 1), + 4); what elements past K hold does not matter.  scales [N/16][K/group][16]; zeros [N/16][K/group][8 bytes], column
  *   r of the 16 in byte r / 2, even r in the low nibble.
- * group 32, 64 or 128, K a multiple of it, N of 16, 1 <= M <= 65536; the weights are read once for every 32 rows.  N * ceil(K/128) * 64 and M * K * 2 bytes below 4 GiB;
+ * group 32, 64 or 128, K a multiple of it, N of 16, 1 <= M <= 65536; the weights are read once for every 32 rows, or for every 16 where N and K are large (more than 96 columns a CU on rows too
+ * long for one pass).  N * ceil(K/128) * 64 and M * K * 2 bytes below 4 GiB;
  * a and w 16-byte, c, bias and scales 8-byte, zeros 2-byte aligned.
  */
 typedef struct psg_w4a16_args {
