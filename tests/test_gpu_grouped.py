@@ -238,3 +238,48 @@ def test_refusals():
                 fn(*{**good, name: bad}.values(), 4, stream)
         with pytest.raises(ValueError, match="outside"):
             fn(*good.values(), 0, stream)
+
+
+def _exact_on_the_device(rows, n, k, groups, dtype, out, sizes, tile_rows):
+    """Whole numbers as in _operands, made and compared on the device; rows behind the last group stay as they were."""
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    top = 8 if dtype == "int8" else 4
+    a, w = (torch.randint(-top, top + 1, s, generator=g, device="cuda", dtype=torch.int8).to(DT[dtype]) for s in ((rows, k), (groups, n, k)))
+    sa = sb = None
+    if dtype in ("fp8", "int8"):
+        sa, sb = (torch.exp2(-torch.randint(0, 4, s, generator=g, device="cuda").float()) for s in ((rows,), (groups, n)))
+    offsets = _offsets(sizes)
+    c = torch.full((rows, n), GUARD, dtype=DT[out], device="cuda")
+    fn = compile_grouped_gemm(N=n, K=k, groups=groups, in_dtype=dtype, out_dtype=out)
+    laid = torch.stack([_shuffled(x) for x in w])
+    print(f"grouped M={rows} N={n} K={k} groups={groups} {dtype} {out} tile {tile_rows}", flush=True)
+    fn.tile_rows = tile_rows
+    try:
+        fn(c, a, laid, sa, sb, torch.tensor(offsets, dtype=torch.int32).cuda(), rows, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+    finally:
+        fn.tile_rows = 0
+    for e in range(groups):
+        for at in range(offsets[e], offsets[e + 1], 2048):
+            r = slice(at, min(at + 2048, offsets[e + 1]))
+            want = a[r].double() @ w[e].double().t().contiguous()
+            if sa is not None:
+                want = want * sa[r, None].double() * sb[e].double()
+            assert torch.equal(c[r], want.float().to(DT[out]))
+    assert (c[offsets[-1] :] == GUARD).all()
+
+
+@pytest.mark.parametrize("dtype,out,n,k", [("fp8", "bf16", 4112, 4096), ("int8", "fp16", 4112, 4160), ("bf16", "bf16", 2064, 4128), ("fp16", "fp16", 2064, 4096)])
+@pytest.mark.parametrize("tile_rows", [16, 32, 64])
+def test_weights_past_the_caches(tile_rows, dtype, out, n, k):
+    """Eight weights of 135 MB together, rows for three quarters of a tile each: the builds that read W past the caches."""
+    rows = tile_rows * 6
+    sizes = [tile_rows, 1, 0, tile_rows - 1, tile_rows + 2, 5, 0]
+    sizes.append(rows - 3 - sum(sizes))
+    _exact_on_the_device(rows, n, k, 8, dtype, out, sizes, tile_rows)
+
+
+@pytest.mark.parametrize("dtype,out", [("fp8", "bf16"), ("fp8", "fp16"), ("int8", "bf16"), ("int8", "fp16"), ("bf16", "bf16"), ("bf16", "fp16"), ("fp16", "bf16"), ("fp16", "fp16")])
+def test_outputs_past_the_caches(dtype, out):
+    """C of 176 MB, in ragged tiles of 128 rows and columns that end inside one."""
+    _exact_on_the_device(22000, 4112, 192 if dtype in ("fp8", "int8") else 96, 5, dtype, out, [7000, 0, 129, 8255, 6600], 128)

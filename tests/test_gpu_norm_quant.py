@@ -360,3 +360,19 @@ def test_outputs_are_allocated_for_the_stream_of_the_launch():
         for t in (q, s, y):
             at = [g["stream"] for g in segments if g["address"] <= t.data_ptr() < g["address"] + g["total_size"]]
             assert at == [handle]
+
+
+@pytest.mark.parametrize("dt,wt", [(torch.float32, None), (torch.bfloat16, None), (torch.bfloat16, torch.float32), (torch.float16, None), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("rows,dim", [(3, 12296), (2, 16384), (1100, 4099), (1030, 9001), (3, 16392), (2, 20001), (2, 32768), (4, 9001), (3, 12281)])
+def test_long_rows_of_every_build(rows, dim, dt, wt):
+    """Four vectors a thread on up to 512 threads (4097 elements and more, by rows and ends), on 576 to 1024, and two on up to 768 with a row's end."""
+    for residual, qd in ((True, FP8), (False, torch.int8)):
+        x, w, r = _inputs(rows, dim, dt, residual, seed=dim, wt=wt)
+        wide = torch.full((rows, dim + 3), 7.0, dtype=dt, device="cuda")  # (rows off 16 bytes, and something behind them)
+        v = wide[:, :dim]
+        v.copy_(x)
+        keep, out = None if r is None else r.clone(), (torch.empty(rows, dim, dtype=qd, device="cuda"), torch.empty(rows, 1, device="cuda"))
+        print(f"norm rows={rows} dim={dim} {dt} {wt}", flush=True)
+        q, s = quant_device.rmsnorm_quant(v, w, 1e-6, residual=r, quant_dtype=qd, normed=v, stream=torch.cuda.current_stream(), out=out)
+        _check(x, w, keep, 1e-6, qd, q, s, r, v)
+        assert (wide[:, dim:] == 7).all()

@@ -203,3 +203,26 @@ def test_infinities_and_sums_beyond_fp32(m, n, k, group, zero_points, dtype):
     assert torch.isfinite(want[rows]).all() and torch.isinf(want[[0, 1]]).any() and torch.isnan(want[m - 1]).any()
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(got.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))
+
+
+# one size for every build of the kernel that the sizes above do not take: three steps of up to 24 rows, passes of two steps of up to 24 rows, of three and of two steps of 16
+BUILDS = [(24, 2048, 2560, 128, False), (20, 8720, 5248, 128, True), (17, 8208, 5184, 64, False), (16, 4112, 9216, 128, True), (9, 1040, 9152, 64, False), (3, 33024, 8320, 128, False), (16, 32784, 8320, 128, True),
+          (5, 33040, 7232, 64, False), (1, 32784, 7232, 64, True)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k,group,zero_points", BUILDS)
+def test_exact_sums_of_the_other_builds(m, n, k, group, zero_points, dtype):
+    dt = DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8, device="cuda")
+    scale = torch.exp2(-torch.randint(4, 7, (n, k // group), generator=g, device="cuda").float()).to(dt)
+    zero = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8, device="cuda") if zero_points else None
+    a = torch.randint(-8, 9, (m, k), generator=g, device="cuda").to(dt)
+    got = _run(a, codes, scale, zero, None, group, dtype, "none")
+    for n0 in range(0, n, 4096):  # (8 bytes a weight here)
+        c = slice(n0, n0 + 4096)
+        z = torch.full_like(scale[c], 8.0, dtype=torch.float64) if zero is None else zero[c].double()
+        w = (codes[c].double() - z.repeat_interleave(group, 1)) * scale[c].double().repeat_interleave(group, 1)
+        want = (a.double() @ w.t().contiguous()).float()
+        assert torch.equal(got[:, c], want.to(dt).cpu())
