@@ -283,3 +283,11 @@ def test_weights_past_the_caches(tile_rows, dtype, out, n, k):
 def test_outputs_past_the_caches(dtype, out):
     """C of 176 MB, in ragged tiles of 128 rows and columns that end inside one."""
     _exact_on_the_device(22000, 4112, 192 if dtype in ("fp8", "int8") else 96, 5, dtype, out, [7000, 0, 129, 8255, 6600], 128)
+
+
+@pytest.mark.parametrize("tile_rows", [0, 16, 32, 64, 128])
+def test_groups_in_front_of_offsets_that_go_back(tile_rows):
+    n, k = 272, 128
+    a, w, sa, sb = _operands(90, n, k, 4, "fp8", 5)
+    for offsets, sound in [([0, 30, 10, 10, 5], [0, 30, 30, 30, 30]), ([3, 20, 61, 7, 7], [3, 20, 61, 61, 61]), ([-4, 90, 80, 70, 0], [0, 90, 90, 90, 90])]:
+        _check_exact(_run(a, w, sa, sb, offsets, "fp8", "bf16", tile_rows), a, w, sa, sb, sound, "bf16")
