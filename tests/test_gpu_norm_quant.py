@@ -376,3 +376,11 @@ def test_long_rows_of_every_build(rows, dim, dt, wt):
         q, s = quant_device.rmsnorm_quant(v, w, 1e-6, residual=r, quant_dtype=qd, normed=v, stream=torch.cuda.current_stream(), out=out)
         _check(x, w, keep, 1e-6, qd, q, s, r, v)
         assert (wide[:, dim:] == 7).all()
+
+
+@pytest.mark.parametrize("dim", [515, 40011])
+def test_residual_that_is_x(dim):
+    x, w, _ = _inputs(5, dim, torch.bfloat16, False, seed=9)
+    a, normed = x.clone(), torch.empty_like(x)
+    q, s = quant_device.rmsnorm_quant(a, w, residual=a, normed=normed)
+    _check(x, w, x, 1e-6, FP8, q, s, a, normed)
