@@ -10,9 +10,9 @@
 // the maximum leave a row together, with one barrier, and the row stays in registers as h w in between.  The rms cancels in q = h w dmax / max|h w|, which is taken
 // like this, to fp32 with one rounding: q is the definition's but where that rounding meets a border, and the row's maximum is dmax exactly.
 // A row whose squares are beyond fp32 or below it (h from about 2^58 on; below 2^-50 with an eps below 2^-60) is read a second and a third time, scaled by powers of two.
-// Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves: 8192 rows of 8192, bf16 to fp8 with a residual, 470 MB in 80.6 us (5.8 TB/s),
-// with the 16-bit rows 604 MB in 104 (5.8); 256 rows 5.0; one row 3.5.  Rows that begin off 16 bytes cost nothing (8192
-// of 2048, 2048 to 2056 elements apart, 26.3 to 28.5 us), off four bytes some, and so does an end that is no whole vector: 2048 24.7, 2056 27.8, 2050 30.4, 2047 30.3, 2049 35.5.
+// Bound: HBM, every operand read once and every output written once, behind 2.9 us that a launch takes whatever it moves.  us, bf16 to fp8 with a residual, launches on end over three sets of
+// operands: 8192 rows of 8192 82.7 (470 MB, 5.7 TB/s), 256 of 4096 4.4, 67 of 8192 4.7, one of 4096 3.9.  Rows that begin off 16 bytes cost nothing (8192 of 2048, 2048 to 2056 elements apart,
+// 26.3 to 28.5), off four bytes some, and so does an end that is no whole vector: 8192 of 2048 25.0, 2056 29.3, 2046 28.4, 2050 30.8, 2047 31.0, 2049 35.3.
 #include "psg_common.h"
 #include "quant_rows.h"
 #include "norm_quant.h"
@@ -26,7 +26,8 @@ typedef int int_any __attribute__((aligned(1)));
 typedef uint16_t half_any __attribute__((aligned(1)));
 
 // Elements [i, i + 8) as they are stored.  Of a row's end, n < 8 of them, its last eight are read: line_up() moves them into their places once every load is on its way (a branch for
-// each element, with a wait of its own, took as long as the rest of the row: 8192 rows of 2047 45.6 us, of 2041 30.8, like this 27.6 and 27.4).  The others among the eight, which their own
+// each element, with a wait of its own, took as long as the rest of the row: 8192 rows of 2047 38.2 us, of 2050 37.9, of 2041 30.7, like this, all else as it
+// was then, 29.9, 33.5 and 28.7; but fp32, 2049 47.1 / 52.1).  The others among the eight, which their own
 // thread may be writing, are dropped.  Rows of less than eight are read by elements.
 template <int XT, bool WHOLE>
 __device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n, int dim) {
@@ -126,7 +127,8 @@ __device__ __forceinline__ float times_over(float v, float d, float m, float rm)
     return __builtin_copysignf(q, v);
 }
 
-// A row belongs to a workgroup of up to MOST threads.  (Four rows a workgroup, one to a wavefront, without the barrier, were level: 8192 rows of 280 6.9 / 7.3 us, of 512 9.2 / 8.1.)  The first KEEP 8-element vectors of every thread stay in registers; a
+// A row belongs to a workgroup of up to MOST threads.  (Rows of up to 256 vectors as four to a workgroup, one to a wavefront, without
+// the barrier, took / take like this, 8192 of them, us: 280 6.9 / 7.3, 512 9.2 / 8.1, 1024 14.2 / 12.3, 2048 25.5 / 25.0, but with ends 2041 28.7 / 30.9, 2047 29.9 / 31.1, 2049 40.0 / 35.3.)  The first KEEP 8-element vectors of every thread stay in registers; a
 // longer row writes its h, or has it in x, and reads the rest of it once more, every thread what it has written itself.
 // WHOLE: rows are whole vectors.  WT: type of the weight.
 template <int XT, int WT, int MOST, int KEEP, bool WHOLE>
@@ -415,7 +417,7 @@ hipError_t launch(const NormParams& p, hipStream_t stream) {
 
 // x_dtype: 0 fp32, 1 bf16, 2 fp16.  Requires rows, dim >= 1 and addresses that are multiples of their elements.
 hipError_t psg_launch_rmsnorm_quant(const NormParams& p, int x_dtype, hipStream_t stream) {
-    // (what WHOLE spares is the code for the end of a row: 8192 rows of 2048 28.5 / 29.9 us)
+    // (what WHOLE spares is the code for the end of a row: 8192 rows of 2048 25.0 / 27.3 us, in fp32 44.0 / 49.4, of 8192 82.8 / 88.4)
     const bool whole = p.dim % 8 == 0;
 #define PSG_NORM_T(XT_, WT_) return whole ? launch<XT_, WT_, true>(p, stream) : launch<XT_, WT_, false>(p, stream);
     switch (x_dtype) {
