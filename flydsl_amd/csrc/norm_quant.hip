@@ -400,13 +400,14 @@ hipError_t launch(const NormParams& p, hipStream_t stream) {
     const int nvec = (p.dim + 7) / 8;
     const int64_t cus = psg_cu_count();
 #define PSG_NORM(MOST_, KEEP_) return launch_rows<XT, WT, MOST_, KEEP_, WHOLE>(p, (nvec + KEEP_ * 64 - 1) / (KEEP_ * 64) * 64, stream);
-    // Vectors of a thread; as many wavefronts as the row then fills (all sixteen of 1024 threads where nine have work: 8192 rows of 9042 169 us / 111).  us, bf16 to fp8 with a residual, one vector / two / four:
-    // few and short rows want their loads at once, 4 rows of 1204 3.3 / 3.9 / 4.5, 777 of 2051 5.9 / 6.4 / 7.5, 300 of 3401 5.1 / 5.3 / 6.4 (of 3584, without an end, level); of many rows a CU holds more that way, 8192 of 2048 26.8 / 24.5 / 25.1, of 2880 40.7 / 33.4 / 33.5, of
-    // 5120 70 / 54.6 / 54.2; with the code for a row's end 8192 of 5124 82 / 66 / 59, but 300 5.8 / 6.1 / 6.6.
+    // Vectors of a thread; as many wavefronts as the row then fills (all sixteen of 1024 threads where nine have work: 8192 rows of 9042 169 us / 111).  us, bf16 to fp8 with a residual.
+    // One vector or two, few or short rows, which want their loads at once: 4 rows of 1204 3.3 / 3.9, 777 of 2051 5.9 / 6.4, 300 of 3401 5.1 / 5.3 (of 3584, without an end, level); of many rows a CU
+    // holds more with two, 8192 of 2048 27.4 / 25.2, of 2880 40.7 / 33.4, of 5120 70 / 54.6.
     if (nvec <= 64 || (nvec <= (WHOLE ? 320 : 512) && p.rows * nvec <= 1024 * cus)) PSG_NORM(512, 1)
+    // Two or four: 4 of 1204 3.9 / 4.5, 300 of 3401 5.3 / 6.4, 8192 of 2048 25.2 / 25.3, of 5120 54.6 / 54.2; but with the code for a row's end 8192 of 5124 66 / 59, 300 6.1 / 6.6.
     if (nvec <= 512 || (nvec <= 1024 && (WHOLE || p.rows <= 4 * cus))) PSG_NORM(512, 2)
-    // Longer ones two / four: 4 of 9042 4.7 / 5.5, 1100 of 12288 20.9 / 22.8, 8192 122 / 125, but with the code for a row's end 8192 of 9715 147 / 136, and 13 to 15 wavefronts leave room for no second
-    // workgroup beside them, 8192 of 14336 157 / 143.
+    // The same on up to 768 threads: 4 of 9042 4.7 / 5.5, 1100 of 12288 20.9 / 22.8, 8192 122 / 125; but with ends 8192 of 9715 147 / 136, and 13 to 15 wavefronts leave room for no second workgroup
+    // beside them, 8192 of 14336 157 / 143.
     if (nvec > 1024 && nvec <= 1536 && (WHOLE || p.rows <= 4 * cus)) PSG_NORM(1024, 2)
     if (nvec <= 2048) PSG_NORM(512, 4)
     return launch_rows<XT, WT, 1024, 4, WHOLE>(p, nvec > 4096 ? 1024 : (nvec + 255) / 256 * 64, stream);  // (beyond 32768 elements threads come back for the rest)

@@ -98,7 +98,6 @@ def per_1x32_f4_quant(x: torch.Tensor, shuffle: bool = True, stream=None, out=No
 
 
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
-_NUMBERS = (float, int)  # (what equal values stand for equal plans: a tensor is found by its identity, whatever it holds now)
 _norm_plans = {}  # what shapes and types alone decide about a call of rmsnorm_quant, by them
 
 
@@ -169,8 +168,8 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     0, and ``dim`` anything up to 2^24.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]`` and fp32 ``[rows]`` / ``[rows, 1]``): no allocation, so
     the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``; without ``out`` the outputs are allocated for that stream, as torch
     allocates what is made with it as the current one."""
-    # a call with its outputs, on the current device, goes on in native code, which looks at the operands
-    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and type(weight) in _TENSORS and quant_dtype is not None and (residual is not None or residual_out is None) and type(eps) in _NUMBERS:
+    # a call with its outputs, on the current device, goes on in native code, which looks at the operands (eps a number: a tensor would be found by its identity, whatever it holds now)
+    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and type(weight) in _TENSORS and quant_dtype is not None and (residual is not None or residual_out is None) and isinstance(eps, (float, int)):
         q, scale = out
         h = residual if residual_out is None else residual_out
         if type(q) is type(scale) is torch.Tensor and x.is_cuda and _lib.is_current(x.get_device()):
