@@ -72,6 +72,9 @@ EXPORTS = (
     "psg_rmsnorm_quant",
     "psg_gemm_w4a16",
     "psg_gemm_grouped",
+    "psg_quant_block",
+    "psg_gemm_blockscale",
+    "psg_moe_grouped_topk_gating",
 )
 
 
@@ -290,6 +293,58 @@ class GroupedArgs(ctypes.Structure):
     ]
 
 
+class QuantBlockArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("scale_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32),
+        ("gated", ctypes.c_int32),
+        ("pad0", ctypes.c_int32),
+    ]
+
+
+class BlockscaleArgs(ctypes.Structure):
+    _fields_ = [
+        ("c", ctypes.c_void_p),
+        ("a", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("scale_a", ctypes.c_void_p),
+        ("scale_a_stride", ctypes.c_int64),
+        ("scale_b", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("M", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("tile_rows", ctypes.c_int32),
+    ]
+
+
+class MoeGroupedGatingArgs(ctypes.Structure):
+    _fields_ = [
+        ("gating", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("indices", ctypes.c_void_p),
+        ("tokens", ctypes.c_int32),
+        ("experts", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scores", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("topk_groups", ctypes.c_int32),
+        ("group_score", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _lib = None
 
 
@@ -336,7 +391,7 @@ def lib() -> ctypes.CDLL:
     handle.psg_moe_softmax_sorting_fused.restype = ctypes.c_int
     handle.psg_moe_softmax_sorting_fused.argtypes = [ctypes.c_int32] * 3
     for name in ("psg_gemm_a8w8", "psg_gemm_mxfp4", "psg_gemm_a8w8_static", "psg_moe_gemm", "psg_moe_mx_gemm", "psg_moe_sorting", "psg_moe_topk_gating",
-                 "psg_rmsnorm_quant", "psg_gemm_w4a16", "psg_gemm_grouped"):
+                 "psg_rmsnorm_quant", "psg_gemm_w4a16", "psg_gemm_grouped", "psg_quant_block", "psg_gemm_blockscale", "psg_moe_grouped_topk_gating"):
         fn = getattr(handle, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
@@ -561,3 +616,18 @@ def check_operand(name, t, *, min_elems, elem_sizes, device=None):
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the output is on {device}")
     return t.device
+
+
+def block_stride(name, t, blocks, rows, device) -> int:
+    """Floats from a block's scales to the next block's (0: dense) of ``t``, fp32 ``[blocks, rows]`` on ``device`` with dense rows that do not overlap."""
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a device (cuda) tensor, got {getattr(t, 'device', type(t).__name__)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands are on {device}")
+    if t.dtype != torch.float32 or t.shape != (blocks, rows):
+        raise ValueError(f"{name} must be fp32 [{blocks}, {rows}], got {t.dtype} {list(t.shape)}")
+    if (rows > 1 and t.stride(1) != 1) or (blocks > 1 and t.stride(0) < rows):
+        raise ValueError(f"{name} must have dense rows that do not overlap (strides {tuple(t.stride())})")
+    return t.stride(0) if blocks > 1 else 0

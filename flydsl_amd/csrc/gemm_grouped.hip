@@ -17,16 +17,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
     constexpr int BM = 16 * MR, CB = 4 / KS, TN = 16 * CB * NR, SETS = 4;  // (CB: column blocks side by side)
     constexpr int TILE = BM * TK;                                          // bytes of A a step; a stage holds KS of them
     constexpr int A_LOADS = (KS * BM * 8 + 255) / 256;                     // 16-byte pieces of a stage a thread
-    constexpr bool SCALED = KIND == KIND_INT8 || KIND == KIND_FP8;
+    constexpr bool SCALED = KIND == KIND_INT8 || KIND == KIND_FP8, BLOCKED = KIND == KIND_FP8B;
     constexpr int ROWB = TN * 2, GR = ROWB / 16;                           // bytes and 16-byte granules of a row of the tile of C
     constexpr int SUMS = KS > 1 ? 4 * MR * NR * 1024 : 0;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * KS * TILE > SUMS ? 2 * KS * TILE : SUMS];
+    __shared__ float s_scale[BLOCKED ? 2 * KS * BM : 1];  // a stage's products of row and column scale
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int slice = KS > 1 ? wave : 0, block = KS > 1 ? 0 : wave;
     GroupTile t;
-    if (!group_tile(g, p.M, BM, (int)blockIdx.x, (p.N + TN - 1) / TN, lane, t)) return;
+    if (!group_tile<BLOCKED>(g, p.M, BM, (int)blockIdx.x, (p.N + TN - 1) / TN, lane, t)) return;
     const int n0 = t.n_tile * TN;
-    const uint32_t K = SCALED ? (uint32_t)p.K : (uint32_t)p.K * 2u;  // bytes of a row
+    const uint32_t K = SCALED || BLOCKED ? (uint32_t)p.K : (uint32_t)p.K * 2u;  // bytes of a row
     const int KT = (int)((K + KS * TK - 1) / (KS * TK));
 
     // rows past the group's end and columns past N lie behind the descriptors' bounds or are redirected there, and read as zero
@@ -47,6 +48,25 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
         a_lds[j] = sub < KS ? sub * TILE + lds_off(row, kc) : -1;
     }
     v4i ar[SETS][A_LOADS], wlo[SETS][NR], whi[SETS][NR];
+    // block scales of a stage: a row of a slice a thread, and that of the tile's columns, which lie in one block (rows past the group's end have others' scales, and zeros behind the array)
+    static_assert(KS * BM <= 64, "the scales of a stage are a wavefront's");
+    float sar[SETS], sbr[SETS];
+    const uint32_t sa_off = ((uint32_t)(tid / BM) * g.sa_stride + (uint32_t)(tid % BM)) * 4u;
+    const uint32_t KB = (K + TK - 1) / TK, NB = ((uint32_t)p.N + 127u) / 128u;
+    const __amdgpu_buffer_rsrc_t rsa = make_rsrc(BLOCKED ? p.sa + t.row : nullptr, BLOCKED ? ((uint64_t)(KB - 1) * g.sa_stride + (uint32_t)(p.M - t.row)) * 4ull : 0ull);
+    const __amdgpu_buffer_rsrc_t rsb = make_rsrc(BLOCKED ? p.sb + ((uint64_t)t.e * NB + (uint32_t)n0 / 128u) * KB : nullptr, BLOCKED ? KB * 4ull : 0ull);
+    auto load_s = [&](int kt, int set) __attribute__((always_inline)) {
+        if constexpr (BLOCKED) {
+            const bool has = tid < KS * BM && (uint32_t)kt * KS + (uint32_t)(tid / BM) < KB;
+            sar[set] = __int_as_float(buf_load4(rsa, has ? sa_off : OOB, kt < KT ? (uint32_t)kt * (KS * 4u) * g.sa_stride : 0u));
+            sbr[set] = __int_as_float(buf_load4(rsb, has ? (uint32_t)(tid / BM) * 4u : OOB, kt < KT ? (uint32_t)kt * (KS * 4u) : 0u));
+        }
+    };
+    auto store_s = [&](int stage, int set) __attribute__((always_inline)) {
+        if constexpr (BLOCKED) {
+            if (tid < KS * BM) s_scale[stage * KS * BM + tid] = sar[set] * sbr[set];
+        }
+    };
     __builtin_assume(KT > 0);
     auto load_a = [&](int kt, int set) __attribute__((always_inline)) {
 #pragma unroll
@@ -75,12 +95,36 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
         constexpr int S = decltype(I)::value & 1, set = decltype(I)::value % SETS;
         load_a(kt + 3, (set + 3) % SETS);
         load_w(kt + 3, (set + 3) % SETS);
+        load_s(kt + 3, (set + 3) % SETS);
         // (addresses in front, MFMAs behind: one that writes a register has two wait states to the vector instruction that wrote it last)
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_nop 1");
         const uint8_t* const mine = lds + (S * KS + slice) * TILE;
+        if constexpr (BLOCKED) {
+            // a step is a block: its products' sums by MFMAs that begin with zero, then times both scales into the sums of the blocks, behind the next MFMA
+            v4f part[2];
+            float s[2];
+            v4i alo[1], ahi[1];
+            static_for<MR * NR + 1>([&](auto I) {
+                constexpr int i = decltype(I)::value, mi = i / NR, ni = i % NR, before = i > 0 ? i - 1 : 0;
+                if constexpr (i < MR * NR) {
+                    if constexpr (ni == 0) {
+                        alo[0] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, lg)), ahi[0] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, 4 + lg));
+                        s[mi & 1] = s_scale[(S * KS + slice) * BM + mi * 16 + li];
+                    }
+                    part[i & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(wlo[set][ni], whi[set][ni], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                                   __builtin_shufflevector(alo[0], ahi[0], 0, 1, 2, 3, 4, 5, 6, 7), (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                }
+                if constexpr (i > 0) {
 #pragma unroll
-        for (int mi = 0; mi < MR; mi++) {
+                    for (int j = 0; j < 4; j++) acc[before / NR][before % NR][j] = __builtin_fmaf(part[before & 1][j], s[before / NR & 1], acc[before / NR][before % NR][j]);
+                    // (here, and not where the sums are used in the end: the compiler takes the additions of four steps behind the last branch and keeps what the MFMAs gave until then)
+                    asm volatile("" : "+v"(acc[before / NR][before % NR]));
+                }
+            });
+        }
+#pragma unroll
+        for (int mi = 0; mi < (BLOCKED ? 0 : MR); mi++) {
             const v4i alo = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, lg)), ahi = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, 4 + lg));
 #pragma unroll
             for (int ni = 0; ni < NR; ni++) {
@@ -101,11 +145,13 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
             }
         }
         store_a(S ^ 1, (set + 1) % SETS);
+        store_s(S ^ 1, (set + 1) % SETS);
         __syncthreads();
     };
 
     static_for<3>([&](auto I) { load_w(decltype(I)::value, decltype(I)::value); });
     static_for<3>([&](auto I) { load_a(decltype(I)::value, decltype(I)::value); });
+    static_for<3>([&](auto I) { load_s(decltype(I)::value, decltype(I)::value); });
     // the scales of the lane's rows and columns, under the loop
     float sa[MR];
     v4f sb[NR];
@@ -119,6 +165,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
         }
     }
     store_a(0, 0);
+    store_s(0, 0);
     __syncthreads();
     int kt = 0;
     for (; kt + SETS <= KT; kt += SETS) static_for<SETS>([&](auto I) { step(kt + decltype(I)::value, I); });
@@ -187,7 +234,7 @@ bool goes_past(const A8W8Params& p, const GroupParams& g, int bm, int bytes) {
 
 template <int KIND>
 hipError_t launch_kind(const A8W8Params& p, const GroupParams& g, GroupedPlan plan, hipStream_t stream) {
-    const bool past = goes_past(p, g, plan.bm, KIND == KIND_INT8 || KIND == KIND_FP8 ? 1 : 2);
+    const bool past = goes_past(p, g, plan.bm, KIND == KIND_INT8 || KIND == KIND_FP8 || KIND == KIND_FP8B ? 1 : 2);
     switch (plan.bm) {
         case 16:
             if (plan.sliced) return launch<KIND, 1, 1, 4, false>(p, g, stream);
@@ -231,6 +278,7 @@ hipError_t psg_launch_grouped(const A8W8Params& p, const GroupParams& g, int kin
     switch (kind) {
         case KIND_INT8: return launch_kind<KIND_INT8>(p, g, plan, stream);
         case KIND_FP8: return launch_kind<KIND_FP8>(p, g, plan, stream);
+        case KIND_FP8B: return launch_kind<KIND_FP8B>(p, g, plan, stream);
         case KIND_FP16: return launch_kind<KIND_FP16>(p, g, plan, stream);
         case KIND_BF16: return launch_kind<KIND_BF16>(p, g, plan, stream);
     }

@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p, GROUPS... groups)
     using acc_t = typename Acc<KIND>::type;
     using P = Pair<KIND>;
     constexpr int MR = P::MR, NR = P::NR, TM = P::TM, TN = P::TN;
-    constexpr bool SCALED = KIND == KIND_INT8 || KIND == KIND_FP8, BIAS = STORE == STORE_C_GENERIC;
+    constexpr bool SCALED = KIND == KIND_INT8 || KIND == KIND_FP8, BLOCKED = KIND == KIND_FP8B, BIAS = STORE == STORE_C_GENERIC;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[P::LDS_BYTES];
     __shared__ float s_a[SCALED ? TM : 1], s_b[SCALED ? TN : 1];
     __shared__ __attribute__((aligned(8))) uint16_t s_bias[BIAS ? TN : 1];
@@ -25,19 +25,32 @@ __global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p, GROUPS... groups)
     const int wave = wave_id();
     const int lane = tid & 63, li = lane & 15, lg = lane >> 4;
     int tm, tn, m0;
+    __amdgpu_buffer_rsrc_t block_scales;
+    uint32_t scale_voff = 0, scale_step = 0;
     if constexpr (sizeof...(GROUPS) == 1) {
         GroupTile t;
-        if (!group_tile((groups, ...), p.M, TM, (int)blockIdx.x, (p.N + TN - 1) / TN, lane, t)) return;
+        if (!group_tile<BLOCKED>((groups, ...), p.M, TM, (int)blockIdx.x, (p.N + TN - 1) / TN, lane, t)) return;
         m0 = t.row, tn = t.n_tile;
+        if constexpr (BLOCKED) {
+            // the scales that this wavefront brings: of 64 rows, or of 128 columns (behind the last block zeros)
+            const uint32_t KB = ((uint32_t)p.K + TK - 1) / TK, NB = ((uint32_t)p.N + 127u) / 128u, nb = (uint32_t)tn * 2u + (uint32_t)(wave - 2);
+            if (wave < 2) {
+                block_scales = make_rsrc_uniform(p.sa + m0, ((uint64_t)(KB - 1) * (groups, ...).sa_stride + (uint32_t)(p.M - m0)) * 4ull);
+                scale_voff = (uint32_t)tid * 4u, scale_step = (groups, ...).sa_stride * 4u;
+            } else {
+                block_scales = make_rsrc_uniform(p.sb + (uint64_t)t.e * NB * KB, (uint64_t)NB * KB * 4ull);
+                scale_voff = nb < NB ? nb * KB * 4u : OOB, scale_step = 4u;
+            }
+        }
         p.M = t.row + t.rows;  // the group's end
-        p.b += (uint64_t)t.e * (uint64_t)p.N * (uint64_t)p.K * (SCALED ? 1u : 2u);
+        p.b += (uint64_t)t.e * (uint64_t)p.N * (uint64_t)p.K * (SCALED || BLOCKED ? 1u : 2u);
         if constexpr (SCALED) p.sb += (uint64_t)t.e * (uint64_t)p.N;
     } else {
         tile_coords((int)blockIdx.x, (p.M + TM - 1) / TM, (p.N + TN - 1) / TN, p.group_m, tm, tn);
         m0 = tm * TM;
     }
     const int n0 = tn * TN;
-    const uint32_t K = SCALED ? (uint32_t)p.K : (uint32_t)p.K * 2u;  // bytes of a row
+    const uint32_t K = SCALED || BLOCKED ? (uint32_t)p.K : (uint32_t)p.K * 2u;  // bytes of a row
     const int steps = (int)((K + TK - 1) / TK), per = STORE == STORE_ACC ? (steps + p.splits - 1) / p.splits : steps;
     uint32_t k0 = STORE == STORE_ACC ? blockIdx.y * (uint32_t)(per * TK) : 0u;
     if (k0 > K) k0 = K;
@@ -63,7 +76,8 @@ __global__ void __launch_bounds__(256, 2) k_pair(A8W8Params p, GROUPS... groups)
     if constexpr (BIAS) s_bias[tid] = p.epi != EPI_NONE ? p.bias[n0 + tid < p.N ? n0 + tid : p.N - 1] : 0;
 
     acc_t acc[MR][NR];
-    pair_loop<KIND>(acc, lds, ra, a_voff, rb, b_voff, (int)kn, wave, lane, b_step, b_half, ra, ra);
+    if constexpr (BLOCKED) pair_loop<KIND>(acc, lds, ra, a_voff, rb, b_voff, (int)kn, wave, lane, b_step, b_half, block_scales, block_scales, scale_voff, 0, 0, scale_step);
+    else pair_loop<KIND>(acc, lds, ra, a_voff, rb, b_voff, (int)kn, wave, lane, b_step, b_half, ra, ra);
 
     if constexpr (STORE == STORE_ACC) {
         static_for<MR>([&](auto MI) {
@@ -134,7 +148,7 @@ hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind,
     // C goes past the caches where C, A and the weights are more than five eighths of the last level (256 MB), so that of two such products on end one has put out what the other left: weights and
     // rows of A stay in C's place.  us through the caches / past them, with what reads C next, by their MB together: bf16 2816 x 1088 on 17, 110 27.3 / 28.0, 143 62.2 / 63.0; fp8 4096 x 1536 on 8, 67 29.8 / 30.3,
     // on 16, 134 53.5 / 54.1, on 32, 230 79.2 / 72.6, 268 104.7 / 102.8, 420 243 / 234, 496 315 / 301; bf16 4096 x 4096 on 4, 192 147.1 / 145.8, on 8, 512 943 / 938.
-    const int64_t bytes = kind == KIND_INT8 || kind == KIND_FP8 ? 1 : 2, weights = (int64_t)(g.groups < p.M ? g.groups : p.M) * p.N * p.K * bytes;
+    const int64_t bytes = kind == KIND_FP16 || kind == KIND_BF16 ? 2 : 1, weights = (int64_t)(g.groups < p.M ? g.groups : p.M) * p.N * p.K * bytes;
     g.past = weights + (int64_t)p.M * p.K * bytes + (int64_t)p.M * p.N * 2 > 160ll << 20;
     const dim3 grid((unsigned)g.most * (unsigned)((p.N + 255) / 256));
 #define PSG_GROUPED(KIND_)                                                                                                                             \
@@ -145,6 +159,7 @@ hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind,
     switch (kind) {
         PSG_GROUPED(KIND_INT8)
         PSG_GROUPED(KIND_FP8)
+        PSG_GROUPED(KIND_FP8B)
         PSG_GROUPED(KIND_FP16)
         PSG_GROUPED(KIND_BF16)
     }

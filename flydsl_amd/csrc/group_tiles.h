@@ -5,10 +5,12 @@
 
 // Groups of rows: group e has rows [offsets[e], offsets[e + 1]) of A and C (clamped to the rows there are; none where the next offset is not above) and weight e.
 struct GroupParams {
-    const int32_t* offsets;  // [groups + 1]
+    const int32_t* offsets;  // [groups + 1]; nullptr: all rows are one group (block-scaled products only)
     int groups;
     int past;  // set by the launcher (128x256 tiles): C goes past the caches
     int most;  // set by the launcher: tiles along M that the grid was made for (offsets that go back may say more)
+    // block-scaled products: A8W8Params::sa is [ceil(K / 128)][M], rows of sa_stride floats; sb [groups][ceil(N / 128)][ceil(K / 128)]
+    uint32_t sa_stride;
 };
 
 // Rows of a tile (16, 32, 64 or 128), and whether K is cut into slices (16 rows only)
@@ -46,7 +48,16 @@ __device__ __forceinline__ int sum_upto(int v) {
 
 // Workgroup `wg` of the launch -> its tile; false for the workgroups that the bound of the grid counts too many.  Every wavefront works it out by itself, a group a lane: no
 // barrier; uniform.  Tiles are walked as in psg_tile_order, eight of them along M at a time, so that an XCD reads a group's weight once.
+template <bool ONE = false>
 __device__ __forceinline__ bool group_tile(const GroupParams& g, int M, int bm, int wg, int n_tiles, int lane, GroupTile& t) {
+    if constexpr (ONE) {
+        if (!g.offsets) {
+            int m;
+            psg_tile_order(wg, g.most, n_tiles, 8, &m, &t.n_tile);
+            t.e = 0, t.row = m * bm, t.rows = M - t.row;
+            return true;
+        }
+    }
     // of group base + lane: first row, rows, and its tiles with those of the lanes in front of it
     auto look = [&](int base, int& row, int& rows, int& upto) __attribute__((always_inline)) {
         const int e = base + lane;

@@ -19,63 +19,6 @@
 
 namespace {
 
-// 16-byte pieces at any address that is a multiple of the element (global accesses of this target need no more)
-typedef v4i v4i_any __attribute__((aligned(2)));  // (fp32 elements are on 4 bytes)
-typedef v2i v2i_any __attribute__((aligned(1)));
-typedef int int_any __attribute__((aligned(1)));
-typedef uint16_t half_any __attribute__((aligned(1)));
-
-// Elements [i, i + 8) as they are stored.  Of a row's end, n < 8 of them, its last eight are read: line_up() moves them into their places once every load is on its way (a branch for
-// each element, with a wait of its own, took as long as the rest of the row: 8192 rows of 2047 38.2 us, of 2050 37.9, of 2041 30.7, like this, all else as it
-// was then, 29.9, 33.5 and 28.7; but fp32, 2049 47.1 / 52.1).  The others among the eight, which their own
-// thread may be writing, are dropped.  Rows of less than eight are read by elements.
-template <int XT, bool WHOLE>
-__device__ __forceinline__ Raw8<XT> load_row(const void* base, int64_t i, int n, int dim) {
-    constexpr int B = XT == X_F32 ? 4 : 2;
-    Raw8<XT> r;
-    if (WHOLE || dim >= 8) {
-        const v4i_any* p = reinterpret_cast<const v4i_any*>(static_cast<const uint8_t*>(base) + (WHOLE || n >= 8 ? i : i + n - 8) * B);
-        r.w[0] = p[0];
-        if constexpr (XT == X_F32) r.w[1] = p[1];
-    } else {
-#pragma unroll
-        for (int k = 0; k < (XT == X_F32 ? 2 : 1); k++) r.w[k] = (v4i){0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < n) {
-                if constexpr (XT == X_F32) r.w[e >> 2][e & 3] = static_cast<const int*>(base)[i + e];
-                else r.w[0][e >> 1] |= (int)((uint32_t)static_cast<const uint16_t*>(base)[i + e] << (16 * (e & 1)));
-            }
-    }
-    return r;
-}
-
-// the last n of the eight elements to the front, zeros behind them
-template <int XT>
-__device__ __forceinline__ void line_up(Raw8<XT>& r, int n) {
-    if constexpr (XT == X_F32) {
-        int v[15];
-#pragma unroll
-        for (int e = 0; e < 15; e++) v[e] = e < 8 ? r.w[e >> 2][e & 3] : 0;
-#pragma unroll
-        for (int k = 4; k > 0; k >>= 1)
-            if ((8 - n) & k) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = e + k < 8 ? v[e + k] : 0;
-            }
-#pragma unroll
-        for (int e = 0; e < 8; e++) r.w[e >> 2][e & 3] = v[e];
-    } else {
-        v4i w = r.w[0];
-        if ((8 - n) & 4) w = (v4i){w[2], w[3], 0, 0};
-        if ((8 - n) & 2) w = (v4i){w[1], w[2], w[3], 0};
-        if ((8 - n) & 1)
-            w = (v4i){(int)__builtin_amdgcn_alignbit((unsigned)w[1], (unsigned)w[0], 16u), (int)__builtin_amdgcn_alignbit((unsigned)w[2], (unsigned)w[1], 16u),
-                      (int)__builtin_amdgcn_alignbit((unsigned)w[3], (unsigned)w[2], 16u), (int)((unsigned)w[3] >> 16)};
-        r.w[0] = w;
-    }
-}
-
 // (a row's end in pieces of 4, 2 and 1)
 template <int XT, bool WHOLE>
 __device__ __forceinline__ void store_row(void* base, int64_t i, int n, const Raw8<XT>& r) {

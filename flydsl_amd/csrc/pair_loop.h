@@ -34,7 +34,7 @@ struct Pair {
     static constexpr int MR = 8, NR = 4, NS = 4;  // 16-row blocks of A, of W a wavefront; LDS stages
     static constexpr int TM = 128, TN = 256;
     static constexpr int STAGE = TM * TK;         // bytes of one A stage
-    static constexpr int SC_SLOT = KIND == KIND_MXFP4 ? 12 * 256 : 0;  // scale dwords of a step
+    static constexpr int SC_SLOT = KIND == KIND_MXFP4 ? 12 * 256 : KIND == KIND_FP8B ? 4 * 256 : 0;  // scale dwords of a step
     static constexpr int LDS_BYTES = NS * (STAGE + SC_SLOT);
     // two workgroups a CU, with `more` bytes each for what a kernel adds
     static constexpr bool fits(int more) { return 2 * (LDS_BYTES + more) <= 160 * 1024; }
@@ -52,6 +52,8 @@ using MxPair = Pair<KIND_MXFP4>;
 //            lane / 16, 16-byte piece lane % 16
 //   chunk0/1 which of the eight W-side chunks belong to the wavefront's blocks 0, 1 and 2, 3
 //   SCB = 4: `rs` the A side, s_voff chunk `wave` of it, 4-byte piece `lane`; `rs_w` the W side, in chunks of chunk_bytes (SCB = 16: any descriptor)
+// fp8 with block scales only: `rs` and s_voff the wavefront's scales of a step, one a lane, chunk_bytes from a step to the next: wavefront 0 and 1 those of the tile's rows, 2 and 3 that of the
+//            first and second 128 columns, the same in every lane
 template <int KIND, int SCB = 16, class ACC>
 __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const __amdgpu_buffer_rsrc_t ra, const uint32_t (&a_voff)[4],
                                           const __amdgpu_buffer_rsrc_t rb, const uint32_t (&b_voff)[4], const int K, const int wave, const int lane,
@@ -59,21 +61,29 @@ __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const 
                                           const uint32_t s_voff = 0, const int chunk0 = 0, const int chunk1 = 0, const uint32_t chunk_bytes = 0) {
     using P = Pair<KIND>;
     constexpr int MR = P::MR, NR = P::NR, NS = P::NS, STAGE = P::STAGE, SC_SLOT = P::SC_SLOT;
-    constexpr bool MX = KIND == KIND_MXFP4, WHOLE = KIND == KIND_FP8;  // WHOLE: an MFMA takes both halves of a step
+    constexpr bool MX = KIND == KIND_MXFP4, BLOCKED = KIND == KIND_FP8B, WHOLE = KIND == KIND_FP8 || BLOCKED;  // WHOLE: an MFMA takes both halves of a step
     const int li = lane & 15, lg = lane >> 4;
     const int KT = (K + TK - 1) / TK, KF = K / TK;  // steps, whole steps
     // 16-byte piece of its row that this lane fetches, by the parity of the block (the rows of a block count from 8 j)
     const int a_kc[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (lane >> 4) ^ 4};
     const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
+    // block scales: where the wavefront's rows and scales go in a stage, in scalar registers that the compiler cannot trace to the thread's number.  (It keeps the address of every stage and
+    // 1 KB block in a vector register through the loop, which has none left for them.)
+    uint32_t a_dst = 0, block_dst = 0;
+    if constexpr (BLOCKED) {
+        a_dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_base + (uint32_t)wave * 4096u)), block_dst = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_base + (uint32_t)(NS * STAGE) + (uint32_t)wave * 256u));
+        asm volatile("" : "+s"(a_dst), "+s"(block_dst));
+    }
     uint8_t* const lds_x = lds + NS * STAGE;
     // (wavefront 3 brings the bytes of wavefront 0 once more: all of them count the same number of DMAs)
     const uint32_t sc_dst = lds_base + (uint32_t)(NS * STAGE) + (uint32_t)(wave == 3 ? 0 : wave) * 1024u;
 
     // DMA j of step kt: 0..3 A, from 4 on scales.  Without CHK the step is known to be before the end
-    constexpr int N_DMA = !MX ? 4 : SCB == 16 ? 5 : 7;
+    constexpr int N_DMA = BLOCKED ? 5 : !MX ? 4 : SCB == 16 ? 5 : 7;
     auto dma = [&](int kt, int stage, int j, auto CHK) __attribute__((always_inline)) {
         const bool has = !decltype(CHK)::value || kt < KT, in = !decltype(CHK)::value || kt * TK + a_kc[j & 1] * 16 < K;
-        if (j < 4) dma16(ra, lds_base + (uint32_t)(stage * STAGE + (wave * 4 + j) * 1024), in ? a_voff[j < 4 ? j : 0] : OOB, has ? (uint32_t)kt * TK : 0u);
+        if (j < 4) dma16(ra, BLOCKED ? a_dst + (uint32_t)(stage * STAGE + j * 1024) : lds_base + (uint32_t)(stage * STAGE + (wave * 4 + j) * 1024), in ? a_voff[j < 4 ? j : 0] : OOB, has ? (uint32_t)kt * TK : 0u);
+        else if (BLOCKED) dma4(rs, block_dst + (uint32_t)(stage * SC_SLOT), has ? s_voff : OOB, has ? (uint32_t)kt * chunk_bytes : 0u);
         else if (SCB == 16) dma16(rs, sc_dst + (uint32_t)(stage * SC_SLOT), has ? s_voff : OOB, has ? (uint32_t)kt * 256u : 0u);
         else if (j == 4) dma4(rs, lds_base + (uint32_t)(NS * STAGE + stage * SC_SLOT + wave * 256), has ? s_voff : OOB, has ? (uint32_t)kt * 256u : 0u);
         else {
@@ -93,6 +103,18 @@ __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const 
     auto read_frag = [&](int stage, int half, int mi, v4i& dst) __attribute__((always_inline)) {
         dst = *reinterpret_cast<const v4i*>(&lds[stage * STAGE + mi * 16 * TK + f_base[half]]);
     };
+    // fp8 with block scales: the sums of a block, the lane's row scale of two m-blocks and their products with the column scale
+    v4f part[2] = {};
+    float row_scale[2], column_scale[2], scale[2] = {};
+    // (behind 64 KB an LDS instruction's own offset does not reach: with the addresses as constants every one of them takes a register through the loop)
+    int rows_at = NS * STAGE + li * 4, columns_at = NS * STAGE + 512 + (wave >> 1) * 256 + lane * 4;
+    if constexpr (BLOCKED) asm volatile("" : "+v"(rows_at), "+v"(columns_at));
+    auto read_row_scale = [&](int stage, int mi, float& dst) __attribute__((always_inline)) {
+        dst = *reinterpret_cast<const float*>(lds + rows_at + stage * SC_SLOT + mi * 64);
+    };
+    auto read_column_scale = [&](int stage, float& dst) __attribute__((always_inline)) {
+        dst = *reinterpret_cast<const float*>(lds + columns_at + stage * SC_SLOT);
+    };
     int sav[2][4], sbv[2][2];
     auto read_sc = [&](int slot, int q, int set) __attribute__((always_inline)) {
         if (q < 4) sav[set][q < 4 ? q : 0] = *reinterpret_cast<const int*>(lds_x + slot * SC_SLOT + q * 256 + lane * 4);
@@ -109,14 +131,25 @@ __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const 
                 constexpr int at = decltype(NI)::value, ni = mi & 1 ? NR - 1 - at : at, slot = mi * NR + at;
                 const v8i a = {fr[f][0], fr[f][1], fr[f][2], fr[f][3], fr[f + 1][0], fr[f + 1][1], fr[f + 1][2], fr[f + 1][3]};
                 const v8i b = {bw[B0][ni][0], bw[B0][ni][1], bw[B0][ni][2], bw[B0][ni][3], bw[B0 + 1][ni][0], bw[B0 + 1][ni][1], bw[B0 + 1][ni][2], bw[B0 + 1][ni][3]};
-                if constexpr (WHOLE) mfma_f8(acc[mi][ni], b, a);
+                if constexpr (BLOCKED) part[slot & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                else if constexpr (WHOLE) mfma_f8(acc[mi][ni], b, a);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (at < 2) {
                     if constexpr (mi + 1 < MR) read_frag(S, at, mi + 1, fr[fn + at]);
                     else read_frag((S + 1) % NS, at, 0, fr[fn + at]);
                 }
-                if constexpr (slot >= 3 && slot < 7) dma(kt + 3, (S + 3) % NS, slot - 3, CHK);
-                if constexpr (slot >= 7 && slot < 15) load_w(kt + 1, slot & 1, (slot - 7) / 2, bw[B1 + (slot & 1)], CHK);
+                if constexpr (BLOCKED) {
+                    if constexpr (at == 0) scale[mi & 1] = row_scale[mi & 1] * column_scale[S & 1];
+                    if constexpr (at == 1) read_row_scale(mi + 1 < MR ? S : (S + 1) % NS, mi + 1 < MR ? mi + 1 : 0, row_scale[(mi + 1) & 1]);
+                    if constexpr (at == 2 && mi + 1 == MR) read_column_scale((S + 1) % NS, column_scale[(S + 1) & 1]);
+                    // the block's sums of the MFMA in front of this one
+                    constexpr int last = slot == 0 ? MR * NR - 1 : slot - 1, lm = last / NR, ln = lm & 1 ? NR - 1 - last % NR : last % NR;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[lm][ln][i] = __builtin_fmaf(part[last & 1][i], scale[lm & 1], acc[lm][ln][i]);
+                }
+                constexpr int W0 = 3 + N_DMA;
+                if constexpr (slot >= 3 && slot < W0) dma(kt + 3, (S + 3) % NS, slot - 3, CHK);
+                if constexpr (slot >= W0 && slot < W0 + 8) load_w(kt + 1, (slot - W0 + 1) & 1, (slot - W0) / 2, bw[B1 + ((slot - W0 + 1) & 1)], CHK);
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
@@ -197,6 +230,10 @@ __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const 
     if constexpr (WHOLE) {
         read_frag(0, 0, 0, fr[0]);
         read_frag(0, 1, 0, fr[1]);
+        if constexpr (BLOCKED) {
+            read_row_scale(0, 0, row_scale[0]);
+            read_column_scale(0, column_scale[0]);
+        }
     } else {
         static_for<AHEAD>([&](auto I) { read_frag(0, 0, decltype(I)::value, fr[decltype(I)::value]); });
     }
@@ -213,6 +250,10 @@ __device__ __forceinline__ void pair_loop(ACC (&acc)[8][4], uint8_t* lds, const 
     static_for<NS - 1>([&](auto I) {
         if (kt + decltype(I)::value < KT) step(kt + decltype(I)::value, I, std::true_type{});
     });
+    if constexpr (BLOCKED) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[MR - 1][0][i] = __builtin_fmaf(part[1][i], scale[1], acc[MR - 1][0][i]);
+    }
     // wait states between the last MFMA and the first ordinary read of an accumulator (the compiler does not know that the asm statements are
     // MFMAs); every DMA still on its way (redirected past the bounds) is done before the stages are reused
     asm volatile("s_nop 15\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");

@@ -14,6 +14,8 @@
 #include "gemm_w4a16.h"
 #include "group_tiles.h"
 #include "norm_quant.h"
+#include "quant_block.h"
+#include "moe_route.h"
 #include "tile_order.h"
 
 hipError_t psg_launch_a8w8_tiled(const A8W8Params& p, int kind, int store, int tile_m, int tile_n, hipStream_t stream);
@@ -1413,6 +1415,88 @@ int psg_gemm_grouped(const psg_grouped_args* a, void* stream) {
     const GroupParams g = {a->offsets, a->groups, 0, 0};
     const hipError_t e = psg_launch_grouped(p, g, a->in_dtype, plan, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "psg_gemm_grouped launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_quant_block(const psg_quant_block_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (a->x_dtype < 0 || a->x_dtype > 2) return fail(PSG_E_DTYPE, "x_dtype %d unknown (0 fp32, 1 bf16, 2 fp16)", a->x_dtype);
+    if (a->gated != 0 && a->gated != 1) return fail(PSG_E_SHAPE, "gated must be 0 or 1, got %d", a->gated);
+    if (a->rows < 0 || a->rows > 0x7FFFFFFF) return fail(PSG_E_SHAPE, "rows=%lld outside [0, 2^31)", (long long)a->rows);
+    if (a->dim < 1 || a->dim > (1 << 24)) return fail(PSG_E_SHAPE, "dim=%d outside [1, 2^24]", a->dim);
+    const int64_t cols = (int64_t)a->dim << a->gated, xs = a->x_stride ? a->x_stride : cols, ss = a->scale_stride ? a->scale_stride : a->rows;
+    if (xs < cols || xs > (1ll << 40)) return fail(PSG_E_SHAPE, "x_stride=%lld is below a row of %lld elements or beyond 2^40", (long long)a->x_stride, (long long)cols);
+    if (ss < a->rows || ss > (1ll << 40)) return fail(PSG_E_SHAPE, "scale_stride=%lld is below rows=%lld or beyond 2^40", (long long)a->scale_stride, (long long)a->rows);
+    if (a->rows == 0) {
+        g_err[0] = 0;
+        return 0;
+    }
+    if (!a->x || !a->q || !a->scale) return fail(PSG_E_NULL, "x, q and scale must be non-NULL");
+    if (!aligned(a->x, a->x_dtype == 0 ? 4 : 2) || !aligned(a->scale, 4)) return fail(PSG_E_ALIGN, "every operand must be aligned to its elements");
+    const QuantBlockParams p = {a->x, static_cast<uint8_t*>(a->q), a->scale, xs, ss, a->rows, a->dim, a->gated};
+    const hipError_t e = psg_launch_quant_block(p, a->x_dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_quant_block launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_gemm_blockscale(const psg_blockscale_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (!a->c || !a->a || !a->w || !a->scale_a || !a->scale_b) return fail(PSG_E_NULL, "c, a, w, scale_a and scale_b must be non-NULL");
+    if (a->out_dtype != PSG_OUT_BF16 && a->out_dtype != PSG_OUT_FP16) return fail(PSG_E_DTYPE, "out_dtype %d unknown", a->out_dtype);
+    if (a->M < 1 || a->M > (1 << 22)) return fail(PSG_E_SHAPE, "M=%d outside [1, 2^22]", a->M);
+    if (a->groups < 1 || a->groups > 4096) return fail(PSG_E_SHAPE, "groups=%d outside [1, 4096]", a->groups);
+    if (!a->offsets && a->groups != 1) return fail(PSG_E_NULL, "offsets must be non-NULL with groups=%d", a->groups);
+    if (a->N < 16 || a->N % 16) return fail(PSG_E_SHAPE, "N=%d must be a positive multiple of 16", a->N);
+    if (a->K < 64 || a->K % 64) return fail(PSG_E_SHAPE, "K=%d must be a positive multiple of 64", a->K);
+    if ((uint64_t)a->N * (uint64_t)a->K >= OOB) return fail(PSG_E_SHAPE, "N*K bytes exceed the 4 GiB descriptor range");
+    if (128ull * (uint64_t)a->K >= OOB || 128ull * (uint64_t)a->N * 2ull >= OOB) return fail(PSG_E_SHAPE, "128 rows of a or c exceed the 4 GiB descriptor range");
+    const int64_t kb = (a->K + 127ll) / 128, ss = a->scale_a_stride ? a->scale_a_stride : a->M;
+    if (ss < a->M) return fail(PSG_E_SHAPE, "scale_a_stride=%lld is below M=%d", (long long)a->scale_a_stride, a->M);
+    if (ss > 0x7FFFFFFF || (uint64_t)kb * (uint64_t)ss * 4ull >= OOB) return fail(PSG_E_SHAPE, "scale_a exceeds the 4 GiB descriptor range");
+    if (a->tile_rows != 0 && a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64 or 128", a->tile_rows);
+    const GroupedPlan plan = a->tile_rows ? GroupedPlan{a->tile_rows, false} : psg_grouped_plan(a->M, a->groups, a->N, a->K);
+    const int tn = plan.sliced ? 16 : plan.bm <= 32 ? 64 : 2 * plan.bm;  // columns of a tile
+    // (256 threads each: a grid holds less than 2^32)
+    if (group_tiles_most(a->M, a->groups, plan.bm) * ((a->N + tn - 1ll) / tn) >= 1ll << 24) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
+    if (!aligned(a->a, 16) || !aligned(a->w, 16) || !aligned(a->c, 16)) return fail(PSG_E_ALIGN, "a, w and c must be 16-byte aligned");
+    if (!aligned(a->scale_a, 4) || !aligned(a->scale_b, 4) || !aligned(a->offsets, 4)) return fail(PSG_E_ALIGN, "scale_a, scale_b and offsets must be 4-byte aligned");
+    A8W8Params p = {};
+    p.c = a->c, p.a = static_cast<const uint8_t*>(a->a), p.b = static_cast<const uint8_t*>(a->w), p.sa = a->scale_a, p.sb = a->scale_b;
+    p.M = a->M, p.N = a->N, p.K = a->K, p.epi = EPI_NONE, p.out = a->out_dtype, p.splits = 1;
+    const GroupParams g = {a->offsets, a->groups, 0, 0, (uint32_t)ss};
+    const hipError_t e = psg_launch_grouped(p, g, KIND_FP8B, plan, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_gemm_blockscale launch");
+    g_err[0] = 0;
+    return 0;
+}
+
+int psg_moe_grouped_topk_gating(const psg_moe_grouped_gating_args* a, void* stream) {
+    if (!a) return fail(PSG_E_NULL, "args is NULL");
+    if (a->dtype < 0 || a->dtype > 2) return fail(PSG_E_DTYPE, "dtype %d unknown (0 fp32, 1 bf16, 2 fp16)", a->dtype);
+    if (a->tokens < 0 || a->tokens >= (1 << 24)) return fail(PSG_E_SHAPE, "tokens=%d outside [0, 2^24)", a->tokens);
+    if (a->experts < 1 || a->experts > GATE_MAX_EXPERTS) return fail(PSG_E_SHAPE, "experts=%d outside [1, %d]", a->experts, GATE_MAX_EXPERTS);
+    if (a->groups < 1 || a->groups > 64 || a->experts % a->groups) return fail(PSG_E_SHAPE, "groups=%d must divide experts=%d and be at most 64", a->groups, a->experts);
+    if (a->topk_groups < 1 || a->topk_groups > a->groups) return fail(PSG_E_SHAPE, "topk_groups=%d outside [1, groups=%d]", a->topk_groups, a->groups);
+    const int open = a->experts / a->groups * a->topk_groups;  // experts of the kept groups
+    if (a->topk < 1 || a->topk > GATE_MAX_TOPK || a->topk > open) return fail(PSG_E_SHAPE, "topk=%d outside [1, min(%d, %d experts of topk_groups)]", a->topk, GATE_MAX_TOPK, open);
+    if (a->scores != 0 && a->scores != 1) return fail(PSG_E_DTYPE, "scores %d unknown (0 sigmoid, 1 softmax)", a->scores);
+    if (a->group_score != 0 && a->group_score != 1) return fail(PSG_E_DTYPE, "group_score %d unknown (0 the best, 1 the sum of the two best)", a->group_score);
+    if (a->group_score == 1 && a->topk_groups < a->groups && a->experts / a->groups < 2) return fail(PSG_E_SHAPE, "groups of one expert have no two best");
+    if (!(std::fabs(a->scale) <= 3.402823466e38f)) return fail(PSG_E_SHAPE, "scale must be finite");
+    if (a->tokens == 0) {
+        g_err[0] = 0;
+        return 0;
+    }
+    if (!a->gating || !a->weights || !a->indices) return fail(PSG_E_NULL, "gating, weights and indices must be non-NULL");
+    if (!aligned(a->gating, a->dtype == 0 ? 4 : 2) || !aligned(a->bias, 4) || !aligned(a->weights, 4) || !aligned(a->indices, 4)) return fail(PSG_E_ALIGN, "every operand must be aligned to its elements");
+    RouteParams p = {};
+    p.gating = a->gating, p.bias = a->bias, p.weights = a->weights, p.indices = a->indices;
+    p.tokens = a->tokens, p.experts = a->experts, p.topk = a->topk, p.softmax = a->scores;
+    p.groups = a->groups, p.topk_groups = a->topk_groups, p.top2 = a->group_score, p.renorm = a->renormalize != 0, p.scale = a->scale;
+    const hipError_t e = psg_launch_moe_route(p, a->dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "psg_moe_grouped_topk_gating launch");
     g_err[0] = 0;
     return 0;
 }

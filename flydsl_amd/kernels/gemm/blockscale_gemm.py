@@ -1,0 +1,148 @@
+"""Products of e4m3 rows and weights with one fp32 scale for every 128 elements along K: of a row on the one side, of 128 rows of the weight on the other.
+
+    fn = compile_blockscale_gemm(N=..., K=..., out_dtype="bf16")
+    fn(C, A, B, scale_a, scale_b, M, stream)
+
+    fn = compile_grouped_blockscale_gemm(N=..., K=..., groups=..., out_dtype="bf16")
+    fn(C, A, B, scale_a, scale_b, offsets, M, stream)
+
+``C[r, n] = sum_b scale_a[b, r] * scale_b[n // 128, b] * (A[r, b] @ B[n, b])`` over the blocks ``b`` of 128 elements of K, the last one shorter where K ends inside it.  ``A [M, K]`` and ``C [M, N]``
+row-major; ``B`` ``[N, K]`` in the order of ``flydsl_amd.layout.shuffle_weight``; ``scale_a [ceil(K/128), M]`` fp32, block by block as ``flydsl_amd.quant_device.per_1x128_f8_quant``
+writes them, the blocks any distance apart (the first columns of a wider tensor will do); ``scale_b [ceil(N/128), ceil(K/128)]`` fp32 (``flydsl_amd.quant.per_128x128_f8_quant``).
+
+Grouped, the rows are sorted by group without padding, every group has a weight of its own, ``B [groups, N, K]`` and ``scale_b [groups, ceil(N/128), ceil(K/128)]``, and row ``r`` belongs to
+group ``e`` for ``offsets[e] <= r < offsets[e + 1]``, ``offsets [groups + 1]`` int32 on the device, as in ``compile_grouped_gemm``: groups may be empty, rows of ``C`` outside of
+``[offsets[0], offsets[groups])`` are left as they are, and ``M`` bounds the rows.
+
+A block's products are summed in fp32, its sum is scaled by ``scale_a * scale_b`` (rounded to fp32) and added in fp32.  Nothing is read on the host and no workspace is needed: one launch, which can be
+recorded into a HIP graph.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import threading
+
+import torch
+
+from ... import _lib
+
+_OUT = {"bf16": (torch.bfloat16, _lib.TYPE_BF16), "fp16": (torch.float16, _lib.TYPE_FP16)}
+
+
+class _Forced(threading.local):
+    tile_rows = 0  # rows of a tile; 0: the library's choice (another for tests)
+
+
+class BlockscaleGemm:
+    """Launcher returned by :func:`compile_blockscale_gemm` (``groups`` 0) and :func:`compile_grouped_blockscale_gemm`.  Holds no tensor references."""
+
+    def __init__(self, N, K, groups, out_dtype):
+        self.N, self.K, self.groups, self.out_dtype = N, K, groups, out_dtype
+        self.blocks_n, self.blocks_k = -(-N // 128), -(-K // 128)
+        self._lib = _lib.lib()
+        self._plans = {}  # (argument struct without its addresses, operands) by M
+        self._forced = _Forced()  # (one launcher serves all callers of its sizes: what a thread forces is its own)
+
+    @property
+    def tile_rows(self):
+        return self._forced.tile_rows
+
+    @tile_rows.setter
+    def tile_rows(self, rows):
+        self._forced.tile_rows = rows
+
+    def _args(self, M):
+        if M < 1 or M > 1 << 22:
+            raise ValueError(f"M={M} outside [1, 2^22]")
+        a = _lib.BlockscaleArgs()
+        a.M, a.N, a.K, a.groups = M, self.N, self.K, self.groups or 1
+        a.out_dtype, a.tile_rows = _lib.OUT_DTYPE[self.out_dtype], self.tile_rows
+        return a
+
+    def _plan(self, M):
+        f, any_, n = _lib.BlockscaleArgs, _lib.TYPE_ANY, self.groups or 1
+        ops = [(f.c, 2, _OUT[self.out_dtype][1], 2 * M * self.N), (f.a, 1, any_, M * self.K), (f.w, 1, any_, n * self.N * self.K), (f.scale_a, 4, _lib.TYPE_FP32 + _lib.ROWS, self.blocks_k << 32 | M),
+               (f.scale_b, 4, _lib.TYPE_FP32, 4 * n * self.blocks_n * self.blocks_k)]
+        if self.groups:
+            ops.append((f.offsets, 4, _lib.TYPE_INT32, 4 * (self.groups + 1)))
+        return (bytes(self._args(M)),), _lib.operands(*ops)
+
+    def __call__(self, C, A, B, scale_a, scale_b, *rest, **named):
+        """Launch on ``stream`` (``None``: the current stream of the device of ``C``)."""
+        offsets, M, stream = self._rest(*rest, **named)
+        if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and _lib.is_current(C.get_device()):
+            key = (M, self._forced.tile_rows)
+            plan = self._plans.get(key)
+            if plan is None:
+                if len(self._plans) >= 256:
+                    self._plans.clear()
+                plan = self._plans[key] = self._plan(M)
+            more = (offsets,) if self.groups else ()
+            rc = _lib._native.launch(_lib.address("psg_gemm_blockscale"), plan[0], plan[1], stream, C, A, B, scale_a, scale_b, *more)
+            if rc != _lib._native.DECLINED:
+                if rc:
+                    _lib.check(rc, "psg_gemm_blockscale")
+                return
+        M = int(M)
+        a = self._args(M)
+        n, f8 = self.groups or 1, (1,)
+        operands = [("C", "c", C, M * self.N, (2,), _OUT[self.out_dtype][0]), ("A", "a", A, M * self.K, f8, None), ("B", "w", B, n * self.N * self.K, f8, None),
+                    ("scale_b", "scale_b", scale_b, n * self.blocks_n * self.blocks_k, (4,), torch.float32)]
+        if self.groups:
+            operands.append(("offsets", "offsets", offsets, self.groups + 1, (4,), torch.int32))
+        dev = None
+        for name, field, t, least, sizes, dtype in operands:
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name} must be a device (cuda) tensor, got {type(t).__name__}")
+            dev = dev or t.device
+            _lib.check_operand(name, t, min_elems=least, elem_sizes=sizes, device=dev)
+            if dtype is not None and t.dtype != dtype:
+                raise ValueError(f"{name} is {t.dtype}, this launcher needs {dtype}")
+            setattr(a, field, t.data_ptr())
+        a.scale_a_stride = _lib.block_stride("scale_a", scale_a, self.blocks_k, M, dev)
+        a.scale_a = scale_a.data_ptr()
+        rc = _lib.launch_on(dev, self._lib.psg_gemm_blockscale, ctypes.byref(a), _lib.stream_on(stream, dev))
+        if rc:
+            _lib.check(rc, "psg_gemm_blockscale")
+
+    def _rest(self, M, stream=None):
+        return None, M, stream
+
+
+class GroupedBlockscaleGemm(BlockscaleGemm):
+    """Launcher returned by :func:`compile_grouped_blockscale_gemm`."""
+
+    def _rest(self, offsets, M, stream=None):
+        return offsets, M, stream
+
+
+def _sizes(N, K, out_dtype):
+    if out_dtype not in _OUT:
+        raise ValueError(f"out_dtype must be bf16/fp16, got {out_dtype!r}")
+    N, K = int(N), int(K)
+    if N < 16 or N % 16:
+        raise ValueError(f"N must be a positive multiple of 16 (preshuffled B layout), got {N}")
+    if K < 64 or K % 64:
+        raise ValueError(f"K must be a positive multiple of 64 (preshuffled B layout), got {K}")
+    return N, K
+
+
+def compile_blockscale_gemm(*, N: int, K: int, out_dtype: str = "bf16"):
+    """Build the dense launcher; see the module for its call.  ``out_dtype`` bf16 / fp16, ``N % 16 == 0``, ``K % 64 == 0``."""
+    return _cached_launcher(BlockscaleGemm, *_sizes(N, K, out_dtype), 0, out_dtype)
+
+
+def compile_grouped_blockscale_gemm(*, N: int, K: int, groups: int, out_dtype: str = "bf16"):
+    """Build the launcher for rows sorted by group; see the module for its call.  Sizes as in :func:`compile_blockscale_gemm`, up to 4096 groups."""
+    N, K = _sizes(N, K, out_dtype)
+    groups = int(groups)
+    if not 1 <= groups <= 4096:
+        raise ValueError(f"groups={groups} outside [1, 4096]")
+    return _cached_launcher(GroupedBlockscaleGemm, N, K, groups, out_dtype)
+
+
+@functools.lru_cache(maxsize=256)
+def _cached_launcher(kind, N, K, groups, out_dtype):
+    return kind(N, K, groups, out_dtype)

@@ -199,3 +199,29 @@ def pergroup_w4_quant(w: torch.Tensor, group_size: int = 128, zero_points: bool 
     zero = torch.round(-lo / scale.float()).clamp(0, 15) if zero_points else torch.full_like(scale, 8, dtype=torch.float32)
     codes = (torch.round(v / scale.float()) + zero).clamp(0, 15).to(torch.uint8).reshape(n, k)
     return codes, scale.squeeze(-1).contiguous(), zero.to(torch.uint8).squeeze(-1).contiguous() if zero_points else None
+
+
+def per_1x128_f8_quant(x: torch.Tensor):
+    """e4m3 quantisation of rows ``[M, K]`` with one fp32 scale for every 128 consecutive elements: ``scale = max|block| / 448`` (1 for a block of zeros), ``q = x / scale`` to nearest even.  NaN counts as 0,
+    infinities as +-448.  Returns ``(q [M, K] float8_e4m3fn, scale [ceil(K/128), M] fp32)``: the scales block by block, as the block-scaled products read them."""
+    m, k = x.shape
+    h = torch.nan_to_num(x.float(), nan=0.0, posinf=448.0, neginf=-448.0)
+    v = torch.nn.functional.pad(h, (0, -k % 128)).view(m, -(-k // 128), 128)
+    scale = v.abs().amax(-1, keepdim=True) / 448
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    q = (v / scale).clamp(-448, 448).to(torch.float8_e4m3fn).view(m, -1)[:, :k]
+    return q.contiguous(), scale.squeeze(-1).t().contiguous()
+
+
+def per_128x128_f8_quant(w: torch.Tensor):
+    """e4m3 quantisation of weights ``[..., N, K]`` with one fp32 scale for every 128 x 128 block (shorter where N or K end inside one), by the rule of :func:`per_1x128_f8_quant`.  Returns
+    ``(q [..., N, K] float8_e4m3fn, scale [..., ceil(N/128), ceil(K/128)] fp32)``.  ``w`` must be finite (ValueError otherwise)."""
+    n, k = w.shape[-2:]
+    h = w.float().reshape(-1, n, k)
+    if not torch.isfinite(h).all():
+        raise ValueError("w must be finite")
+    v = torch.nn.functional.pad(h, (0, -k % 128, 0, -n % 128)).view(-1, -(-n // 128), 128, -(-k // 128), 128)
+    scale = v.abs().amax((2, 4), keepdim=True) / 448
+    scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+    q = (v / scale).clamp(-448, 448).to(torch.float8_e4m3fn).view(v.shape[0], v.shape[1] * 128, v.shape[3] * 128)[:, :n, :k]
+    return q.contiguous().view(w.shape), scale.view(*w.shape[:-2], v.shape[1], v.shape[3]).contiguous()

@@ -223,3 +223,79 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resi
     if q is None:
         return normed
     return q if q.dtype == quant_dtype else q.view(quant_dtype), scale if scale.shape == (rows, 1) else scale.view(rows, 1)
+
+
+_block_plans = {}  # what shapes and types alone decide about a call of per_1x128_f8_quant, by them
+
+
+def _block_args(x, gated):
+    """The argument struct of a call, without its addresses and strides."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _X_DTYPE:
+        raise TypeError(f"x must be a tensor of fp32, bf16 or fp16, got {getattr(x, 'dtype', type(x).__name__)}")
+    if not x.is_cuda or x.dim() != 2 or x.shape[1] < 1 + gated:
+        raise ValueError(f"x must be a 2-D device tensor with at least {1 + gated} column(s)")
+    if gated and x.shape[1] % 2:
+        raise ValueError(f"x must have an even number of columns with gated=True, got {x.shape[1]}")
+    a = _lib.QuantBlockArgs()
+    a.dim = x.shape[1] >> gated if x.shape[1] < 1 << 31 else 0
+    if x.shape[0] >= 1 << 31 or not 1 <= a.dim <= 1 << 24:
+        raise ValueError(f"x may have up to 2^31 - 1 rows of up to 2^24 outputs, got {tuple(x.shape)}")
+    a.rows, a.x_dtype, a.gated = x.shape[0], _X_DTYPE[x.dtype], int(gated)
+    return a
+
+
+def _block_plan(x, gated):
+    a = _block_args(x, gated)
+    f, rows, dim = _lib.QuantBlockArgs, a.rows, a.dim
+    typed = {torch.float32: _lib.TYPE_FP32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16}[x.dtype]
+    ops = _lib.operands((f.x, x.element_size(), typed + _lib.ROWS, rows << 32 | x.shape[1]), (f.q, 1, _lib.TYPE_ANY + _lib.EXACT, rows * dim),
+                        (f.scale, 4, _lib.TYPE_FP32 + _lib.ROWS, -(-dim // 128) << 32 | rows))
+    return (bytes(a),), ops
+
+
+def per_1x128_f8_quant(x: torch.Tensor, gated: bool = False, stream=None, out=None):
+    """Rows to e4m3 with one fp32 scale for every 128 columns, what the block-scaled products read (``kernels.gemm.blockscale_gemm``).  Returns ``(q [rows, dim] e4m3fn,
+    scale [ceil(dim/128), rows] fp32)``: the scales block by block.
+
+    ``scale = max|y| / 448`` over a block, 1 where that is 0, ``q = y / scale`` to nearest even; NaN counts as 0 and infinities as +-448, as in :func:`pertoken_quant`.  ``y`` is ``x [rows, dim]``, or
+    with ``gated`` the gated activation ``silu(g) * u`` of ``x = [g, u] [rows, 2 * dim]`` in fp32, not rounded in between: what stands between the two products of an expert.
+
+    ``x`` is fp32 / bf16 / fp16 with dense rows any distance apart, ``dim`` anything up to 2^24, and ``rows`` may be 0.  ``out=(q, scale)`` reuses caller-owned outputs (1-byte ``[rows, dim]``, contiguous, and
+    fp32 ``[ceil(dim/128), rows]`` with blocks any distance apart): no allocation, so the call can be recorded into a HIP graph.  ``stream=None`` is the current stream of the device of ``x``;
+    without ``out`` the outputs are allocated for that stream."""
+    gated = bool(gated)
+    if stream is not None and type(out) is tuple and len(out) == 2 and type(x) is torch.Tensor and x.is_cuda and _lib.is_current(x.get_device()):
+        q, scale = out
+        if type(q) is type(scale) is torch.Tensor:
+            key = (x.shape, x.dtype, gated)
+            plan = _block_plans.get(key)
+            if plan is None:
+                a = _block_plan(x, gated)
+                if len(_block_plans) >= 256:
+                    _block_plans.clear()
+                plan = _block_plans[key] = a
+            rc = _lib._native.launch(_lib.address("psg_quant_block"), plan[0], plan[1], stream, x, q, scale)
+            if rc != _lib._native.DECLINED:
+                if rc:
+                    _lib.check(rc, "psg_quant_block")
+                return q.view(torch.float8_e4m3fn) if q.dtype is not torch.float8_e4m3fn else q, scale
+    a = _block_args(x, gated)
+    rows, dim, blocks = a.rows, a.dim, -(-a.dim // 128)
+    a.x_stride = _norm_row_stride("x", x, x)
+    a.x = x.data_ptr()
+    if out is None:
+        with _allocating_for(stream, x.device):
+            q, scale = torch.empty((rows, dim), dtype=torch.float8_e4m3fn, device=x.device), torch.empty((blocks, rows), dtype=torch.float32, device=x.device)
+    else:
+        q, scale = out
+        if not isinstance(q, torch.Tensor) or not isinstance(scale, torch.Tensor):
+            raise TypeError("out must be (q, scale) tensors")
+        _check_out(x, q)
+        if q.numel() != rows * dim or q.element_size() != 1:
+            raise ValueError("out must be (1-byte [rows, dim], fp32 [ceil(dim/128), rows]) tensors")
+    a.scale_stride = _lib.block_stride("scale", scale, blocks, rows, x.device)
+    a.q, a.scale = q.data_ptr(), scale.data_ptr()
+    rc = _lib.launch_on(x.device, _lib.lib().psg_quant_block, ctypes.byref(a), _lib.stream_on(stream, x.device))
+    if rc:
+        _lib.check(rc, "psg_quant_block")
+    return q if q.dtype == torch.float8_e4m3fn else q.view(torch.float8_e4m3fn), scale

@@ -21,6 +21,8 @@
  *   psg_gemm_mxfp4      kernels/gemm/mxfp4_preshuffle.py:57-488 (launch_gemm / kernel_gemm): fp4/fp6/fp8 A x fp4/fp8 W,
  *                       caller strides, batch over grid.z
  *   psg_gemm_mxfp4_acc  no counterpart: fp32 accumulators of the MXFP4 mainloop, for parity tests
+ *   psg_quant_block, psg_gemm_blockscale, psg_moe_grouped_topk_gating
+ *                       no counterpart: fp8 with an fp32 scale for every block of 128, dense and by expert, and the routing in front of it
  *   psg_rmsnorm_quant, psg_gemm_w4a16, psg_gemm_grouped
  *                       no counterpart of these call shapes: the norm in front of the quantised products, products with 4-bit
  *                       weights and group scales, and ragged products grouped by expert, beside the quantisers, GEMMs and MoE stages
@@ -542,6 +544,86 @@ typedef struct psg_grouped_args {
 } psg_grouped_args;
 
 int psg_gemm_grouped(const psg_grouped_args *args, void *stream);
+
+/*
+ * Rows to e4m3 with one fp32 scale for every 128 columns, what psg_gemm_blockscale reads.
+ *   y = x, or with gated = 1 y = (g * sigmoid(g)) * u of x = [g, u], in fp32 (g the first dim columns of a row, u the dim behind them: the two halves of a gate-up product)
+ *   scale[b, r] = max|y| / 448 over the columns [128 b, 128 b + 128) of row r, the last block shorter where dim ends inside it; 1 where that is 0
+ *   q = y / scale, rounded once, to nearest even.  NaN -> 0 and +-Inf -> +-448 in front of the maximum, as in psg_quant_pertoken
+ * x rows of dim (gated: 2 * dim) elements, x_stride elements apart (0 = dense, else at least a row), at addresses and strides that need only be multiples of an element; q [rows, dim] dense; scale
+ * [ceil(dim / 128)][rows], scale_stride floats from a block to the next (0 = rows, else at least rows).  x_dtype 0 = fp32, 1 = bf16, 2 = fp16.  rows = 0 launches nothing.
+ * dim <= 2^24, rows < 2^31.
+ */
+typedef struct psg_quant_block_args {
+    const void *x;
+    int64_t x_stride;
+    void *q;
+    float *scale;
+    int64_t scale_stride;
+    int64_t rows;
+    int32_t dim;
+    int32_t x_dtype;
+    int32_t gated; /* 0 or 1 */
+    int32_t pad0;  /* 0 */
+} psg_quant_block_args;
+
+int psg_quant_block(const psg_quant_block_args *args, void *stream);
+
+/*
+ * Products of e4m3 operands with one fp32 scale for every 128 elements of a row of A and for every 128 x 128 of a weight:
+ *   C[r,n] = sum over b of scale_a[b, r] * scale_b[e, n / 128, b] * (sum over the k of block b of A[r,k] W[e,n,k])
+ * for all rows (offsets NULL, groups 1), or for offsets[e] <= r < offsets[e+1] with the weights of expert e.
+ *   a [M,K] and c [M,N] row-major, c bf16 or fp16; w [groups][N,K] preshuffled as in psg_gemm_a8w8
+ *   scale_a [ceil(K/128)][M], scale_a_stride floats from a block to the next (0 = M, else at least M); scale_b [groups][ceil(N/128)][ceil(K/128)]
+ *   offsets as in psg_gemm_grouped, with all that is said there about rows outside of the groups
+ * A block's products are summed in fp32, and its sum times scale_a * scale_b, itself rounded to fp32, is added to those of the blocks in front of it with one rounding: the product of two scales
+ * that meet has to be a normal number of fp32 for the result to have its precision.  Within a call every row is summed in the same order; a call of other sizes may take other tiles, and with
+ * few of them four slices of K, whose sums differ in the last places.
+ * tile_rows 0 (the library's choice) or 16, 32, 64, 128.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K % 64 == 0, the bytes of one weight and of scale_a below 4 GiB.
+ * a, w and c 16-byte, the scales and offsets 4-byte aligned.  One launch, no workspace.
+ */
+typedef struct psg_blockscale_args {
+    void *c;
+    const void *a;
+    const void *w;
+    const float *scale_a;
+    int64_t scale_a_stride;
+    const float *scale_b;
+    const int32_t *offsets;
+    int32_t M, N, K;
+    int32_t groups;
+    int32_t out_dtype;
+    int32_t tile_rows;
+} psg_blockscale_args;
+
+int psg_gemm_blockscale(const psg_blockscale_args *args, void *stream);
+
+/*
+ * Routing to experts with a bias and groups of experts:
+ *   s = sigmoid(x) (scores 0) or softmax(x) over the experts (scores 1); c = s + bias (bias NULL: c = s)
+ *   the experts lie in `groups` runs of equal length, a run is worth the sum of its two best c (group_score 1) or its best (0), and the topk_groups best runs are kept
+ *   indices = the topk best c of the kept runs in their order, weights = s of these; renormalize = 1: divided by max(their sum, 1e-20); times scale
+ * Of equal ones the lower index comes first; scores and comparisons are in 64 bits, weights in fp32.  A logit of -Inf or NaN, or a c that is NaN, counts as -Inf: such an expert, like one of a
+ * run that is not kept, is taken (lowest index first) when nothing else is left, with weight 0, so that the indices of a token are always topk different ones.  A run with
+ * one such c among its two best is worth -Inf.
+ * gating [tokens, experts] row-major, dtype 0 = fp32, 1 = bf16, 2 = fp16; bias [experts] fp32; weights [tokens, topk] fp32, indices [tokens, topk] int32.
+ * experts <= 1024, a multiple of groups; groups <= 64; 1 <= topk_groups <= groups; topk <= min(32, topk_groups * experts / groups); tokens < 2^24, 0 launches nothing; scale finite.
+ */
+typedef struct psg_moe_grouped_gating_args {
+    const void *gating;
+    const float *bias;
+    float *weights;
+    int32_t *indices;
+    int32_t tokens, experts, topk;
+    int32_t dtype;
+    int32_t scores;
+    int32_t groups, topk_groups;
+    int32_t group_score;
+    int32_t renormalize;
+    float scale;
+} psg_moe_grouped_gating_args;
+
+int psg_moe_grouped_topk_gating(const psg_moe_grouped_gating_args *args, void *stream);
 
 #ifdef __cplusplus
 }
