@@ -323,6 +323,8 @@ class BlockscaleArgs(ctypes.Structure):
         ("groups", ctypes.c_int32),
         ("out_dtype", ctypes.c_int32),
         ("tile_rows", ctypes.c_int32),
+        ("slice_columns", ctypes.c_int32),
+        ("pad0", ctypes.c_int32),
     ]
 
 

@@ -12,7 +12,7 @@ namespace {
 
 // KS: K slices, 1 or 4: with four, the wavefronts have the same 16 NR columns and every fourth step each.  NT: W past the caches.
 template <int KIND, int MR, int NR, int KS, bool NT>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 2 ? 4 : 3))) k_grouped(A8W8Params p, GroupParams g) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 2 ? 4 : KIND == KIND_FP8B ? 2 : 3))) k_grouped(A8W8Params p, GroupParams g) {
     using acc_t = typename Acc<KIND>::type;
     constexpr int BM = 16 * MR, CB = 4 / KS, TN = 16 * CB * NR, SETS = 4;  // (CB: column blocks side by side)
     constexpr int TILE = BM * TK;                                          // bytes of A a step; a stage holds KS of them
@@ -91,36 +91,38 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
     for (int mi = 0; mi < MR; mi++)
 #pragma unroll
         for (int ni = 0; ni < NR; ni++) acc[mi][ni] = (acc_t){0, 0, 0, 0};
+    // Block scales: what the last BEHIND MFMAs gave, added into the blocks' sums BEHIND MFMAs later, where it is there without a wait (that of a step's last ones in the next step).
+    constexpr int BEHIND = MR * NR < 2 ? MR * NR : 2, SCALES = BEHIND / NR + 1 < MR ? BEHIND / NR + 1 : MR;
+    v4f part[BEHIND] = {};
+    float part_scale[SCALES] = {};
+    auto add_part = [&](auto I) __attribute__((always_inline)) {
+        if constexpr (BLOCKED) {
+            constexpr int i = decltype(I)::value, mi = i / NR, ni = i % NR;
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[mi][ni][j] = __builtin_fmaf(part[i % BEHIND][j], part_scale[mi % SCALES], acc[mi][ni][j]);
+            // (here, and not where the sums are used in the end: the compiler takes the additions of four steps behind the last branch and keeps what the MFMAs gave until then)
+            asm volatile("" : "+v"(acc[mi][ni]));
+        }
+    };
     auto step = [&](int kt, auto I) __attribute__((always_inline)) {
         constexpr int S = decltype(I)::value & 1, set = decltype(I)::value % SETS;
         load_a(kt + 3, (set + 3) % SETS);
+        load_s(kt + 3, (set + 3) % SETS);  // (in front of W, or the wait for the scales would be one for the W that is not due yet)
         load_w(kt + 3, (set + 3) % SETS);
-        load_s(kt + 3, (set + 3) % SETS);
         // (addresses in front, MFMAs behind: one that writes a register has two wait states to the vector instruction that wrote it last)
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_nop 1");
         const uint8_t* const mine = lds + (S * KS + slice) * TILE;
         if constexpr (BLOCKED) {
             // a step is a block: its products' sums by MFMAs that begin with zero, then times both scales into the sums of the blocks, behind the next MFMA
-            v4f part[2];
-            float s[2];
-            v4i alo[1], ahi[1];
-            static_for<MR * NR + 1>([&](auto I) {
-                constexpr int i = decltype(I)::value, mi = i / NR, ni = i % NR, before = i > 0 ? i - 1 : 0;
-                if constexpr (i < MR * NR) {
-                    if constexpr (ni == 0) {
-                        alo[0] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, lg)), ahi[0] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, 4 + lg));
-                        s[mi & 1] = s_scale[(S * KS + slice) * BM + mi * 16 + li];
-                    }
-                    part[i & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(wlo[set][ni], whi[set][ni], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                                                   __builtin_shufflevector(alo[0], ahi[0], 0, 1, 2, 3, 4, 5, 6, 7), (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-                }
-                if constexpr (i > 0) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[before / NR][before % NR][j] = __builtin_fmaf(part[before & 1][j], s[before / NR & 1], acc[before / NR][before % NR][j]);
-                    // (here, and not where the sums are used in the end: the compiler takes the additions of four steps behind the last branch and keeps what the MFMAs gave until then)
-                    asm volatile("" : "+v"(acc[before / NR][before % NR]));
-                }
+            v4i alo[2], ahi[2];
+            static_for<MR * NR>([&](auto I) {
+                constexpr int i = decltype(I)::value, mi = i / NR, ni = i % NR;
+                if constexpr (ni == 0) alo[mi & 1] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, lg)), ahi[mi & 1] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, 4 + lg));
+                add_part(std::integral_constant<int, (i + MR * NR - BEHIND) % (MR * NR)>{});
+                if constexpr (ni == 0) part_scale[mi % SCALES] = s_scale[(S * KS + slice) * BM + mi * 16 + li];
+                part[i % BEHIND] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(wlo[set][ni], whi[set][ni], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                                    __builtin_shufflevector(alo[mi & 1], ahi[mi & 1], 0, 1, 2, 3, 4, 5, 6, 7), (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
             });
         }
 #pragma unroll
@@ -172,6 +174,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
     static_for<SETS - 1>([&](auto I) {
         if (kt + decltype(I)::value < KT) step(kt + decltype(I)::value, I);
     });
+
+    static_for<BEHIND>([&](auto I) { add_part(std::integral_constant<int, MR * NR - BEHIND + decltype(I)::value>{}); });
 
     auto finish = [&](acc_t r, int mi, int ni) __attribute__((always_inline)) {
         v4f x = {(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
@@ -237,7 +241,9 @@ hipError_t launch_kind(const A8W8Params& p, const GroupParams& g, GroupedPlan pl
     const bool past = goes_past(p, g, plan.bm, KIND == KIND_INT8 || KIND == KIND_FP8 || KIND == KIND_FP8B ? 1 : 2);
     switch (plan.bm) {
         case 16:
-            if (plan.sliced) return launch<KIND, 1, 1, 4, false>(p, g, stream);
+            if constexpr (KIND != KIND_FP8B) {  // (whose slices are in gemm_blockscale.hip)
+                if (plan.sliced) return launch<KIND, 1, 1, 4, false>(p, g, stream);
+            }
             return past ? launch<KIND, 1, 1, 1, true>(p, g, stream) : launch<KIND, 1, 1, 1, false>(p, g, stream);
         case 32: return past ? launch<KIND, 2, 1, 1, true>(p, g, stream) : launch<KIND, 2, 1, 1, false>(p, g, stream);
         default: return past ? launch<KIND, 4, 2, 1, true>(p, g, stream) : launch<KIND, 4, 2, 1, false>(p, g, stream);

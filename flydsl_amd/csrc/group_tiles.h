@@ -20,6 +20,15 @@ struct GroupedPlan {
 };
 GroupedPlan psg_grouped_plan(int64_t rows, int groups, int N, int64_t kbytes);
 hipError_t psg_launch_grouped(const A8W8Params& p, const GroupParams& g, int kind, GroupedPlan plan, hipStream_t stream);
+// How a block-scaled product is done: by tiles of bm rows and tn columns, with K in one piece or in slices, or (bm = 1) as a few rows against streamed weights
+struct BlockPlan {
+    int bm, tn;
+    bool sliced;
+};
+BlockPlan psg_block_plan(int64_t rows, int groups, bool dense, int N, int K);
+double psg_blockscale_stream_us(int M, int N, int K);
+hipError_t psg_launch_block_sliced(const A8W8Params& p, const GroupParams& g, int bm, int tn, hipStream_t stream);
+hipError_t psg_launch_blockscale_stream(const A8W8Params& p, const GroupParams& g, hipStream_t stream);
 hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream);
 
 // Upper bound of the tiles of `bm` rows that the rows of `groups` groups make, for the grid: a group's last tile may be almost empty, a group without rows makes none

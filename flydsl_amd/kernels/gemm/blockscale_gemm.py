@@ -32,7 +32,7 @@ _OUT = {"bf16": (torch.bfloat16, _lib.TYPE_BF16), "fp16": (torch.float16, _lib.T
 
 
 class _Forced(threading.local):
-    tile_rows = 0  # rows of a tile; 0: the library's choice (another for tests)
+    tile = (0, 0)  # rows of a tile, and its columns where K is cut into slices; (0, 0): the library's choice (another for tests)
 
 
 class BlockscaleGemm:
@@ -46,19 +46,19 @@ class BlockscaleGemm:
         self._forced = _Forced()  # (one launcher serves all callers of its sizes: what a thread forces is its own)
 
     @property
-    def tile_rows(self):
-        return self._forced.tile_rows
+    def tile(self):
+        return self._forced.tile
 
-    @tile_rows.setter
-    def tile_rows(self, rows):
-        self._forced.tile_rows = rows
+    @tile.setter
+    def tile(self, tile):
+        self._forced.tile = tile
 
     def _args(self, M):
         if M < 1 or M > 1 << 22:
             raise ValueError(f"M={M} outside [1, 2^22]")
         a = _lib.BlockscaleArgs()
         a.M, a.N, a.K, a.groups = M, self.N, self.K, self.groups or 1
-        a.out_dtype, a.tile_rows = _lib.OUT_DTYPE[self.out_dtype], self.tile_rows
+        a.out_dtype, (a.tile_rows, a.slice_columns) = _lib.OUT_DTYPE[self.out_dtype], self.tile
         return a
 
     def _plan(self, M):
@@ -73,7 +73,7 @@ class BlockscaleGemm:
         """Launch on ``stream`` (``None``: the current stream of the device of ``C``)."""
         offsets, M, stream = self._rest(*rest, **named)
         if stream is not None and type(M) is int and type(C) is torch.Tensor and C.is_cuda and _lib.is_current(C.get_device()):
-            key = (M, self._forced.tile_rows)
+            key = (M, self._forced.tile)
             plan = self._plans.get(key)
             if plan is None:
                 if len(self._plans) >= 256:

@@ -16,6 +16,9 @@ FP8 = torch.float8_e4m3fn
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
 HALF = {"bf16": 2.0**-8, "fp16": 2.0**-11}
 GUARD = -77.0
+AUTO, STREAM = (0, 0), (1, 0)
+WHOLE = [(16, 0), (32, 0), (64, 0), (128, 0)]  # rows of a tile, K in one piece
+SLICED = [(16, 16), (16, 32), (32, 32), (32, 64), (64, 64)]  # rows and columns of a tile, K in slices
 
 
 def _operands(rows, n, k, groups, seed, exact=True):
@@ -55,7 +58,7 @@ def _want(a, w, sa, sb, offsets):
     return rows, torch.cat(vals or [torch.empty(0, n, dtype=torch.float64)]), torch.cat(mags or [torch.empty(0, n, dtype=torch.float64)])
 
 
-def _run(a, w, sa, sb, offsets, out, tile_rows=0, strided=False, same=True):
+def _run(a, w, sa, sb, offsets, out, tile=AUTO, strided=False, same=True):
     """offsets None: the dense product of the one weight."""
     groups, n, k = w.shape
     m = a.shape[0]
@@ -68,15 +71,15 @@ def _run(a, w, sa, sb, offsets, out, tile_rows=0, strided=False, same=True):
         scales = wide[:, 1 : 1 + m]
     rest = (m,) if offsets is None else (torch.tensor(offsets, dtype=torch.int32).cuda(), m)
     args = a.cuda(), _shuffled(w).cuda(), scales, sb.cuda(), *rest
-    print(f"blockscale M={m} N={n} K={k} groups={groups if offsets is not None else '-'} {out} tile {tile_rows} strided {strided}", flush=True)
-    fn.tile_rows = tile_rows
+    print(f"blockscale M={m} N={n} K={k} groups={groups if offsets is not None else '-'} {out} tile {tile} strided {strided}", flush=True)
+    fn.tile = tile
     try:
         fn(c, *args, torch.cuda.current_stream())
         again = torch.full_like(c, GUARD)
         fn(again, *args)
         torch.cuda.synchronize()
     finally:
-        fn.tile_rows = 0
+        fn.tile = AUTO
     assert not same or torch.equal(c.view(torch.int16), again.view(torch.int16))
     return c.cpu()
 
@@ -95,18 +98,18 @@ def _check_random(c, a, w, sa, sb, offsets, out):
     assert ((c[rows].double() - vals).abs() <= HALF[out] * vals.abs() + (128 + -(-k // 128) + 2) * 2.0**-23 * (1 + HALF[out]) * mags + 2.0**-25).all()
 
 
-@pytest.mark.parametrize("tile_rows", [0, 16, 32, 64, 128])
+@pytest.mark.parametrize("tile", [AUTO, STREAM] + WHOLE + SLICED)
 @pytest.mark.parametrize("m,n,k", [(1, 16, 64), (1, 272, 192), (5, 128, 128), (17, 400, 576), (33, 256, 1088), (64, 144, 2048), (129, 528, 320), (300, 640, 1152), (257, 272, 64), (16, 16, 8192)])
-def test_dense_exact(m, n, k, tile_rows):
+def test_dense_exact(m, n, k, tile):
     a, w, sa, sb = _operands(m, n, k, 1, m + n + k)
     for out in ("bf16", "fp16"):
-        _check_exact(_run(a, w, sa, sb, None, out, tile_rows), a, w, sa, sb, None, out)
+        _check_exact(_run(a, w, sa, sb, None, out, tile), a, w, sa, sb, None, out)
 
 
-@pytest.mark.parametrize("tile_rows", [0, 16, 32, 64, 128])
-def test_scales_of_a_wider_tensor(tile_rows):
+@pytest.mark.parametrize("tile", [AUTO, STREAM] + WHOLE + SLICED)
+def test_scales_of_a_wider_tensor(tile):
     a, w, sa, sb = _operands(150, 272, 448, 1, 3)
-    _check_exact(_run(a, w, sa, sb, None, "bf16", tile_rows, strided=True), a, w, sa, sb, None, "bf16")
+    _check_exact(_run(a, w, sa, sb, None, "bf16", tile, strided=True), a, w, sa, sb, None, "bf16")
 
 
 @pytest.mark.parametrize("steps", range(1, 15))
@@ -114,7 +117,16 @@ def test_every_length_of_the_large_tile(steps):
     """1 to 14 steps of K, with half a step at the end and without: the loop's builds with and without checks, and its ends."""
     for k in (steps * 128 - 64, steps * 128):
         a, w, sa, sb = _operands(140, 288, k, 1, k)
-        _check_exact(_run(a, w, sa, sb, None, "bf16", 128), a, w, sa, sb, None, "bf16")
+        _check_exact(_run(a, w, sa, sb, None, "bf16", (128, 0)), a, w, sa, sb, None, "bf16")
+
+
+@pytest.mark.parametrize("tile", SLICED)
+@pytest.mark.parametrize("steps", [1, 2, 7, 8, 9, 15, 16, 17, 23, 24, 25, 31, 32, 33, 40, 41, 48, 49, 57])
+def test_every_length_of_the_slices(steps, tile):
+    """Up to eight steps a slice, with some slices a step shorter: the loop, its ends, and slices without a step."""
+    for k in (steps * 128 - 64, steps * 128):
+        a, w, sa, sb = _operands(70, 144, k, 1, k)
+        _check_exact(_run(a, w, sa, sb, None, "bf16", tile), a, w, sa, sb, None, "bf16")
 
 
 SIZES = {
@@ -135,14 +147,14 @@ def _offsets(sizes, first=0):
 
 
 @pytest.mark.parametrize("out", ["bf16", "fp16"])
-@pytest.mark.parametrize("tile_rows", [0, 16, 32, 64, 128])
+@pytest.mark.parametrize("tile", [AUTO] + WHOLE + SLICED)
 @pytest.mark.parametrize("sizes", SIZES)
-def test_groups_exact(sizes, tile_rows, out):
+def test_groups_exact(sizes, tile, out):
     s = SIZES[sizes]
     n, k = 272, 320  # half a step at the end, columns that end inside every tile and block
     offsets = _offsets(s, first=2)
     a, w, sa, sb = _operands(offsets[-1] + 5, n, k, len(s), len(s))
-    _check_exact(_run(a, w, sa, sb, offsets, out, tile_rows, strided=tile_rows == 0), a, w, sa, sb, offsets, out)
+    _check_exact(_run(a, w, sa, sb, offsets, out, tile, strided=tile == AUTO), a, w, sa, sb, offsets, out)
 
 
 @pytest.mark.parametrize("n,k", [(16, 64), (1040, 4096), (512, 1600)])
@@ -157,12 +169,13 @@ def test_groups_widths_and_lengths(sizes, n, k):
 def test_random_values_and_the_same_bits_on_every_tile(out):
     offsets = _offsets(SIZES["ragged"])
     a, w, sa, sb = _operands(offsets[-1], 400, 1088, len(offsets) - 1, 3, exact=False)
-    first = None
-    for tile_rows in (16, 32, 64, 128):
-        c = _run(a, w, sa, sb, offsets, out, tile_rows)
-        _check_random(c, a, w, sa, sb, offsets, out)
-        first = c if first is None else first
-        assert torch.equal(c.view(torch.int16), first.view(torch.int16))
+    for tiles in WHOLE, SLICED:
+        first = None
+        for tile in tiles:
+            c = _run(a, w, sa, sb, offsets, out, tile)
+            _check_random(c, a, w, sa, sb, offsets, out)
+            first = c if first is None else first
+            assert torch.equal(c.view(torch.int16), first.view(torch.int16))
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 6144, 4096), (16, 2048, 7168), (100, 1536, 2240), (333, 2832, 2240), (700, 1024, 5120)])
@@ -173,8 +186,8 @@ def test_dense_random(m, n, k):
 
 def test_a_group_alone_is_the_dense_product():
     a, w, sa, sb = _operands(300, 512, 1024, 1, 9, exact=False)
-    for tile_rows in (16, 32, 64, 128):
-        assert torch.equal(_run(a, w, sa, sb, [0, 300], "bf16", tile_rows).view(torch.int16), _run(a, w, sa, sb, None, "bf16", tile_rows).view(torch.int16))
+    for tile in WHOLE + SLICED:
+        assert torch.equal(_run(a, w, sa, sb, [0, 300], "bf16", tile).view(torch.int16), _run(a, w, sa, sb, None, "bf16", tile).view(torch.int16))
 
 
 def test_scales_of_one_are_the_plain_product():
@@ -189,16 +202,16 @@ def test_scales_of_one_are_the_plain_product():
     assert torch.equal(c[:200], dense.cpu())
 
 
-@pytest.mark.parametrize("tile_rows", [0, 16, 32, 64, 128])
-def test_special_values_stay_in_their_rows_and_columns(tile_rows):
+@pytest.mark.parametrize("tile", [AUTO, STREAM] + WHOLE + SLICED)
+def test_special_values_stay_in_their_rows_and_columns(tile):
     a, w, sa, sb = _operands(70, 288, 640, 1, 8)
-    clean = _run(a, w, sa, sb, None, "bf16", tile_rows)[:70]
+    clean = _run(a, w, sa, sb, None, "bf16", tile)[:70]
     a2, w2, sa2, sb2 = a.clone(), w.clone(), sa.clone(), sb.clone()
     a2.view(torch.uint8)[3, 200] = 0x7F  # NaN
     w2.view(torch.uint8)[0, 17, 5] = 0xFF
     sa2[1, 9], sa2[4, 33] = float("inf"), float("nan")
     sb2[0, 2, 0] = float("nan")
-    c = _run(a2, w2, sa2, sb2, None, "bf16", tile_rows)[:70]
+    c = _run(a2, w2, sa2, sb2, None, "bf16", tile)[:70]
     bad = torch.zeros(70, 288, dtype=torch.bool)
     bad[[3, 33]] = True
     bad[:, 17] = True
@@ -225,8 +238,8 @@ def test_last_tiles_at_the_end_of_the_arrays():
     for m, n, k in ((129, 272, 192), (130, 16, 64), (7, 400, 704)):
         a, w, sa, sb = _operands(m, n, k, 2, m)
         offsets = [0, m // 2, m]
-        for tile_rows in (16, 32, 64, 128):
-            _check_exact(_run(a, w, sa, sb, offsets, "bf16", tile_rows), a, w, sa, sb, offsets, "bf16")
+        for tile in WHOLE + SLICED:
+            _check_exact(_run(a, w, sa, sb, offsets, "bf16", tile), a, w, sa, sb, offsets, "bf16")
 
 
 def test_replayed_with_other_sizes():
