@@ -14,5 +14,6 @@ struct RouteParams {
     int renorm;
     float scale;
     int lanes, lanes_group;  // set by the launcher: lanes of a token and of a run of experts
+    int vec;                 // set by the launcher: a lane's logits and bias are whole vectors
 };
 hipError_t psg_launch_moe_route(RouteParams p, int dtype, hipStream_t stream);

@@ -58,7 +58,7 @@ def test_rows_are_the_host_quantisers(rows, dim, dt):
 
 @pytest.mark.parametrize("rows,dim,gated", [(16384, 512, False), (5003, 2056, False), (9000, 1000, True), (4111, 2050, True), (70000, 129, False)])
 def test_many_rows(rows, dim, gated):
-    """The build for many rows, four of them a wavefront, and its end."""
+    """Grids of many workgroups, and their end."""
     x = _x(rows, dim * (2 if gated else 1), torch.bfloat16, rows)
     print(f"quant {rows}x{dim} gated={gated}", flush=True)
     q, s = quant_device.per_1x128_f8_quant(x.cuda(), gated=gated)

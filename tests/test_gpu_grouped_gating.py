@@ -1,7 +1,7 @@
 """GPU tests of the routing with a bias and groups of experts against its definition in 64 bits.
 
-The experts have to be equal.  The definition's scores and the kernel's are both in 64 bits, so they order the same but where two differ by some 2^-52, which these inputs do not have: logits
-are random in 24 bits, or on a grid where equal ones are equal in both.  Weights: the score rounded to fp32, topk of them added, a division and a product: topk + 3 roundings of 2^-24.
+The experts have to be equal.  Without a bias they are compared by their logits, exactly; with one the definition's scores and the kernel's are both in 64 bits, so they order the same but where two differ
+by some 2^-52, which these inputs do not have: logits are random in 24 bits, or on a grid where equal ones are equal in both.  Weights: the score rounded to fp32, topk of them added, a division and a product: topk + 3 roundings of 2^-24.
 """
 
 import math
@@ -27,12 +27,12 @@ def _want(x, bias, topk, scores, groups, topk_groups, group_score, renorm, scale
         top = x.amax(1, keepdim=True)
         p = torch.where(x == top, torch.ones_like(x), torch.exp(x - top)).masked_fill(masked, 0)
         s = p / p.sum(1, keepdim=True)
-    c = s if bias is None else s + bias.double().cpu()
+    c = x if bias is None else s + bias.double().cpu()  # (without a bias the logits themselves, which order like their scores)
     masked = masked | c.isnan()
     c = c.masked_fill(masked, -INF)
     s = s.masked_fill(masked, 0)
     if topk_groups < groups:
-        parts = c.view(t, groups, -1)
+        parts = (s.masked_fill(masked, -INF) if bias is None and group_score == "top2" else c).view(t, groups, -1)
         best = parts.topk(min(2, e // groups), -1)[0]
         worth = best[..., 0] if group_score == "max" else torch.where(best[..., 1] == -INF, best[..., 1], best[..., 0] + best[..., 1])
         order = torch.sort(worth, dim=1, descending=True, stable=True)[1]
@@ -131,6 +131,31 @@ def test_scores_far_from_one(scores):
     x[2, 7] = 0.0
     _run(x, None, 8, scores, renorm=False)
     _run(x, None, 4, scores, 4, 2, "max", renorm=False)
+
+
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+def test_saturated_scores_order_by_their_logits(scores):
+    """sigmoid(40) and sigmoid(60) are both 1 in 64 bits, exp(-800) and exp(-900) both 0: the logits tell them apart."""
+    x = torch.linspace(40, 60, 64)[torch.randperm(64, generator=torch.Generator().manual_seed(0))].repeat(3, 1)
+    x[1] = -x[1] * 20
+    x[2, 5] = INF
+    _run(x, None, 8, scores)
+    _run(x, None, 8, scores, 8, 4, "max")
+
+
+def test_close_scores():
+    """Values a few units of the 32-bit scores apart, inside the last bits that the selection's numbers drop, equal ones among them: what is taken again in 64 bits."""
+    g = torch.Generator().manual_seed(4)
+    for e, groups, kept in ((64, 1, 1), (256, 8, 4), (17, 1, 1), (1024, 1, 1)):
+        x = 0.5 + torch.randint(0, 40, (50, e), generator=g) * 2.0**-22
+        _run(x, None, 8, "sigmoid", groups, kept, "max")
+        _run(x, None, 8, "softmax", groups, kept, "max")
+        bias = torch.randint(0, 3, (e,), generator=g) * 2.0**-30
+        _run(x, bias, 8, "sigmoid", groups, kept, "max")
+    x = _x(50, 64, 3).bfloat16().float()
+    for dtype in ("bf16", "f32"):
+        _run(x, torch.zeros(64), 8, "sigmoid", dtype=dtype)
+        _run(x, torch.zeros(64), 8, "softmax", 8, 3, "max", dtype=dtype)
 
 
 def test_border_that_32_bits_do_not_see():
