@@ -38,7 +38,8 @@ struct Acc<KIND_INT8> {
 
 // MB = 16-row blocks of A (1 to 4); NWIN = 16-column windows per wavefront group (1 or 2).
 // CH = 128-byte K steps per chunk; NWAVES = wavefronts per workgroup.
-// KIND_FP8B: an MFMA's sum is a block's, which its row's and its columns' scale multiply on the way to the sum of the blocks; GROUPS is GroupParams, of which the row scales' stride is used.
+// KIND_FP8B: an MFMA's sum is a block's, which its row's and its columns' scale multiply on the way to the sum of the blocks (16 x 6144 x 4096
+// 7.0 us, against 6.7 with one scale a row); GROUPS is GroupParams, of which the row scales' stride is used.
 template <int KIND, int MB, int NWIN, int NWAVES, int CH, int STORE, class... GROUPS>
 __global__ void __launch_bounds__(NWAVES * 64, KIND == KIND_FP8B ? 2 : 1) k_a8w8_stream(A8W8Params p, GROUPS... groups) {
     using acc_t = typename Acc<KIND>::type;

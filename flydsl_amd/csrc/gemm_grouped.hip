@@ -10,6 +10,8 @@
 
 namespace {
 
+// With block scales (KIND_FP8B) an MFMA's sum is scaled and added a step later, under the next step's MFMAs; the scales of a step stand in LDS beside A: 512 rows on 32 groups, 3584 x 4096, 75.1 us, 5.9 TB/s
+// (one scale a row 74.6).  Its 64-row tile has 180 registers and two wavefronts a SIMD; for three it would spill.
 // KS: K slices, 1 or 4: with four, the wavefronts have the same 16 NR columns and every fourth step each.  NT: W past the caches.
 template <int KIND, int MR, int NR, int KS, bool NT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 2 ? 4 : KIND == KIND_FP8B ? 2 : 3))) k_grouped(A8W8Params p, GroupParams g) {

@@ -1467,7 +1467,8 @@ int psg_gemm_blockscale(const psg_blockscale_args* a, void* stream) {
         if (a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128 && !(a->tile_rows == 1 && !a->offsets && a->M <= 65535 * 64)) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64, 128 or, without offsets, 1", a->tile_rows);
         plan.tn = a->tile_rows <= 32 ? 64 : 2 * a->tile_rows;
     }
-    // (up to 512 threads each: a grid holds less than 2^32)
+    // (up to 512 threads each: a grid holds less than 2^32; a plan without tiles has streamed rows, which know no groups)
+    if (plan.bm == 1 && (a->offsets || a->M > 65535 * 64)) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
     if (plan.bm > 1 && group_tiles_most(a->M, a->groups, plan.bm) * ((a->N + plan.tn - 1ll) / plan.tn) >= 1ll << 23) return fail(PSG_E_SHAPE, "more tiles than a launch holds");
     if (!aligned(a->a, 16) || !aligned(a->w, 16) || !aligned(a->c, 16)) return fail(PSG_E_ALIGN, "a, w and c must be 16-byte aligned");
     if (!aligned(a->scale_a, 4) || !aligned(a->scale_b, 4) || !aligned(a->offsets, 4)) return fail(PSG_E_ALIGN, "scale_a, scale_b and offsets must be 4-byte aligned");

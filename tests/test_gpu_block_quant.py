@@ -176,3 +176,15 @@ def test_replayed():
         graph.replay()
         torch.cuda.synchronize()
         _check_plain(x, *out)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_past_four_gib(gated):
+    """q of more than 2^32 bytes, x of two and four times as many, in more than one launch: rows at the front, about the borders and at the end."""
+    m, dim = 4200007, 1032
+    x = _x(65521, dim * (2 if gated else 1), torch.bfloat16, 4).cuda().repeat(-(-m // 65521), 1)[:m]
+    print(f"quant {m}x{dim} gated={gated}", flush=True)
+    q, s = quant_device.per_1x128_f8_quant(x, gated=gated)
+    torch.cuda.synchronize()
+    rows = torch.tensor([r for at in (0, 2**31 // dim, 2**32 // dim, 2**32 // x.shape[1] // 2, 4 * ((1 << 23) // 3), m) for r in range(max(at - 9, 0), min(at + 9, m))], device="cuda")
+    (_check_gated if gated else _check_plain)(x[rows], q.view(torch.uint8)[rows].view(FP8), s[:, rows])

@@ -304,3 +304,57 @@ def test_refusals():
         for off in (e(2, dt=torch.int32), e(3, dt=torch.int64), e(3, dt=torch.int32, dev="cpu"), None):
             with pytest.raises(ValueError):
                 grouped(*good, off, 10, stream)
+
+
+@pytest.mark.parametrize("n,k,tile", [(16, 1088, AUTO), (16, 1088, STREAM), (16, 1088, (16, 0)), (16, 1088, (128, 0)), (16, 1088, (64, 64)), (528, 64, AUTO), (528, 64, STREAM), (528, 64, (64, 64))])
+def test_rows_past_four_gib(n, k, tile):
+    """A (k = 1088) or C (n = 528) of more than 2^32 bytes: rows at the front, about the border and at the end."""
+    m = 4190003
+    block, w, _, sb = _operands(65521, n, k, 1, 11)
+    a = block.cuda().view(torch.uint8).repeat(-(-m // 65521), 1)[:m].view(FP8)
+    sa = torch.exp2(-torch.randint(0, 4, (-(-k // 128), m), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).float())
+    c = torch.full((m + 1, n), GUARD, dtype=torch.bfloat16, device="cuda")
+    fn = compile_blockscale_gemm(N=n, K=k)
+    print(f"blockscale M={m} N={n} K={k} tile {tile}", flush=True)
+    fn.tile = tile
+    try:
+        fn(c, a, _shuffled(w).cuda(), sa, sb.cuda(), m, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+    finally:
+        fn.tile = AUTO
+    border = 2**32 // (k if n == 16 else 2 * n)
+    rows = torch.tensor([r for at in (0, border // 2, border, m) for r in range(max(at - 70, 0), min(at + 70, m))], device="cuda")
+    want, _ = _product(a.view(torch.uint8)[rows].view(FP8).cpu(), w[0], sa[:, rows].cpu(), sb[0])
+    assert torch.equal(c[rows].cpu(), want.float().bfloat16())
+    assert (c[m] == GUARD).all()
+
+
+@pytest.mark.parametrize("tile", [AUTO, (32, 0), (128, 0), (16, 16)])
+def test_weights_past_four_gib(tile):
+    """37 groups' weights of 5 GB: rows of the first, of those about the border and of the last."""
+    groups, n, k = 37, 16400, 8128
+    sizes = [3 if e in (0, 31, 32, 36) else 0 for e in range(groups)]
+    offsets, m = _offsets(sizes), sum(sizes)
+    a, _, sa, _ = _operands(m, 16, k, 1, 21)
+    codes = torch.arange(-4, 5).float().to(FP8).view(torch.int8).cuda()
+    laid, plain = torch.empty(groups, n, k, dtype=torch.int8, device="cuda"), {}
+    for e in range(groups):
+        w = codes[torch.randint(0, 9, (n, k), device="cuda", generator=torch.Generator("cuda").manual_seed(e))]
+        laid[e] = layout.shuffle_weight(w.unsqueeze(0))[0]
+        if sizes[e]:
+            plain[e] = w.view(FP8)
+    sb = torch.exp2(-torch.randint(0, 4, (groups, -(-n // 128), -(-k // 128)), generator=torch.Generator().manual_seed(1)).float())
+    fn = compile_grouped_blockscale_gemm(N=n, K=k, groups=groups)
+    c = torch.full((m + 1, n), GUARD, dtype=torch.bfloat16, device="cuda")
+    print(f"blockscale {groups} x {n} x {k} tile {tile}", flush=True)
+    fn.tile = tile
+    try:
+        fn(c, a.cuda(), laid.view(FP8), sa.cuda(), sb.cuda(), torch.tensor(offsets, dtype=torch.int32).cuda(), m, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+    finally:
+        fn.tile = AUTO
+    for e, w in plain.items():
+        r = slice(offsets[e], offsets[e + 1])
+        want, _ = _product(a[r].cuda(), w, sa[:, r].cuda(), sb[e].cuda())
+        assert torch.equal(c[r], want.float().bfloat16()), e
+    assert (c[m] == GUARD).all()

@@ -200,3 +200,20 @@ def test_replayed():
         torch.cuda.synchronize()
         want, ww = _want(x, bias, 8, "sigmoid", 8, 4, "top2", True, 1.0)
         assert torch.equal(ids.cpu().long(), want) and ((w.double().cpu() - ww).abs() <= 11 * 2.0**-24 * ww).all()
+
+
+def test_most_tokens():
+    """2^24 - 1 tokens, logits of more than 2^32 bytes: tokens at the front, about the border and at the end."""
+    t, e = (1 << 24) - 1, 130
+    x = _x(65521, e, 3).bfloat16().cuda().repeat(-(-t // 65521), 1)[:t]
+    bias = _x(1, e, 4, 0.1)[0]
+    fn = build_grouped_topk_gating_module(e, 4, "bf16", scores="sigmoid", groups=10, topk_groups=3, group_score="top2", scale=1.5)
+    ids, w = torch.full((t + 1, 4), -7, dtype=torch.int32, device="cuda"), torch.full((t + 1, 4), -7.0, device="cuda")
+    print(f"route {t}x{e}", flush=True)
+    fn(x, bias.cuda(), w, ids, t, stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    rows = torch.tensor([r for at in (0, 2**31 // (2 * e), 2**32 // (2 * e), t) for r in range(max(at - 40, 0), min(at + 40, t))], device="cuda")
+    want, ww = _want(x[rows], bias, 4, "sigmoid", 10, 3, "top2", True, 1.5)
+    assert torch.equal(ids[rows].cpu().long(), want)
+    assert ((w[rows].double().cpu() - ww).abs() <= 7 * 2.0**-24 * ww.abs()).all()
+    assert (ids[t] == -7).all() and (w[t] == -7).all()
