@@ -1,5 +1,5 @@
 // Block-scaled fp8 products of few tiles (gfx950): C[r, n] = sum over blocks b of 128 along K of sa[b, r] sb[n / 128, b] (A[r, b] W[n, b]^T), by tiles of 16 to 64 rows whose K is cut into eight slices; and which way such a product takes.
-// (Few rows: gemm_a8w8_stream.hip.  Many tiles: gemm_grouped.hip and gemm_pair.hip.)
+// (Few rows: gemm_a8w8_stream.hip.  Many tiles: gemm_grouped.hip, gemm_pair.hip, and the 128 x 128 tile of gemm_tiled8.h, which is built here.)
 //
 // With about a tile for every CU what counts is how soon its operands are there: a step of 128 bytes of K takes a workgroup that goes from step to step together a memory latency, whatever it
 // multiplies.  Here the eight wavefronts of a workgroup have the same tile and every eighth step each, and nothing to do with each other until their sums meet in LDS: a wavefront asks for all of its
@@ -10,6 +10,7 @@
 #include <cmath>
 
 #include "gemm_tiled.h"
+#include "gemm_tiled8.h"
 #include "group_tiles.h"
 #include "lds_dma.h"
 
@@ -121,12 +122,17 @@ hipError_t launch(const A8W8Params& p, GroupParams g, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int STORE>
+__global__ void __launch_bounds__(256, 2) k_block_square(A8W8Params p, GroupParams g) {
+    tiled_dma<KIND_FP8B, STORE, 8, 4, 4, 3>(p, g);
+}
+
 }  // namespace
 
 // The way of the least estimated time, in us.  Of `load` tiles a CU: a tile's steps when it is alone on its CU, longer as more CUs are at work; a CU's steps and tile ends where it has many (whole rounds of
 // small tiles, up to four); W from memory.
-// The constants are fitted to the times of 3,400 products of 1 to 32,768 rows on 1 to 128 groups; the choice is 3.5 % slower than the best way dense and 2.6 % grouped, in the geometric mean (the choice
-// for one scale a row, psg_grouped_plan, 15 and 7).  Slices with 16 x 64, 32 x 16, 64 x 16 and 64 x 32 tiles win 0.2 % more together and are not built.
+// The constants are fitted to the times of 3,400 products of 1 to 32,768 rows on 1 to 128 groups (128 x 128 tiles to 6,000 others); on 4,900 more the choice is 3.5 % slower than the best way dense and
+// 2.8 % grouped, in the geometric mean (the choice for one scale a row, psg_grouped_plan, 15 and 7).  Slices with 16 x 64, 32 x 16, 64 x 16 and 64 x 32 tiles win 0.2 % more together and are not built.
 // us, whole K on 16, 32, 64, 128 rows / slices on 16 x 16, 16 x 32, 32 x 32, 32 x 64, 64 x 64 / streamed: 346 x 352 x 11328 20.9, 23.3, 44.8, 69.7 / 12.4, 9.6, 11.7, 16.2, 22.3 / 19.1; 201 x 752 x 10624 21.9, 23.5, 41.9, 71.7 / 15.4,
 // 14.0, 11.3, 15.5, 20.6 / 15.1; 775 x 624 x 13184 35.8, 31.5, 52.2, 94.9 / 41.0, 34.3, 26.1, 21.1, 28.4 / -; 127 x 5104 x 2944 12.7, 11.0, 15.1, 21.0 / 15.9, 13.3, 10.9, 12.0, 9.5 / -; 13 x 1616 x 16256 35.7, 38.1, 63.0, 129 /
 // 15.3, 17.4, 18.1, 26.9, 30.6 / 10.4; 8 rows on 8, 1552 x 5504, 12.2, 13.6, 24.1, 33.6 / 6.5, 6.8, 7.3, 8.8, 10.7; 620 x 1760 x 832 7.7, 6.4, 7.2, 9.9 / 14.9, 9.9, 8.8, 10.0, 9.4.
@@ -134,7 +140,7 @@ BlockPlan psg_block_plan(int64_t rows, int groups, bool dense, int N, int K) {
     struct Way { int bm, tn; bool sliced, rounds; double start, alone, more, busy, end; };
     static constexpr Way ways[] = {
         {16, 64, false, true, 2.78, 0.199, 0.135, 0.173, 0.25},  {32, 64, false, true, 2.86, 0.228, 0.131, 0.202, 0.31}, {64, 128, false, false, 3.72, 0.449, 0.179, 0.425, 1.24},
-        {128, 256, false, false, 3.99, 0.729, 0.762, 0.966, 2.51},
+        {128, 128, false, false, 4.28, 0.494, 0.152, 0.696, 1.77}, {128, 256, false, false, 3.99, 0.729, 0.762, 0.966, 2.51},
         {16, 16, true, true, 2.43, 0.471, 0.288, 0.397, 0.24},   {16, 32, true, true, 2.28, 0.597, 0.544, 0.629, 0.19},  {32, 32, true, true, 2.06, 0.718, 0.693, 0.851, 0.32},
         {32, 64, true, false, 2.66, 0.943, 1.030, 1.768, 0.74},  {64, 64, true, false, 2.93, 1.257, 1.492, 2.147, 1.16},
     };
@@ -156,6 +162,17 @@ BlockPlan psg_block_plan(int64_t rows, int groups, bool dense, int N, int K) {
         if (t < least) least = t, best = {w.bm, w.tn, w.sliced};
     }
     return best;
+}
+
+// Tiles of 128 x 128, K in one piece, for one or two tiles a CU; bf16 by STORE_C, fp16 by STORE_C_GENERIC.  us, these / 128 x 256 tiles / the best of the others: 1024 x 4096 x 4096 25.1 / 36.1 / 30.3,
+// 700 x 5120 x 5120 29.2 / 43.8 / 34.6, 512 x 8192 x 8192 44.9 / 69.0 / 55.7, 512 x 7168 x 2048 15.2 / 21.3 / 17.2; of more tiles 2048 x 4096 x 4096 40.1 / 37.9, 8192 x 4096 x 4096 148 / 120, of fewer
+// 256 x 4096 x 4096 23.4 / 36.1 / 12.7, 512 x 4096 x 4096 23.8 / 35.7 / 20.2.
+hipError_t psg_launch_block_square(const A8W8Params& p, GroupParams g, hipStream_t stream) {
+    g.most = (int)group_tiles_most(p.M, g.groups, 128);
+    const dim3 grid((unsigned)g.most * (unsigned)((p.N + 127) / 128));
+    if (p.out == OUT_BF16) hipLaunchKernelGGL((k_block_square<STORE_C>), grid, dim3(256), 0, stream, p, g);
+    else hipLaunchKernelGGL((k_block_square<STORE_C_GENERIC>), grid, dim3(256), 0, stream, p, g);
+    return hipGetLastError();
 }
 
 hipError_t psg_launch_block_sliced(const A8W8Params& p, const GroupParams& g, int bm, int tn, hipStream_t stream) {

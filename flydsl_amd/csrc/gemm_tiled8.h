@@ -31,6 +31,7 @@
 //     converted.  Epilogue scales wait in LDS since the prologue.
 #pragma once
 #include "gemm_tiled.h"
+#include "group_tiles.h"
 #include "lds_dma.h"
 
 namespace {
@@ -62,8 +63,10 @@ __device__ unsigned long long* t8_dbg;
 //       it above 256 rows only: more bytes in flight per CU is not what these launches lack.  Nor is it wavefronts per SIMD: the same
 //       tile with eight wavefronts as 2 x 4 (four m-blocks each, W three steps ahead) took 53.1 against 48.3 us at M=512 and 77.6
 //       against 69.2 at 384x5120x13824 (every W fragment is then loaded by two wavefronts).
-template <int KIND, int STORE, int MR, int WAVES, int NS, int PFW>
-__global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
+//   <8, 4, 4, 3> for block scales (KIND_FP8B, with GroupParams): the same with four stages, two workgroups a CU.  An m-block's sums of a step are scaled and added in vector registers under the MFMAs of the
+//       next one; the scales travel as MX's do.  (Eight stages and one workgroup, whose MFMAs the compiler gives accumulator registers to write and copies out of them, 32.2 against 25.1 us for 1024 x 4096 x 4096.)
+template <int KIND, int STORE, int MR, int WAVES, int NS, int PFW, class... GROUPS>
+__device__ __forceinline__ void tiled_dma(A8W8Params& p, const GROUPS&... groups) {
     using acc_t = typename Acc<KIND>::type;
     constexpr int NR = 2;
     constexpr int TM = 16 * MR, TN = 16 * NR * WAVES;
@@ -76,12 +79,14 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     constexpr bool W4 = KIND == KIND_MXA8W4 || KIND == KIND_MXA6W4;  // fp4 W against a wider A: half a row's bytes
     constexpr bool MX = KIND == KIND_MXFP8 || W4;
     static_assert(!MX || (MR == 16 && NS == 4), "MX scale slots are laid out for the 256-row tile");
+    constexpr bool BLOCKED = KIND == KIND_FP8B;
+    static_assert(BLOCKED == (sizeof...(GROUPS) == 1) && (!BLOCKED || (TM == 128 && TN == 128)), "block scales: those of 128 rows and of one block of columns");
 
     // LDS: the A stages; behind them NS slots of MX scale dwords (per slot 8 A-side chunks + 8 W-side chunks of 256 bytes)
     // or the per-token / per-channel scales of the epilogue (TM + TN floats) and its bias (TN 16-bit values)
-    constexpr int SC_SLOT = 4096;
-    constexpr bool BIAS = STORE == STORE_C_GENERIC && !MX;
-    constexpr int LDS_EXTRA = MX ? NS * SC_SLOT : (TM + TN) * 4 + (BIAS ? TN * 2 : 0);
+    constexpr int SC_SLOT = BLOCKED ? 1024 : 4096;
+    constexpr bool BIAS = STORE == STORE_C_GENERIC && !MX && !BLOCKED;
+    constexpr int LDS_EXTRA = MX || BLOCKED ? NS * SC_SLOT : (TM + TN) * 4 + (BIAS ? TN * 2 : 0);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + LDS_EXTRA];
     uint8_t* const lds_x = lds + NS * STAGE;
 
@@ -94,9 +99,28 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
 
     const int tiles_m = (p.M + TM - 1) / TM;
     const int tiles_n = (p.N + TN - 1) / TN;
-    int tm, tn;
-    tile_coords((int)blockIdx.x, tiles_m, tiles_n, p.group_m, tm, tn);
-    const int m0 = tm * TM;
+    int tm, tn, m0;
+    // block scales: wavefront 0 and 1 bring those of a step's rows, 2 that of its columns, the same in every lane, 3 nothing
+    __amdgpu_buffer_rsrc_t block_scales;
+    uint32_t scale_voff = OOB, scale_step = 0;
+    if constexpr (BLOCKED) {
+        GroupTile t;
+        if (!group_tile<true>((groups, ...), p.M, TM, (int)blockIdx.x, tiles_n, lane, t)) return;
+        m0 = t.row, tn = t.n_tile;
+        const uint32_t KB = ((uint32_t)p.K + TK - 1) / TK;
+        if (wave < 2) {
+            block_scales = make_rsrc_uniform(p.sa + m0, ((uint64_t)(KB - 1) * (groups, ...).sa_stride + (uint32_t)(p.M - m0)) * 4ull);
+            scale_voff = (uint32_t)tid * 4u, scale_step = (groups, ...).sa_stride * 4u;
+        } else {
+            block_scales = make_rsrc_uniform(p.sb + ((uint64_t)t.e * (uint32_t)tiles_n + (uint32_t)tn) * KB, KB * 4ull);
+            scale_voff = wave == 2 ? 0u : OOB, scale_step = 4u;
+        }
+        p.M = t.row + t.rows;  // the group's end
+        p.b += (uint64_t)t.e * (uint64_t)p.N * (uint64_t)p.K;
+    } else {
+        tile_coords((int)blockIdx.x, tiles_m, tiles_n, p.group_m, tm, tn);
+        m0 = tm * TM;
+    }
     const int n0 = tn * TN;
     const int K = IS16 ? (p.K << 1) : p.K;  // BYTES of one operand row
     const int KT = (K + TK - 1) / TK;
@@ -125,6 +149,9 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
         rsb = make_rsrc_uniform(p.mx_sb + (sb_mine < sb_chunks ? sb_mine : sb_chunks) * chunk_bytes, sb_mine < sb_chunks ? chunk_bytes : 0);
     }
     int sav[2][MP], sbv[2][NP];
+    // the lane's row scales of a step (two sets, read a step ahead) and its columns' one; an m-block's products of them and its MFMAs' sums, which the next m-block adds
+    float row_scale[2][MR], column_scale[2], scale[2] = {};
+    v4f part[2][NR] = {};
 
     acc_t acc[MR][NR];
 #pragma unroll
@@ -167,6 +194,26 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
         if (q < MP) sa_dst[q] = *reinterpret_cast<const int*>(lds_x + slot * SC_SLOT + q * 256 + lane * 4);
         else sb_dst[0] = *reinterpret_cast<const int*>(lds_x + slot * SC_SLOT + 2048 + wave * 256 + lane * 4);
     };
+    auto dma_block_scale = [&](int kt, int slot) __attribute__((always_inline)) {
+        const bool has = kt < kt_end;
+        dma4(block_scales, lds_base + (uint32_t)(NS * STAGE + slot * SC_SLOT + wave * 256), has ? scale_voff : OOB, has ? (uint32_t)kt * scale_step : 0u);
+    };
+    // (behind 64 KB an LDS instruction's own offset does not reach; as constants the addresses are put together in front of every read)
+    int rows_at = NS * STAGE + li * 4, columns_at = NS * STAGE + 512 + lane * 4;
+    if constexpr (BLOCKED) asm volatile("" : "+v"(rows_at), "+v"(columns_at));
+    auto read_block_scale = [&](int slot, int q, int set) __attribute__((always_inline)) {
+        if (q < MR) row_scale[set][q < MR ? q : 0] = *reinterpret_cast<const float*>(lds + rows_at + slot * SC_SLOT + q * 64);
+        else column_scale[set] = *reinterpret_cast<const float*>(lds + columns_at + slot * SC_SLOT);
+    };
+    auto add_parts = [&](auto MI) __attribute__((always_inline)) {
+        constexpr int mi = decltype(MI)::value;
+#pragma unroll
+        for (int ni = 0; ni < NR; ni++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[mi][ni][i] = __builtin_fmaf(part[mi & 1][ni][i], scale[mi & 1], acc[mi][ni][i]);
+            asm volatile("" : "+v"(acc[mi][ni]));  // (here, not behind the branches of the last steps)
+        }
+    };
     const uint32_t b_lane_off = p.b_rowmajor ? (uint32_t)li * (uint32_t)K + (uint32_t)lg * 16u : (uint32_t)lane * 16u;
     const uint32_t b_step = p.b_rowmajor ? 128u : W4 ? 1024u : 2048u, b_half = p.b_rowmajor ? 64u : 1024u;
     auto load_b1 = [&](int kt, int idx, v4i* lo, v4i* hi, auto CHK) __attribute__((always_inline)) {
@@ -195,9 +242,9 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     // m-blocks ahead, the last two those of step kt+1.
     // (always_inline: with many call sites the inliner would otherwise leave this lambda a function of its own, with the
     // accumulators and descriptors passed through memory)
-    constexpr int N_DMA = A_DMA + (MX ? 2 : 0);  // DMAs per wavefront per step
+    constexpr int N_DMA = A_DMA + (MX ? 2 : BLOCKED ? 1 : 0);  // DMAs per wavefront per step
     constexpr int N_W = W4 ? NR : 2 * NR;        // W fragment loads per wavefront per step
-    constexpr int N_OPS = A_DMA + (MX ? 1 : 0) + N_W;          // slots: the two scale DMAs share one
+    constexpr int N_OPS = A_DMA + (MX || BLOCKED ? 1 : 0) + N_W;          // slots: the two scale DMAs share one
     constexpr int OPS_PER = (N_OPS + MR - 2) / (MR - 1);       // slots per m-block (m-blocks 1 .. MR-1)
     auto step = [&](int kt, auto SP, auto CHK) __attribute__((always_inline)) {
         constexpr int S = decltype(SP)::value;   // LDS stage of this step (kt % NS)
@@ -218,6 +265,8 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
                     } else if constexpr (MX && op == A_DMA) {
                         dma_sc(kt + NS - 1, (S + NS - 1) % NS, 0);
                         dma_sc(kt + NS - 1, (S + NS - 1) % NS, 1);
+                    } else if constexpr (BLOCKED && op == A_DMA) {
+                        dma_block_scale(kt + NS - 1, (S + NS - 1) % NS);
                     } else if constexpr (op < N_OPS) {
                         load_b1(kt + PFW, op - (N_OPS - N_W), blo[SN], bhi[SN], CHK);
                     }
@@ -225,6 +274,10 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
             }
             // MX: the scale dwords of step kt+1 leave their slot for the other register set, one per m-block
             if constexpr (MX && mi >= MR - (MP + NP)) read_sc((S + 1) % NS, mi - (MR - (MP + NP)), sav[SS ^ 1], sbv[SS ^ 1]);
+            if constexpr (BLOCKED) {
+                read_block_scale((S + 1) % NS, mi, SS ^ 1);
+                if constexpr (mi == MR - 1) read_block_scale((S + 1) % NS, MR, SS ^ 1);
+            }
             __builtin_amdgcn_sched_barrier(0);
             const v4i alo = flo[mi % FRAG_BUFS], ahi = fhi[mi % FRAG_BUFS];
             if constexpr (KIND == KIND_INT8) {
@@ -255,6 +308,18 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
                         mfma_mx4w<SS, ni & 1, mi & 1>(acc[mi][ni], blo[SB][ni], af, sbv[SS][ni / 2], sav[SS][mi / 2]);
                     }
                 });
+            } else if constexpr (BLOCKED) {
+                const v8i af = {alo[0], alo[1], alo[2], alo[3], ahi[0], ahi[1], ahi[2], ahi[3]};
+#pragma unroll
+                for (int at = 0; at < NR; at++) {
+                    const int ni = mi & 1 ? NR - 1 - at : at;
+                    const v8i bf = {blo[SB][ni][0], blo[SB][ni][1], blo[SB][ni][2], blo[SB][ni][3],
+                                    bhi[SB][ni][0], bhi[SB][ni][1], bhi[SB][ni][2], bhi[SB][ni][3]};
+                    part[mi & 1][ni] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf, af, (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                add_parts(std::integral_constant<int, (mi + MR - 1) % MR>{});
+                scale[mi & 1] = row_scale[SS][mi] * column_scale[SS];
             } else if constexpr (KIND == KIND_MXFP8) {
                 const v8i af = {alo[0], alo[1], alo[2], alo[3], ahi[0], ahi[1], ahi[2], ahi[3]};
                 static_for<NR>([&](auto NI) {
@@ -301,20 +366,37 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
             ep_bias = p.bias[n < p.N ? n : p.N - 1];
         }
     }
+    if constexpr (BLOCKED) {
+        // W in turn with A from A's third step on, so that the first step waits for two of them only
+        static_assert(NS - 1 == PFW && (NS - 3) * N_DMA + PFW * N_W <= 63, "the wait behind");
+        static_for<NS + 1>([&](auto I) {
+            constexpr int s = decltype(I)::value, w = s - 2;
+            if constexpr (s < NS - 1) {
 #pragma unroll
-    for (int s = 0; s < NS - 1; s++) {
+                for (int j = 0; j < A_DMA; j++) dma_a1(kt_begin + s, s, j, std::true_type{});
+                dma_block_scale(kt_begin + s, s);
+            }
+            if constexpr (w >= 0) {
 #pragma unroll
-        for (int j = 0; j < A_DMA; j++) dma_a1(kt_begin + s, s, j, std::true_type{});
-        if constexpr (MX) {
-            dma_sc(kt_begin + s, s, 0);
-            dma_sc(kt_begin + s, s, 1);
+                for (int idx = 0; idx < N_W; idx++) load_b1(kt_begin + w, idx, blo[w], bhi[w], std::true_type{});
+            }
+        });
+    } else {
+#pragma unroll
+        for (int s = 0; s < NS - 1; s++) {
+#pragma unroll
+            for (int j = 0; j < A_DMA; j++) dma_a1(kt_begin + s, s, j, std::true_type{});
+            if constexpr (MX) {
+                dma_sc(kt_begin + s, s, 0);
+                dma_sc(kt_begin + s, s, 1);
+            }
         }
-    }
-    static_for<PFW>([&](auto I) {
-        constexpr int i = decltype(I)::value;
+        static_for<PFW>([&](auto I) {
+            constexpr int i = decltype(I)::value;
 #pragma unroll
-        for (int idx = 0; idx < N_W; idx++) load_b1(kt_begin + i, idx, blo[i], bhi[i], std::true_type{});
-    });
+            for (int idx = 0; idx < N_W; idx++) load_b1(kt_begin + i, idx, blo[i], bhi[i], std::true_type{});
+        });
+    }
     if constexpr (SCALED && STORE != STORE_ACC) {
         if (tid < TM) reinterpret_cast<float*>(lds_x)[tid] = ep_sa;
         if (tid < TN) reinterpret_cast<float*>(lds_x)[TM + tid] = ep_sb;
@@ -322,7 +404,7 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     if constexpr (BIAS) {
         if (tid < TN) reinterpret_cast<uint16_t*>(lds_x + (TM + TN) * 4)[tid] = ep_bias;
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PFW * N_W) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(PFW * N_W + (BLOCKED ? (NS - 3) * N_DMA : 0)) : "memory");
     static_for<FRAG_AHEAD>([&](auto I) {
         constexpr int i = decltype(I)::value;
         read_frag(0, i, flo[i], fhi[i]);
@@ -330,6 +412,11 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     if constexpr (MX) {
 #pragma unroll
         for (int q = 0; q < MP + NP; q++) read_sc(0, q, sav[0], sbv[0]);
+    }
+
+    if constexpr (BLOCKED) {
+#pragma unroll
+        for (int q = 0; q < MR + 1; q++) read_block_scale(0, q, 0);
     }
 
     T8_STAMP(1);
@@ -348,6 +435,7 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     static_for<NS - 1>([&](auto I) {
         if (kt + decltype(I)::value < kt_end) step(kt + decltype(I)::value, I, std::true_type{});
     });
+    if constexpr (BLOCKED) add_parts(std::integral_constant<int, MR - 1>{});
     // wait states between the last MFMA and the first ordinary read of an accumulator (the compiler does not know that the
     // asm statements are MFMAs), and every DMA still on its way (redirected past the bounds) must be done before the
     // stages are reused for C
@@ -450,6 +538,11 @@ __global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     T8_STAMP(3);
 #endif
+}
+
+template <int KIND, int STORE, int MR, int WAVES, int NS, int PFW>
+__global__ void __launch_bounds__(WAVES * 64, 1) k_tiled_dma(A8W8Params p) {
+    tiled_dma<KIND, STORE, MR, WAVES, NS, PFW>(p);
 }
 
 template <int KIND, int STORE, int MR, int WAVES, int NS, int PFW>

@@ -27,6 +27,7 @@ struct BlockPlan {
 };
 BlockPlan psg_block_plan(int64_t rows, int groups, bool dense, int N, int K);
 double psg_blockscale_stream_us(int M, int N, int K);
+hipError_t psg_launch_block_square(const A8W8Params& p, GroupParams g, hipStream_t stream);
 hipError_t psg_launch_block_sliced(const A8W8Params& p, const GroupParams& g, int bm, int tn, hipStream_t stream);
 hipError_t psg_launch_blockscale_stream(const A8W8Params& p, const GroupParams& g, hipStream_t stream);
 hipError_t psg_launch_grouped_pair(const A8W8Params& p, GroupParams g, int kind, hipStream_t stream);

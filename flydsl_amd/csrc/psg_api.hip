@@ -1455,14 +1455,15 @@ int psg_gemm_blockscale(const psg_blockscale_args* a, void* stream) {
     const int64_t kb = (a->K + 127ll) / 128, ss = a->scale_a_stride ? a->scale_a_stride : a->M;
     if (ss < a->M) return fail(PSG_E_SHAPE, "scale_a_stride=%lld is below M=%d", (long long)a->scale_a_stride, a->M);
     if (ss > 0x7FFFFFFF || (uint64_t)kb * (uint64_t)ss * 4ull >= OOB) return fail(PSG_E_SHAPE, "scale_a exceeds the 4 GiB descriptor range");
-    BlockPlan plan = {a->tile_rows, 0, a->slice_columns != 0};
+    BlockPlan plan = {a->tile_rows, a->slice_columns, a->slice_columns != 0 && a->tile_rows != 128};
     if (a->tile_rows == 0) {
         if (a->slice_columns) return fail(PSG_E_SHAPE, "slice_columns=%d without tile_rows", a->slice_columns);
         plan = psg_block_plan(a->M, a->groups, !a->offsets, a->N, a->K);
     } else if (plan.sliced) {
         const int r = a->tile_rows, c = a->slice_columns;
         if (!(r == 16 && (c == 16 || c == 32)) && !(r == 32 && (c == 32 || c == 64)) && !(r == 64 && c == 64)) return fail(PSG_E_SHAPE, "no tiles of %d rows and %d columns in slices", r, c);
-        plan.tn = c;
+    } else if (a->slice_columns) {
+        if (a->slice_columns != 128) return fail(PSG_E_SHAPE, "no tiles of %d rows and %d columns", a->tile_rows, a->slice_columns);
     } else {
         if (a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64 && a->tile_rows != 128 && !(a->tile_rows == 1 && !a->offsets && a->M <= 65535 * 64)) return fail(PSG_E_SHAPE, "tile_rows=%d must be 0, 16, 32, 64, 128 or, without offsets, 1", a->tile_rows);
         plan.tn = a->tile_rows <= 32 ? 64 : 2 * a->tile_rows;
@@ -1477,7 +1478,7 @@ int psg_gemm_blockscale(const psg_blockscale_args* a, void* stream) {
     p.M = a->M, p.N = a->N, p.K = a->K, p.epi = EPI_NONE, p.out = a->out_dtype, p.splits = 1;
     const GroupParams g = {a->offsets, a->groups, 0, 0, (uint32_t)ss};
     hipStream_t const st = static_cast<hipStream_t>(stream);
-    const hipError_t e = plan.bm == 1 ? psg_launch_blockscale_stream(p, g, st) : plan.sliced ? psg_launch_block_sliced(p, g, plan.bm, plan.tn, st) : psg_launch_grouped(p, g, KIND_FP8B, {plan.bm, false}, st);
+    const hipError_t e = plan.bm == 1 ? psg_launch_blockscale_stream(p, g, st) : plan.sliced ? psg_launch_block_sliced(p, g, plan.bm, plan.tn, st) : plan.bm == 128 && plan.tn == 128 ? psg_launch_block_square(p, g, st) : psg_launch_grouped(p, g, KIND_FP8B, {plan.bm, false}, st);
     if (e != hipSuccess) return hip_fail(e, "psg_gemm_blockscale launch");
     g_err[0] = 0;
     return 0;

@@ -581,7 +581,7 @@ int psg_quant_block(const psg_quant_block_args *args, void *stream);
  * that meet has to be a normal number of fp32 for the result to have its precision.  Within a call every row is summed in the same order; a call of other sizes may take other tiles, and with
  * few of them slices of K, whose sums differ in the last places.
  * tile_rows 0 (the library's choice by M, N, K and groups); for tests 16, 32, 64 or 128, 1 (rows against streamed weights, offsets NULL), or 16, 32 or 64 with slice_columns 16 or 32, 32 or 64, and 64: tiles
- * of so many columns with K in eight slices.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K % 64 == 0, the bytes of one weight and of scale_a below 4 GiB.
+ * of so many columns with K in eight slices, or 128 with 128: tiles of 128 columns in place of 256.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K % 64 == 0, the bytes of one weight and of scale_a below 4 GiB.
  * a, w and c 16-byte, the scales and offsets 4-byte aligned.  One launch, no workspace.
  */
 typedef struct psg_blockscale_args {

@@ -85,7 +85,7 @@ def _product(**change):
 @pytest.mark.parametrize("change,code", [
     (dict(c=0), NULL), (dict(a=0), NULL), (dict(w=0), NULL), (dict(scale_a=0), NULL), (dict(scale_b=0), NULL), (dict(offsets=0), NULL), (dict(out_dtype=2), DTYPE), (dict(out_dtype=-1), DTYPE),
     (dict(M=0), SHAPE), (dict(M=(1 << 22) + 1), SHAPE), (dict(groups=0), SHAPE), (dict(groups=4097), SHAPE), (dict(groups=0, offsets=0), SHAPE), (dict(N=40), SHAPE), (dict(N=0), SHAPE), (dict(K=96), SHAPE),
-    (dict(K=0), SHAPE), (dict(N=1 << 18, K=1 << 14), SHAPE), (dict(N=1 << 24, K=64), SHAPE), (dict(N=16, K=1 << 25), SHAPE), (dict(tile_rows=48), SHAPE), (dict(tile_rows=1), SHAPE), (dict(slice_columns=16), SHAPE), (dict(tile_rows=16, slice_columns=64), SHAPE), (dict(tile_rows=128, slice_columns=64), SHAPE), (dict(tile_rows=1, slice_columns=16), SHAPE), (dict(scale_a_stride=9), SHAPE),
+    (dict(K=0), SHAPE), (dict(N=1 << 18, K=1 << 14), SHAPE), (dict(N=1 << 24, K=64), SHAPE), (dict(N=16, K=1 << 25), SHAPE), (dict(tile_rows=48), SHAPE), (dict(tile_rows=1), SHAPE), (dict(slice_columns=16), SHAPE), (dict(tile_rows=16, slice_columns=64), SHAPE), (dict(tile_rows=128, slice_columns=64), SHAPE), (dict(tile_rows=64, slice_columns=128), SHAPE), (dict(tile_rows=128, slice_columns=256), SHAPE), (dict(tile_rows=1, slice_columns=16), SHAPE), (dict(scale_a_stride=9), SHAPE),
     (dict(scale_a_stride=-1), SHAPE), (dict(K=1 << 15, M=1 << 22), SHAPE), (dict(scale_a_stride=1 << 31), SHAPE), (dict(K=256, scale_a_stride=1 << 29), SHAPE), (dict(M=1 << 22, N=1 << 12, tile_rows=16), SHAPE), (dict(M=1 << 22, N=1 << 16, K=64, groups=4096), SHAPE),
     (dict(a=0x1008), ALIGN), (dict(w=0x1008), ALIGN), (dict(c=0x1008), ALIGN), (dict(scale_b=0x1002), ALIGN), (dict(scale_a=0x1002), ALIGN), (dict(offsets=0x1002), ALIGN),
 ])

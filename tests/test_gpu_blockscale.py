@@ -17,7 +17,7 @@ DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
 HALF = {"bf16": 2.0**-8, "fp16": 2.0**-11}
 GUARD = -77.0
 AUTO, STREAM = (0, 0), (1, 0)
-WHOLE = [(16, 0), (32, 0), (64, 0), (128, 0)]  # rows of a tile, K in one piece
+WHOLE = [(16, 0), (32, 0), (64, 0), (128, 0), (128, 128)]  # rows of a tile (and 128 columns in place of 256), K in one piece
 SLICED = [(16, 16), (16, 32), (32, 32), (32, 64), (64, 64)]  # rows and columns of a tile, K in slices
 
 
@@ -112,12 +112,13 @@ def test_scales_of_a_wider_tensor(tile):
     _check_exact(_run(a, w, sa, sb, None, "bf16", tile, strided=True), a, w, sa, sb, None, "bf16")
 
 
+@pytest.mark.parametrize("tile", [(128, 0), (128, 128)])
 @pytest.mark.parametrize("steps", range(1, 15))
-def test_every_length_of_the_large_tile(steps):
+def test_every_length_of_the_large_tile(steps, tile):
     """1 to 14 steps of K, with half a step at the end and without: the loop's builds with and without checks, and its ends."""
     for k in (steps * 128 - 64, steps * 128):
         a, w, sa, sb = _operands(140, 288, k, 1, k)
-        _check_exact(_run(a, w, sa, sb, None, "bf16", (128, 0)), a, w, sa, sb, None, "bf16")
+        _check_exact(_run(a, w, sa, sb, None, "bf16", tile), a, w, sa, sb, None, "bf16")
 
 
 @pytest.mark.parametrize("tile", SLICED)
@@ -306,7 +307,7 @@ def test_refusals():
                 grouped(*good, off, 10, stream)
 
 
-@pytest.mark.parametrize("n,k,tile", [(16, 1088, AUTO), (16, 1088, STREAM), (16, 1088, (16, 0)), (16, 1088, (128, 0)), (16, 1088, (64, 64)), (528, 64, AUTO), (528, 64, STREAM), (528, 64, (64, 64))])
+@pytest.mark.parametrize("n,k,tile", [(16, 1088, AUTO), (16, 1088, STREAM), (16, 1088, (16, 0)), (16, 1088, (128, 0)), (16, 1088, (128, 128)), (16, 1088, (64, 64)), (528, 64, AUTO), (528, 64, STREAM), (528, 64, (64, 64))])
 def test_rows_past_four_gib(n, k, tile):
     """A (k = 1088) or C (n = 528) of more than 2^32 bytes: rows at the front, about the border and at the end."""
     m = 4190003
@@ -329,7 +330,7 @@ def test_rows_past_four_gib(n, k, tile):
     assert (c[m] == GUARD).all()
 
 
-@pytest.mark.parametrize("tile", [AUTO, (32, 0), (128, 0), (16, 16)])
+@pytest.mark.parametrize("tile", [AUTO, (32, 0), (128, 0), (128, 128), (16, 16)])
 def test_weights_past_four_gib(tile):
     """37 groups' weights of 5 GB: rows of the first, of those about the border and of the last."""
     groups, n, k = 37, 16400, 8128
