@@ -13,7 +13,7 @@
 // A token belongs to L lanes of a wavefront, a power of two, VPT experts to a lane; a lane's experts are of one run, so the runs' worth is one butterfly over the LG lanes of a run and their order a
 // count of better ones.  In 32 bits a value is an unsigned number that orders like the float, its last bits replaced by the expert's place in the lane; a lane sorts its own once
 // (a network of minimum and maximum), and a round is a butterfly of v_max_u32 over the token's lanes' first ones, a ballot for the first lane that holds the maximum, and a step forward in that lane.
-// Bound: launch latency for decode (1 x 256 of 8 groups: 5.9 us); for prefill the instructions, 16384 x 256 in 25.4 us, 820 vector instructions a wavefront (with all of it in 64 bits the best split
+// Bound: launch latency for decode (1 x 256 of 8 groups: 5.9 us); for prefill the instructions, 16384 x 256 in 25.4 us, 917 vector instructions a wavefront of two tokens (with all of it in 64 bits the best split
 // took 26.4, by softmax 22.4 against 18.8, and a token alone 6.8).
 #include "moe_gating.h"
 #include "moe_route.h"
