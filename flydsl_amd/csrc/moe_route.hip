@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
     fetch(row, [](T l) { return gate_to_f32<T>(l); }, x);
     if (bias) fetch(p.bias, [](float f) { return f; }, b);
 #pragma unroll
-    for (int v = 0; v < VPT; v++) x[v] = v < have && x[v] > -INFINITY ? x[v] : -INFINITY;  // (NaN too)
+    for (int v = 0; v < VPT; v++) x[v] = v < have && x[v] > -INFINITY ? x[v] + 0.0f : -INFINITY;  // (NaN too; and -0 to +0, which it equals but whose number below would be lower)
     // the score but for the softmax's sum; infinities share what there is
     auto score = [&](float l) __attribute__((always_inline)) {
         if (p.softmax) return l == (float)mx ? 1.0 : exp((double)l - mx);
