@@ -84,8 +84,8 @@ __device__ __forceinline__ void route_sort(uint32_t (&s)[VPT]) {
     }
 }
 
-// How far a score + bias in 32 bits may be from the same in 64: the exponential is off by a unit, 2^-23, and by the rounding of its argument, |a| 2^-23 of which at most a |a| exp(-|a|) <= 0.37th part, or
-// a quarter for a sigmoid, is left in the score; the sum or 1 + e, its reciprocal and their product by 2^-23 each, so a score, 1 at most, by 2^-20.9 altogether; and half a unit of the sum with the bias
+// How far a score + bias in 32 bits may be from the same in 64: the exponential is off by a unit, 2^-23, and by the rounding of its argument, |a| 2^-22.8 of which at most a |a| exp(-|a|) <= 0.37th part, or
+// a quarter for a sigmoid, is left in the score; the sum or 1 + e, its reciprocal and their product by 2^-23 each, so a score, 1 at most, by 2^-20.8 altogether; and half a unit of the sum with the bias
 __device__ __forceinline__ float route_slack(float f) { return __builtin_fmaf(fabsf(f), 0x1p-24f, 0x1p-20f); }
 
 struct Winner {
@@ -190,7 +190,16 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
             });
             const float worth = !p.top2 ? m1 : m2 == -INFINITY ? -INFINITY : bias ? m1 + m2 : score32(m1) + score32(m2);
             const bool exact = !bias && !p.top2;  // (logits: no slack, and of equal ones the lower)
-            const float slack = exact ? 0.0f : 5.0f * route_slack(worth);  // (two values a side, and the roundings of their sum and of the bound)
+            // A worth is off by what its two values are, half a unit of each and 2^-19.8 together, and by the rounding of their sum, half a unit of it: by 2^-23 of the values' magnitudes, whose sum
+            // (A) may be far above the worth's own where they cancel.  Of the token's largest A, 8 A 2^-24 + 2^-18 hold two runs' worths and the rounding of the bound (5 A 2^-24 + 2^-18.8).
+            float slack = 0.0f;
+            if (!exact) {
+                uint32_t size = run < p.groups ? __builtin_bit_cast(uint32_t, p.top2 && bias ? fabsf(m1) + fabsf(m2) : fabsf(worth)) : 0u;
+                gate_steps(sh, [&](auto S) { size = route_join<decltype(S)::value>(size, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); });
+                const float most = __builtin_bit_cast(float, size);
+                slack = __builtin_fmaf(most, 0x1p-21f, 0x1p-18f);
+                again = !(most < 0x1p100f);  // (infinite ones too, whose bounds are no numbers)
+            }
             int better = 0, rivals = 0;
             for (int r = 0; r < p.groups; r++) {
                 const float o = __shfl(worth, shift + (r << gsh), 64);
@@ -198,7 +207,7 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
                 rivals += (r != run) & (o >= worth - slack);
             }
             const bool out = better >= p.topk_groups;
-            again = !exact && run < p.groups && ((!out && rivals >= p.topk_groups) || !(fabsf(worth) < 0x1p100f));
+            again |= !exact && run < p.groups && !out && rivals >= p.topk_groups;
             if (out) {
 #pragma unroll
                 for (int v = 0; v < VPT; v++) f[v] = -INFINITY;
