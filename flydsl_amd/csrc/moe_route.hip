@@ -89,9 +89,9 @@ __device__ __forceinline__ void route_sort(uint32_t (&s)[VPT]) {
 __device__ __forceinline__ float route_slack(float f) { return __builtin_fmaf(fabsf(f), 0x1p-24f, 0x1p-20f); }
 
 struct Winner {
-    double c;      // what was compared, in 64 bits
-    float weight;  // score
-    int index;     // negative: not to be taken, but nothing else was left
+    double c;       // what was compared
+    double weight;  // score
+    int index;      // negative: not to be taken, but nothing else was left
 };
 
 template <typename T, int VPT>
@@ -158,11 +158,11 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
         inv = 1.0 / sum;
     }
     // what the winner of expert e is compared by, and its score
-    auto look = [&](int e, double& c, float& weight) __attribute__((always_inline)) {
+    auto look = [&](int e, double& c, double& weight) __attribute__((always_inline)) {
         const float l = gate_to_f32<T>(row[e]);
         const double s = score(l) * inv;
         c = bias ? s + (double)p.bias[e] : (double)l;
-        weight = (float)s;
+        weight = s;
     };
 
     const int shift = (int)threadIdx.x & 63 & ~(L - 1);
@@ -235,11 +235,10 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
         wave_lds_order();  // (a token's lanes are neighbours in one wavefront)
         for (int k = gl; k < p.topk; k += L) {
             Winner& w = mine[k];
-            double c;
-            float weight;
+            double c, weight;
             look(w.index & 0x7FFFFFFF, c, weight);
             w.c = w.index < 0 ? NO : c;
-            w.weight = w.index < 0 ? 0.0f : weight;
+            w.weight = w.index < 0 ? 0.0 : weight;
         }
         wave_lds_order();
         for (int k = gl; k < p.topk; k += L) {
@@ -306,22 +305,23 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
         wave_lds_order();
         for (int k = gl; k < p.topk; k += L) {
             Winner& w = mine[k];
-            double c64;
-            float weight;
-            look(w.index & 0x7FFFFFFF, c64, weight);
-            w.weight = w.index < 0 ? 0.0f : weight;
+            double unused, weight;
+            look(w.index & 0x7FFFFFFF, unused, weight);
+            w.weight = w.index < 0 ? 0.0 : weight;
         }
         wave_lds_order();
     }
-    float all = 0.0f;
-    if (p.renorm)
+    double factor = p.scale;  // (weights in 64 bits until they are stored, one rounding)
+    if (p.renorm) {
+        double all = 0.0;
         for (int k = 0; k < p.topk; k++) all += mine[k].weight;
-    const float over = p.renorm ? fmaxf(all, 1e-20f) : 1.0f;
+        factor /= __builtin_fmax(all, 1e-20);
+    }
     if (live) {
         for (int k = gl; k < p.topk; k += L) {
             const Winner w = mine[k];
             p.indices[(size_t)t * p.topk + k] = w.index & 0x7FFFFFFF;
-            p.weights[(size_t)t * p.topk + k] = w.weight / over * p.scale;
+            p.weights[(size_t)t * p.topk + k] = (float)(w.weight * factor);
         }
     }
 }

@@ -8,7 +8,7 @@ order found (best first).
 
 ``s`` is the sigmoid of the logits, or their softmax over the experts; ``c = s + bias`` is what is compared, without a bias the logits themselves, which order like ``s``.  The experts lie in ``groups``
 runs of ``num_experts / groups``; a group is worth the sum of its two best ``s + bias`` (``group_score="top2"``) or its best ``c`` (``"max"``), the ``topk_groups`` best groups are kept, and of their experts the ``topk`` best.  The weights are ``s`` of these, without the
-bias; with ``renormalize`` divided by ``max(their sum, 1e-20)``; then times ``scale``.  Scores and comparisons are in 64 bits, and of equal ones the lower index comes first.
+bias; with ``renormalize`` divided by ``max(their sum, 1e-20)``; then times ``scale``.  Scores, comparisons and weights are in 64 bits, the weights rounded once, and of equal ones the lower index comes first.
 
 A logit of -inf masks its expert, a logit of NaN or a ``c`` that is NaN too: such an expert, or one of a group that is not kept, is taken only when nothing else is left, the lowest index first
 and with weight 0, so a token always has ``topk`` different experts.

@@ -607,7 +607,7 @@ int psg_gemm_blockscale(const psg_blockscale_args *args, void *stream);
  *   s = sigmoid(x) (scores 0) or softmax(x) over the experts (scores 1); c = s + bias, with bias NULL c = x itself, which orders like s
  *   the experts lie in `groups` runs of equal length, a run is worth the sum of its two best s + bias (group_score 1) or its best c (0), and the topk_groups best runs are kept
  *   indices = the topk best c of the kept runs in their order, weights = s of these; renormalize = 1: divided by max(their sum, 1e-20); times scale
- * Of equal ones the lower index comes first; scores and comparisons are in 64 bits, weights in fp32.  A logit of -Inf or NaN, or a c that is NaN, counts as -Inf: such an expert, like one of a
+ * Of equal ones the lower index comes first; scores, comparisons and weights are in 64 bits, and the weights rounded to fp32 once.  A logit of -Inf or NaN, or a c that is NaN, counts as -Inf: such an expert, like one of a
  * run that is not kept, is taken (lowest index first) when nothing else is left, with weight 0, so that the indices of a token are always topk different ones.  A run with
  * one such c among its two best is worth -Inf.
  * gating [tokens, experts] row-major, dtype 0 = fp32, 1 = bf16, 2 = fp16; bias [experts] fp32; weights [tokens, topk] fp32, indices [tokens, topk] int32.

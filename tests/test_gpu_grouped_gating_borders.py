@@ -1,5 +1,5 @@
-"""GPU tests of the routing by groups where its choice in 32 bits meets its definition in 64: zeros of both signs at the border of the top-k, and
-groups whose two best cancel.
+"""GPU tests of the routing by groups where its 32 bits meet its definition in 64: zeros of both signs at the border of the top-k, groups whose two
+best cancel, and the weights.
 
 Expected experts come from the definition in 64 bits by stable sorts, lower index first of equal ones, and have to be equal.
 """
@@ -96,3 +96,18 @@ def test_one_group_far_from_the_others(scores):
         bias[24:32] = -size
         bias[26] = size
         assert torch.equal(_launch(x, bias, 8, scores=scores, groups=8, topk_groups=4)[1], _by_group_sums(x, bias, 8, scores, 8, 4))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scores,renormalize", [("sigmoid", True), ("sigmoid", False), ("softmax", True), ("softmax", False)])
+@pytest.mark.parametrize("t,e,groups,kept,topk", [(40, 256, 8, 4, 8), (9000, 256, 8, 4, 8), (33, 1024, 1, 1, 32), (300, 8, 1, 1, 8), (7, 1023, 33, 5, 17), (200, 160, 8, 3, 1)])
+def test_weights_are_rounded_once(t, e, groups, kept, topk, scores, renormalize, dtype):
+    """Scores, their sum, the quotient and the product with the scale in 64 bits, one rounding to 32: half a unit, 2^-24 of the value, and some 64 units of 64 bits, 2^-46, for all that is in front of it."""
+    g = torch.Generator().manual_seed(t + e)
+    x = (1.5 * torch.randn(t, e, generator=g)).to(DT[dtype]).float()
+    bias = 0.1 * torch.randn(e, generator=g)
+    w, ids = _launch(x, bias, topk, dtype, scores=scores, groups=groups, topk_groups=kept, group_score="max" if topk == 1 else "top2", renormalize=renormalize, scale=2.5)
+    want = _scores(x, scores).gather(1, ids)
+    if renormalize:
+        want = want / want.sum(1, keepdim=True)
+    assert ((w.double() - 2.5 * want).abs() <= (2.0**-24 + 2.0**-46) * 2.5 * want).all()
