@@ -36,19 +36,20 @@ __device__ __forceinline__ float silu_near(float g) {
     return g * r;
 }
 
-// g sigmoid(g) for every g, off by a few units in the last place: with z = exp(-|g|), sigmoid is 1 / (1 + z) or z / (1 + z), and exponents below the normal range
-// in two steps, as the exponential instruction has no subnormal results.
-__device__ __forceinline__ float silu(float g) {
+// g sigmoid(g) u for every g, off by a few units in the last place: with z = exp(-|g|), sigmoid is 1 / (1 + z) or z / (1 + z).  Below -83 sigmoid is z itself, from -87 on below the normal range, where the
+// exponential instruction has no results and fp32 no precision; but u can be 2^127 and the product an ordinary number.  There z is kept times 2^160 until u has multiplied it, half of that taken off u, half
+// off the product: z 2^160 is a normal number down to exp(-198), 2^-286, whose product with every u is nothing; and where u 2^-80 is subnormal the product is.
+__device__ __forceinline__ float silu_times(float g, float u) {
     constexpr float L = 1.44269502162933349609375f, L2 = 1.92596298909109e-8f, LN2 = 0.693147180559945f;  // L + L2 = log2(e)
-    const float a = fminf(fabsf(g), 200.0f);
+    const float a = fminf(fabsf(g), 300.0f);
     const float hi = a * L, lo = __builtin_fmaf(a, L2, __builtin_fmaf(a, L, -hi));
-    const bool tiny = hi > 120.0f;
-    float z = __builtin_amdgcn_exp2f((tiny ? 64.0f : 0.0f) - hi);
-    z = __builtin_fmaf(-lo * LN2, z, z) * (tiny ? 0x1p-64f : 1.0f);
-    const float d = 1.0f + z;
+    const bool far = hi > 120.0f && g < 0.0f;
+    float z = __builtin_amdgcn_exp2f((far ? 160.0f : 0.0f) - hi);
+    z = __builtin_fmaf(-lo * LN2, z, z);
+    const float d = 1.0f + (far ? 0.0f : z), half = far ? 0x1p-80f : 1.0f;
     float r = __builtin_amdgcn_rcpf(d);
     r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
-    return g * ((g < 0.0f ? z : 1.0f) * r);
+    return g * ((g < 0.0f ? z : 1.0f) * r) * (u * half) * half;
 }
 
 // WHOLE: rows are whole vectors of eight
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(256) k_quant_block(QuantBlockParams p, int chu
             for (int e = 0; e < 8; e++) v[e] = silu_near(v[e]) * w[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = silu(v[e]) * w[e];
+            for (int e = 0; e < 8; e++) v[e] = silu_times(v[e], w[e]);
         }
     }
     if (!in) {
