@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
     constexpr int ROWB = TN * 2, GR = ROWB / 16;                           // bytes and 16-byte granules of a row of the tile of C
     constexpr int SUMS = KS > 1 ? 4 * MR * NR * 1024 : 0;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * KS * TILE > SUMS ? 2 * KS * TILE : SUMS];
-    __shared__ float s_scale[BLOCKED ? 2 * KS * BM : 1];  // a stage's products of row and column scale
+    __shared__ float s_scale[BLOCKED ? 2 * BM : 1];  // a stage's products of row and column scale
     const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int slice = KS > 1 ? wave : 0, block = KS > 1 ? 0 : wave;
     GroupTile t;
@@ -50,23 +50,22 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
         a_lds[j] = sub < KS ? sub * TILE + lds_off(row, kc) : -1;
     }
     v4i ar[SETS][A_LOADS], wlo[SETS][NR], whi[SETS][NR];
-    // block scales of a stage: a row of a slice a thread, and that of the tile's columns, which lie in one block (rows past the group's end have others' scales, and zeros behind the array)
-    static_assert(KS * BM <= 64, "the scales of a stage are a wavefront's");
+    // block scales of a stage: a row a thread, and that of the tile's columns, which lie in one block (rows past the group's end have others' scales, and zeros behind the array)
+    static_assert(!BLOCKED || (KS == 1 && BM <= 64), "the scales of a stage are a wavefront's; K in slices is gemm_blockscale.hip's");
     float sar[SETS], sbr[SETS];
-    const uint32_t sa_off = ((uint32_t)(tid / BM) * g.sa_stride + (uint32_t)(tid % BM)) * 4u;
     const uint32_t KB = (K + TK - 1) / TK, NB = ((uint32_t)p.N + 127u) / 128u;
     const __amdgpu_buffer_rsrc_t rsa = make_rsrc(BLOCKED ? p.sa + t.row : nullptr, BLOCKED ? ((uint64_t)(KB - 1) * g.sa_stride + (uint32_t)(p.M - t.row)) * 4ull : 0ull);
     const __amdgpu_buffer_rsrc_t rsb = make_rsrc(BLOCKED ? p.sb + ((uint64_t)t.e * NB + (uint32_t)n0 / 128u) * KB : nullptr, BLOCKED ? KB * 4ull : 0ull);
     auto load_s = [&](int kt, int set) __attribute__((always_inline)) {
         if constexpr (BLOCKED) {
-            const bool has = tid < KS * BM && (uint32_t)kt * KS + (uint32_t)(tid / BM) < KB;
-            sar[set] = __int_as_float(buf_load4(rsa, has ? sa_off : OOB, kt < KT ? (uint32_t)kt * (KS * 4u) * g.sa_stride : 0u));
-            sbr[set] = __int_as_float(buf_load4(rsb, has ? (uint32_t)(tid / BM) * 4u : OOB, kt < KT ? (uint32_t)kt * (KS * 4u) : 0u));
+            const bool has = tid < BM && kt < KT;
+            sar[set] = __int_as_float(buf_load4(rsa, has ? (uint32_t)tid * 4u : OOB, kt < KT ? (uint32_t)kt * 4u * g.sa_stride : 0u));
+            sbr[set] = __int_as_float(buf_load4(rsb, has ? 0u : OOB, kt < KT ? (uint32_t)kt * 4u : 0u));
         }
     };
     auto store_s = [&](int stage, int set) __attribute__((always_inline)) {
         if constexpr (BLOCKED) {
-            if (tid < KS * BM) s_scale[stage * KS * BM + tid] = sar[set] * sbr[set];
+            if (tid < BM) s_scale[stage * BM + tid] = sar[set] * sbr[set];
         }
     };
     __builtin_assume(KT > 0);
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MR <= 
                 constexpr int i = decltype(I)::value, mi = i / NR, ni = i % NR;
                 if constexpr (ni == 0) alo[mi & 1] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, lg)), ahi[mi & 1] = *reinterpret_cast<const v4i*>(mine + lds_off(mi * 16 + li, 4 + lg));
                 add_part(std::integral_constant<int, (i + MR * NR - BEHIND) % (MR * NR)>{});
-                if constexpr (ni == 0) part_scale[mi % SCALES] = s_scale[(S * KS + slice) * BM + mi * 16 + li];
+                if constexpr (ni == 0) part_scale[mi % SCALES] = s_scale[S * BM + mi * 16 + li];
                 part[i % BEHIND] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(wlo[set][ni], whi[set][ni], 0, 1, 2, 3, 4, 5, 6, 7),
                                                                                     __builtin_shufflevector(alo[mi & 1], ahi[mi & 1], 0, 1, 2, 3, 4, 5, 6, 7), (v4f){0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
             });
