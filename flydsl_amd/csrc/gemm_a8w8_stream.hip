@@ -434,7 +434,7 @@ hipError_t psg_launch_a8w8_stream(const A8W8Params& p, int kind, int store, hipS
 }
 
 // The block-scaled product on the same plan, and its estimated time in us: a step of a wavefront takes 0.21 for every 16 rows and 0.039 for every window, a workgroup's bytes 0.027 a KB of its columns'
-// weights; W from memory, for every 64 rows, 5.8 TB/s (fitted to 1,700 products of 1 to 8,192 rows; off by 6 % at the median, 18 at nine of ten).
+// weights; W from memory, for every 64 rows, 5.8 TB/s (fitted to some of 1 to 8,192 rows; on the 1,700 of profiles/block_scaled_times.csv it is off by 6 % at the median, 17 at nine of ten).
 double psg_blockscale_stream_us(int M, int N, int K) {
     const StreamPlan s = plan_stream(M, N, K);
     const int steps = (K + 127) / 128, groups = (M + 63) / 64, ch = s.nwaves == 8 ? 2 : 4, rows = M < 64 ? M : 64, gpw = s.nwaves / s.ks;

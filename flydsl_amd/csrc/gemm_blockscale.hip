@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(256, 2) k_block_square(A8W8Params p, GroupPara
 
 // The way of the least estimated time, in us.  Of `load` tiles a CU: a tile's steps when it is alone on its CU, longer as more CUs are at work; a CU's steps and tile ends where it has many (whole rounds of
 // small tiles, up to four); W from memory.
-// The constants are fitted to the times of 3,400 products of 1 to 32,768 rows on 1 to 128 groups (128 x 128 tiles to 6,000 others); on 4,900 more the choice is 3.5 % slower than the best way dense and
-// 2.8 % grouped, in the geometric mean (the choice for one scale a row, psg_grouped_plan, 15 and 7).  Slices with 16 x 64, 32 x 16, 64 x 16 and 64 x 32 tiles win 0.2 % more together and are not built.
+// The constants are fitted to the times of 3,400 products of 1 to 32,768 rows on 1 to 128 groups (128 x 128 tiles to 6,000 others), which are not kept; on 4,800 more (profiles/block_scaled_times.csv, every way's
+// time and the choice) it is 3.5 % slower than the best way dense and 2.8 % grouped, in the geometric mean (the choice for one scale a row, psg_grouped_plan, 15 and 7).  Slices with 16 x 64, 32 x 16, 64 x 16 and 64 x 32 tiles win 0.2 % more together and are not built.
 // us, whole K on 16, 32, 64, 128 rows / slices on 16 x 16, 16 x 32, 32 x 32, 32 x 64, 64 x 64 / streamed: 346 x 352 x 11328 20.9, 23.3, 44.8, 69.7 / 12.4, 9.6, 11.7, 16.2, 22.3 / 19.1; 201 x 752 x 10624 21.9, 23.5, 41.9, 71.7 / 15.4,
 // 14.0, 11.3, 15.5, 20.6 / 15.1; 775 x 624 x 13184 35.8, 31.5, 52.2, 94.9 / 41.0, 34.3, 26.1, 21.1, 28.4 / -; 127 x 5104 x 2944 12.7, 11.0, 15.1, 21.0 / 15.9, 13.3, 10.9, 12.0, 9.5 / -; 13 x 1616 x 16256 35.7, 38.1, 63.0, 129 /
 // 15.3, 17.4, 18.1, 26.9, 30.6 / 10.4; 8 rows on 8, 1552 x 5504, 12.2, 13.6, 24.1, 33.6 / 6.5, 6.8, 7.3, 8.8, 10.7; 620 x 1760 x 832 7.7, 6.4, 7.2, 9.9 / 14.9, 9.9, 8.8, 10.0, 9.4.

@@ -13,8 +13,9 @@
 // A token belongs to L lanes of a wavefront, a power of two, VPT experts to a lane; a lane's experts are of one run, so the runs' worth is one butterfly over the LG lanes of a run and their order a
 // count of better ones.  In 32 bits a value is an unsigned number that orders like the float, its last bits replaced by the expert's place in the lane; a lane sorts its own once
 // (a network of minimum and maximum), and a round is a butterfly of v_max_u32 over the token's lanes' first ones, a ballot for the first lane that holds the maximum, and a step forward in that lane.
-// Bound: launch latency for decode (1 x 256 of 8 groups: 5.9 us); for prefill the instructions, 16384 x 256 in 25.4 us, 917 vector instructions a wavefront of two tokens (with all of it in 64 bits the best split
-// took 26.4, by softmax 22.4 against 18.8, and a token alone 6.8).
+// Weights stay in 64 bits until they are stored.
+// Bound: launch latency for decode (1 x 256 of 8 groups: 6.1 us); for prefill the instructions, 16384 x 256 in 25.5 us, 940 vector instructions a wavefront of two tokens (with all of it in 64 bits the best split
+// took 26.4, by softmax 22.4 against 19.1, and a token alone 6.8).
 #include "moe_gating.h"
 #include "moe_route.h"
 #include <type_traits>
@@ -352,9 +353,11 @@ inline int up2(int v) {
 hipError_t psg_launch_moe_route(RouteParams p, int dtype, hipStream_t stream) {
     if (p.topk_groups >= p.groups) p.groups = p.topk_groups = 1;  // every run is kept: one run
     const int size = p.experts / p.groups;
-    // Four values a lane (the shortest way through one token) while the chip holds all the wavefronts at once, 8192 of them: 1 x 256 in 5.9 us against 7.6 with eight and 10.3 with sixteen,
-    // 1024 x 256 7.9 / 9.2 / 13.5, 4096 x 256 11.1 / 12.7 / 18.5.  Beyond, the instructions count, and two tokens a wavefront share them: 16384 x 256 26.2 / 25.4 / 28.9 with groups and
-    // 23.8 / 18.8 / 19.5 by softmax.  And more where 64 lanes would not hold a token: with up to 64 runs of a power of two of lanes each, 32 hold 1024 experts in any division.
+    // Four values a lane (the shortest way through one token) while the chip holds all the wavefronts at once, 8192 of them: 1 x 256 in 6.7 us against 8.4 with eight and 11.5 with sixteen,
+    // 1024 x 256 7.7 / 10.6 / 14.7, 4096 x 256 11.7 / 12.9 / 16.0.  Beyond, the instructions count, and two tokens a wavefront share them: 16384 x 256 26.7 / 26.1 / 28.6 with groups and
+    // 24.2 / 19.1 / 19.1 by softmax.  And more where 64 lanes would not hold a token: with up to 64 runs of a power of two of lanes each, 32 hold 1024 experts in any division.  Sixteen (five
+    // wavefronts a SIMD) take 9.4 us for 1 x 1024, 26.6 for 4096 x 1024 and 68.6 for 16384 x 1024, thirty-two (three, and 128 of the scalars kept in vector registers) 15.7 / 36.0 / 81.2 there and 14.8 / 42.3 / 107
+    // for 33 groups of 31, which need them.
     auto lanes = [&](int vpt) { return up2(p.groups) * up2((size + vpt - 1) / vpt); };
     int vpt = (int64_t)p.tokens * lanes(4) > 8192 * 64 ? 8 : 4;
     while (lanes(vpt) > 64) vpt <<= 1;

@@ -7,7 +7,7 @@
 // A block belongs to 16 lanes, eight columns each: its maximum is four exchanges inside a row of lanes (DPP), no LDS and no barrier.  A wavefront takes 512 columns of one row, which it
 // reads as one kilobyte; the other wavefronts hide its wait (four rows a wavefront, all loads ahead, were 2 to 30 % slower from 256 x 4096 to 8192 x 4096).
 // The scales lie block by block, so that a tile of a product finds those of its rows together: its lanes fetch a block's scales of 64 rows as 256 bytes in a row.
-// Bound: HBM, 8192 x 8192 of bf16 in 39.8 us (5.05 TB/s, a copy's rate; fp32 57.6 us, 5.8 TB/s), gated 68.0 us (4.94 TB/s; 79 with the form of silu that every g needs, the instructions');
+// Bound: HBM, 8192 x 8192 of bf16 in 39.8 us (5.05 TB/s, a copy's rate; fp32 57.6 us, 5.8 TB/s), gated 68.0 us (4.94 TB/s; 96 where most groups of eight have a g beyond 83 and take the form that every g needs, the instructions');
 // of few rows the launch, 256 x 4096 in 3.1 us.
 #include "psg_common.h"
 #include "quant_rows.h"

@@ -552,7 +552,7 @@ int psg_gemm_grouped(const psg_grouped_args *args, void *stream);
  *   q = y / scale, rounded once, to nearest even.  NaN -> 0 and +-Inf -> +-448 in front of the maximum, as in psg_quant_pertoken
  * x rows of dim (gated: 2 * dim) elements, x_stride elements apart (0 = dense, else at least a row), at addresses and strides that need only be multiples of an element; q [rows, dim] dense; scale
  * [ceil(dim / 128)][rows], scale_stride floats from a block to the next (0 = rows, else at least rows).  x_dtype 0 = fp32, 1 = bf16, 2 = fp16.  rows = 0 launches nothing.
- * dim <= 2^24, rows < 2^31.
+ * dim <= 2^24, rows < 2^31.  q and scale overlap neither x nor each other.
  */
 typedef struct psg_quant_block_args {
     const void *x;
@@ -578,7 +578,7 @@ int psg_quant_block(const psg_quant_block_args *args, void *stream);
  *   offsets as in psg_gemm_grouped, with all that is said there about rows outside of the groups
  * A block's products are summed in fp32 (the matrix instruction adds eight consecutive ones in a step and drops what lies more than 13 bits below the largest's exponent, as in every fp8 product of
  * this library), and its sum times scale_a * scale_b, itself rounded to fp32, is added to those of the blocks in front of it with one rounding: the product of two scales
- * that meet has to be a normal number of fp32 for the result to have its precision.  Within a call every row is summed in the same order; a call of other sizes may take other tiles, and with
+ * that meet has to be a normal number of fp32 for the result to have its precision (below, it loses bits; an infinite one makes an infinity of a block's sum, and NaN of a sum of zero).  Within a call every row is summed in the same order; a call of other sizes may take other tiles, and with
  * few of them slices of K, whose sums differ in the last places.
  * tile_rows 0 (the library's choice by M, N, K and groups); for tests 16, 32, 64 or 128, 1 (rows against streamed weights, offsets NULL), or 16, 32 or 64 with slice_columns 16 or 32, 32 or 64, and 64: tiles
  * of so many columns with K in eight slices, or 128 with 128: tiles of 128 columns in place of 256.  1 <= M <= 2^22, 1 <= groups <= 4096, N % 16 == 0, K % 64 == 0, the bytes of one weight and of scale_a below 4 GiB.
