@@ -14,7 +14,7 @@
 // count of better ones.  In 32 bits a value is an unsigned number that orders like the float, its last bits replaced by the expert's place in the lane; a lane sorts its own once
 // (a network of minimum and maximum), and a round is a butterfly of v_max_u32 over the token's lanes' first ones, a ballot for the first lane that holds the maximum, and a step forward in that lane.
 // Weights stay in 64 bits until they are stored.
-// Bound: launch latency for decode (1 x 256 of 8 groups: 6.1 us); for prefill the instructions, 16384 x 256 in 25.5 us, 940 vector instructions a wavefront of two tokens (with all of it in 64 bits the best split
+// Bound: launch latency for decode (1 x 256 of 8 groups: 6.1 us); for prefill the instructions, 16384 x 256 in 25.5 us, 934 vector instructions a wavefront of two tokens (with all of it in 64 bits the best split
 // took 26.4, by softmax 22.4 against 19.1, and a token alone 6.8).
 #include "moe_gating.h"
 #include "moe_route.h"
@@ -191,15 +191,18 @@ __global__ void __launch_bounds__(256) k_route(RouteParams p) {
             });
             const float worth = !p.top2 ? m1 : m2 == -INFINITY ? -INFINITY : bias ? m1 + m2 : score32(m1) + score32(m2);
             const bool exact = !bias && !p.top2;  // (logits: no slack, and of equal ones the lower)
-            // A worth is off by what its two values are, half a unit of each and 2^-19.8 together, and by the rounding of their sum, half a unit of it: by 2^-23 of the values' magnitudes, whose sum
-            // (A) may be far above the worth's own where they cancel.  Of the token's largest A, 8 A 2^-24 + 2^-18 hold two runs' worths and the rounding of the bound (5 A 2^-24 + 2^-18.8).
+            // A worth is off by what its two values are, half a unit of each and 2^-19.8 together, and by the rounding of their sum, half a unit of it.  The values' magnitudes together are the sum's and, where
+            // their signs differ, twice the smaller one (h), which may be far above the sum.  For two runs with |o| <= 2 |worth| that is (8 |worth| + 4 h) 2^-24 + 2^-18.8 at most, the rounding of the
+            // bound in it; where |o| is larger, the two are half of it apart.  h is the token's largest: a run that a bias of -10^9 masks has
+            // none, and keeps the others' bounds as they are (16384 x 256 with one such run 26.1 us; with the largest sum of magnitudes as everyone's bound 41, all tokens in 64 bits).
             float slack = 0.0f;
             if (!exact) {
-                uint32_t size = run < p.groups ? __builtin_bit_cast(uint32_t, p.top2 && bias ? fabsf(m1) + fabsf(m2) : fabsf(worth)) : 0u;
-                gate_steps(sh, [&](auto S) { size = route_join<decltype(S)::value>(size, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); });
-                const float most = __builtin_bit_cast(float, size);
-                slack = __builtin_fmaf(most, 0x1p-21f, 0x1p-18f);
-                again = !(most < 0x1p100f);  // (infinite ones too, whose bounds are no numbers)
+                const float both = p.top2 && bias ? fmaxf(fminf(m1, -m2), 0.0f) : 0.0f;
+                uint32_t h = __builtin_bit_cast(uint32_t, both);
+                if (__ballot(both > 0.0f) != 0) gate_steps(sh, [&](auto S) { h = route_join<decltype(S)::value>(h, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); });
+                const float most = __builtin_bit_cast(float, h);
+                slack = __builtin_fmaf(fabsf(worth), 0x1p-20f, __builtin_fmaf(most, 0x1p-21f, 0x1p-18f));
+                again = (run < p.groups && !(fabsf(worth) < 0x1p100f)) || !(most < 0x1p100f);  // (infinite ones too, whose bounds are no numbers)
             }
             int better = 0, rivals = 0;
             for (int r = 0; r < p.groups; r++) {

@@ -98,6 +98,19 @@ def test_one_group_far_from_the_others(scores):
         assert torch.equal(_launch(x, bias, 8, scores=scores, groups=8, topk_groups=4)[1], _by_group_sums(x, bias, 8, scores, 8, 4))
 
 
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("first", [24, 25, 31])
+@pytest.mark.parametrize("mask", [-30.0, -1e4, -1e9, -1e37])
+def test_experts_masked_by_their_bias(mask, first, scores):
+    """A run whose experts a bias masks, all of them, all but one, and one of them; the others close to each other and not."""
+    g = torch.Generator().manual_seed(first)
+    bias = 0.1 * torch.randn(64, generator=g)
+    bias[first:32] = mask
+    for spread in (1e-5, 1.5):
+        x = 0.3 + spread * torch.randn(400, 64, generator=g)
+        assert torch.equal(_launch(x, bias, 8, scores=scores, groups=8, topk_groups=4)[1], _by_group_sums(x, bias, 8, scores, 8, 4))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("scores,renormalize", [("sigmoid", True), ("sigmoid", False), ("softmax", True), ("softmax", False)])
 @pytest.mark.parametrize("t,e,groups,kept,topk", [(40, 256, 8, 4, 8), (9000, 256, 8, 4, 8), (33, 1024, 1, 1, 32), (300, 8, 1, 1, 8), (7, 1023, 33, 5, 17), (200, 160, 8, 3, 1)])
